@@ -67,6 +67,8 @@ int phc_version(void);                       /* PHC_ABI_VERSION of the loaded li
 #define PHC_IDX_ERR_ATOM 2         /* integer node feature outside its vocabulary (phc_encode_fwd)             */
 #define PHC_IDX_ERR_BOND 4         /* integer edge feature outside its vocabulary (packed codes / enc kernels) */
 #define PHC_IDX_ERR_SEGMENT 8      /* segment id (batch vector) outside [0, num_segments)                      */
+#define PHC_IDX_ERR_TOKEN 32       /* token outside its embedding table (phc_embedding_fwd)                    */
+#define PHC_IDX_ERR_TARGET 64      /* target outside the vocabulary (phc_linear_xent_fwd)                      */
 #define PHC_ERR_RENDEZVOUS 16      /* a fused launch's grid-wide exchange timed out (workgroups not co-resident):
                                     * its outputs are invalid (phc_downstream_fwd / _bwd poll loops are bounded)        */
 int phc_set_error_word(int device, int32_t *dev_word);
@@ -1210,6 +1212,65 @@ size_t phc_phm_weight_reg_ws_bytes(void);
 int phc_phm_weight_reg(const float *const *W, float *const *dW, const int32_t *n, const int32_t *cells, int num_jobs, float coef,
                        int p, float *reg_out, float *loss_inout, void *ws, size_t ws_bytes, void *stream);
 
+/* ------------------------------------------------------------------------- *
+ * Large vocabularies: lookup, loss, gradient norm.  These take fp32 and 16-bit tensors (PHC_DTYPE_*, one type per call unless a
+ * comment says otherwise); sums, statistics and norms are fp32 or fp64 in every case, results are rounded once.  Additions to ABI 8.
+ * ------------------------------------------------------------------------- */
+#define PHC_DTYPE_F32 0
+#define PHC_DTYPE_BF16 1
+#define PHC_DTYPE_F16 2
+
+/* out[i, :] = scale * weight[tokens[i], :]   (out dense [N, D]; weight rows ldw elements apart).  A token outside [0, V) reads row 0
+ * and sets PHC_IDX_ERR_TOKEN.  N <= 2^28, V <= 2^30, D <= 2^20. */
+int phc_embedding_fwd(const int64_t *tokens, const void *weight, int64_t N, int64_t V, int64_t D, int64_t ldw, int dtype, float scale,
+                      void *out, void *stream);
+/* dW[v, :] = scale * sum over i with tokens[i] = v of dy[i, :], for every v (dense [V, D], rows without a token zero); row padding_idx
+ * is zero (negative: none).  Tokens outside [0, V) count as 0, as in the lookup.  Terms are added in a fixed order: bitwise
+ * reproducible.  dy rows are ldy elements apart.  ws: phc_embedding_bwd_ws_bytes(N, V, D) bytes, 16-byte aligned, scratch. */
+size_t phc_embedding_bwd_ws_bytes(int64_t N, int64_t V, int64_t D);
+int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t V, int64_t D, int64_t ldy, int dtype, float scale,
+                      int64_t padding_idx, void *dW, void *ws, size_t ws_bytes, void *stream);
+
+/* Softmax cross entropy of logits = x . W^T + bias over the vocabulary, the logits never in memory as a whole:
+ *   loss_i = logsumexp_v logits[i, v] - logits[i, target_i],   0 where target_i = ignore_index
+ * x [N, D] (rows ldx apart), W [V, D] (rows ldw apart), bias [V] or NULL, target int64 [N].  A target outside [0, V) counts as 0 and
+ * sets PHC_IDX_ERR_TARGET.  A bias of -inf takes a column out.  fp32 operands are expected to be finite: they are multiplied as sums of
+ * three 16-bit terms (accuracy of fp32).  Bitwise reproducible.
+ *   fwd writes loss ([N], or one value for sum and mean; the mean of no rows is NaN), lse [N] and stat {sum, rows that count};
+ *   bwd reads the forward's lse and stat and dloss (fp32, [N] or one value), and writes whichever of dx [N, D], dW [V, D], db [V]
+ *   (dense, of the inputs' type) is not NULL.  Rows that do not count have a zero gradient, whatever x holds there.
+ * The backward walks the vocabulary in pieces of `piece` columns (0: chosen so that a piece's gradients fit the last-level cache).
+ * N, V, ldx, ldw <= 2^22, D <= 2^20, all >= 1.  ws: phc_linear_xent_ws_bytes(desc, backward) bytes, 256-byte aligned, scratch. */
+#define PHC_REDUCE_NONE 0
+#define PHC_REDUCE_SUM 1
+#define PHC_REDUCE_MEAN 2
+typedef struct phc_linear_xent_desc {
+    int64_t N, V, D, ldx, ldw, ignore_index, piece;
+    int32_t dtype, reduction;
+    const void *x, *W, *bias;
+    const int64_t *target;
+    float *loss, *lse, *stat;
+    const float *dloss;
+    void *dx, *dW, *db;
+    void *ws;
+    size_t ws_bytes;
+} phc_linear_xent_desc;                     /* the struct is HOST memory, its pointers device memory */
+size_t phc_linear_xent_ws_bytes(const phc_linear_xent_desc *desc, int backward);
+int phc_linear_xent_fwd(const phc_linear_xent_desc *desc, void *stream);
+int phc_linear_xent_bwd(const phc_linear_xent_desc *desc, void *stream);
+
+/* The norm over n tensors together (any element-aligned addresses, types mixed), and the tensors scaled to a bound:
+ *   norm = (sum g^2)^(1/2) | sum |g| | max |g|;   coef = min(1, max_norm / (norm + 1e-6));   out[i] = coef * grads[i]
+ * norm_coef: device floats {norm, coef}.  out = NULL: the norm only.  out[i] may be grads[i] (same type: in place; nothing is written
+ * when every tensor is in place and coef is 1); any other overlap of a result with a result or an input is refused.  grads, numel, dtype, out,
+ * out_dtype are HOST arrays of n entries, consumed at call time.  Sums in fp64 in a fixed order.  A norm that is not finite makes coef 0 or
+ * NaN, as the formula says.  ws: phc_grad_norm_ws_bytes bytes, 8-byte aligned, scratch. */
+#define PHC_NORM_L2 0
+#define PHC_NORM_L1 1
+#define PHC_NORM_MAX 2
+size_t phc_grad_norm_ws_bytes(int n, const int64_t *numel);
+int phc_grad_norm_clip(int n, const void *const *grads, const int64_t *numel, const int32_t *dtype, int norm_kind, double max_norm,
+                       void *const *out, const int32_t *out_dtype, float *norm_coef, void *ws, size_t ws_bytes, void *stream);
 
 /* ------------------------------------------------------------------------- *
  * Opt-in launch profiler (process-global).  When enabled every kernel launch

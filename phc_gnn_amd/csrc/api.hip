@@ -36,6 +36,8 @@ static const char *const kKernelNames[K_NUM_KERNELS] = {
     "pack_edge_codes", "aggregate_softmax_fwd", "aggregate_softmax_bwd",
     "bce_masked_fwd", "bce_masked_bwd", "gated_pool_fwd", "gated_pool_bwd", "clip_adam", "small_linear", "sum_n",
     "downstream_fwd", "downstream_bwd", "phm_gemm_ag_fwd",
+    "embedding_fwd", "embedding_sort", "embedding_bwd", "grad_norm", "grad_scale", "xent_logits", "xent_rows", "xent_dlogits", "xent_dx",
+    "xent_dw", "xent_layout",
 };
 
 // ---- profiler ------------------------------------------------------------------

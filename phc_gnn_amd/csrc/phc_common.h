@@ -96,6 +96,17 @@ enum KernelId : int {
     K_DOWNSTREAM_FWD,
     K_DOWNSTREAM_BWD,
     K_PHM_GEMM_AG,
+    K_EMBEDDING_FWD,
+    K_EMBEDDING_SORT,
+    K_EMBEDDING_BWD,
+    K_GRAD_NORM,
+    K_GRAD_SCALE,
+    K_XENT_LOGITS,
+    K_XENT_ROWS,
+    K_XENT_DLOGITS,
+    K_XENT_DX,
+    K_XENT_DW,
+    K_XENT_LAYOUT,
     K_NUM_KERNELS
 };
 

@@ -42,6 +42,13 @@ class HJob(C.Structure):
                 ("Hk4", _P), ("HTk4", _P), ("gate_w", _P), ("gate_b", _P), ("phm_b", _P), ("gate_c", _P), ("gate_k", C.c_int32)]
 
 
+class LinearXentDesc(C.Structure):
+    """phc_linear_xent_desc (include/phc_hip.h)."""
+    _fields_ = [("N", _L), ("V", _L), ("D", _L), ("ldx", _L), ("ldw", _L), ("ignore_index", _L), ("piece", _L),
+                ("dtype", C.c_int32), ("reduction", C.c_int32), ("x", _P), ("W", _P), ("bias", _P), ("target", _P),
+                ("loss", _P), ("lse", _P), ("stat", _P), ("dloss", _P), ("dx", _P), ("dW", _P), ("db", _P), ("ws", _P), ("ws_bytes", _S)]
+
+
 class DownstreamNorm(C.Structure):
     """phc_downstream_norm (include/phc_hip.h)."""
     _fields_ = [("weight", _P), ("bias", _P), ("running_mean", _P), ("running_var", _P), ("num_batches_tracked", _P),
@@ -310,6 +317,14 @@ SIGNATURES = {
     "phc_clip_adam_fused_ws_bytes": (C.c_size_t, [_I]),
     "phc_clip_adam_fused_supported": (_I, [_I, _I]),
     "phc_clip_adam_fused": (_I, [_P, _P, _I, _P, _I, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float, _P, _P, _P, C.c_size_t, _I, _P]),
+    "phc_embedding_fwd": (_I, [_P, _P, _L, _L, _L, _L, _I, C.c_float, _P, _P]),
+    "phc_embedding_bwd_ws_bytes": (_S, [_L, _L, _L]),
+    "phc_embedding_bwd": (_I, [_P, _P, _L, _L, _L, _L, _I, C.c_float, _L, _P, _P, _S, _P]),
+    "phc_linear_xent_ws_bytes": (_S, [C.POINTER(LinearXentDesc), _I]),
+    "phc_linear_xent_fwd": (_I, [C.POINTER(LinearXentDesc), _P]),
+    "phc_linear_xent_bwd": (_I, [C.POINTER(LinearXentDesc), _P]),
+    "phc_grad_norm_ws_bytes": (_S, [_I, _P]),
+    "phc_grad_norm_clip": (_I, [_I, _P, _P, _P, _I, C.c_double, _P, _P, _P, _P, _S, _P]),
     "phc_prof_enable": (_I, [_I]),
     "phc_prof_reset": (_I, []),
     "phc_prof_num_kernels": (_I, []),
@@ -389,7 +404,9 @@ def require_device(*tensors: Optional[torch.Tensor]) -> torch.device:
 _ERR_WORDS: dict = {}
 _SELF_CHECKED: set = set()
 _ERR_BITS = {1: "edge_index entry outside [0, num_nodes)", 2: "node feature index outside its embedding's vocabulary",
-             4: "edge feature index outside its embedding's vocabulary", 8: "segment id (batch vector) outside [0, num_graphs)"}
+             4: "edge feature index outside its embedding's vocabulary", 8: "segment id (batch vector) outside [0, num_graphs)",
+             32: "token outside its embedding table", 64: "target outside the vocabulary"}
+DTYPE_IDS = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}        # PHC_DTYPE_*
 ERR_RENDEZVOUS = 16                # PHC_ERR_RENDEZVOUS (include/phc_hip.h)
 CHECK_EAGERLY = os.environ.get("PHC_CHECK_INDICES", "0") == "1"
 

@@ -6,7 +6,8 @@ These are the engine-side counterparts of the reference's functional layer:
 ``propagate(aggr='add')`` as used by PHMConv / PHMGINEConv
 (phc/hypercomplex/undirectional/messagepassing.py:55-74,132-146) and
 ``global_add_pool`` (phc/hypercomplex/pooling.py:14).
-All inputs must be fp32 tensors on a ROCm device; there is no CPU path.
+All inputs must be fp32 tensors on a ROCm device (``embedding`` and ``linear_cross_entropy`` take
+16-bit ones too); there is no CPU path.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ import torch
 
 from . import lib as L
 from .graph import EdgeStructure, SegmentStructure, edge_structure, segment_structure
+from .vocab import embedding, linear_cross_entropy  # noqa: F401  (one large table / a large vocabulary: fp32, bf16, fp16)
 
 _SLOW_PATHS_SEEN: set = set()
 

@@ -8,11 +8,13 @@ norm / clip coefficient from the partial sums themselves.  There is no CPU path.
 from __future__ import annotations
 
 import ctypes as C
-from typing import Iterable, List, Optional
+import math
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import lib as L
+from .vocab import on_device
 
 
 # clip + Adam as ONE launch whose workgroups exchange the sums of squares inside it (csrc/optim.hip, round 6); 0 = the two launches
@@ -170,3 +172,98 @@ class ClipAdam:
         self.exp_avg_flat.copy_(sd["exp_avg"])
         self.exp_avg_sq_flat.copy_(sd["exp_avg_sq"])
         self.lr, self.betas, self.eps, self.max_norm = float(sd["lr"]), tuple(sd["betas"]), float(sd["eps"]), float(sd["max_norm"])
+
+
+# ---- the norm over many tensors, clipping (any optimizer; csrc/grad_norm.hip) ---------------------------------------------------
+_NORM_KINDS = {2.0: 0, 1.0: 1, math.inf: 2}
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Its elements fill one piece of memory without gaps (in any order of the dimensions)."""
+    return t.is_contiguous() or torch._prims_common.is_non_overlapping_and_dense(t)
+
+
+def _norm_clip(who: str, grads: Sequence[torch.Tensor], max_norm: float, norm_type: float, out: Optional[Sequence[torch.Tensor]]):
+    """{norm, coefficient} of ``grads`` as a device tensor; the scaled gradients in ``out``."""
+    lib = L.load()
+    kind = _NORM_KINDS.get(float(norm_type))
+    if kind is None:
+        raise L.PhcError(f"{who}: norm_type {norm_type} (known: 1, 2, inf)")
+    if not max_norm >= 0.0:
+        raise L.PhcError(f"{who}: max_norm {max_norm}")
+    dev = L.require_device(*grads, *(out or ()))
+    n = len(grads)
+    ids = L.DTYPE_IDS
+    try:
+        dtypes = (C.c_int32 * n)(*[ids[g.dtype] for g in grads])
+        out_dtypes = None if out is None else (C.c_int32 * n)(*[ids[o.dtype] for o in out])
+    except KeyError as exc:
+        raise L.PhcError(f"{who}: float32, bfloat16 or float16 expected, got {exc.args[0]}") from None
+    numel = (C.c_int64 * n)(*[g.numel() for g in grads])
+    src = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
+    dst = None if out is None else (C.c_void_p * n)(*[o.data_ptr() for o in out])
+    ws_bytes = lib.phc_grad_norm_ws_bytes(n, numel)
+    res = torch.empty(2 + ws_bytes // 4, dtype=torch.float32, device=dev)          # {norm, coefficient} | workspace
+    with on_device(dev):
+        L.check(lib.phc_grad_norm_clip(n, src, numel, dtypes, kind, float(max_norm), dst, out_dtypes, L.ptr(res), L.ptr(res) + 8, ws_bytes,
+                                       L.stream_ptr(dev)), who)
+    return res
+
+
+def _finite_or_raise(who: str, norm: torch.Tensor) -> None:
+    if not torch.isfinite(norm):
+        raise RuntimeError(f"{who}: the total norm of the gradients is {float(norm)}")
+
+
+@torch.no_grad()
+def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
+    """The norm (2, 1 or inf) over all ``tensors`` together (fp32 / bf16 / fp16, mixed) as an fp32 device scalar; 0 for none."""
+    ts = [t if _dense(t) else t.contiguous() for t in tensors]
+    if not ts:
+        return torch.zeros(())
+    return _norm_clip("grad_norm", ts, 0.0, norm_type, None)[0]
+
+
+@torch.no_grad()
+def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float = 2.0, out: Optional[Sequence[torch.Tensor]] = None,
+               error_if_nonfinite: bool = False) -> Tuple[torch.Tensor, List[torch.Tensor]]:
+    """``(norm, results)``: the norm over ``grads`` together, and ``grads`` times ``min(1, max_norm / (norm + 1e-6))`` in new tensors or in
+    ``out`` (same shapes, contiguous, fp32 / bf16 / fp16 — e.g. an optimizer's fp32 copies of 16-bit gradients).  ``out`` may be ``grads``
+    themselves; results must share memory neither with each other nor with another gradient."""
+    gs = [g.contiguous() for g in grads]
+    if out is None:
+        out = [torch.empty_like(g) for g in gs]
+    out = list(out)
+    if len(out) != len(gs):
+        raise L.PhcError(f"clip_grads: {len(gs)} gradients, {len(out)} results")
+    if not gs:
+        return torch.zeros(()), out
+    for i, (g, o) in enumerate(zip(gs, out)):
+        if o.shape != g.shape or not o.is_contiguous():
+            raise L.PhcError(f"clip_grads: result {i} has to be a contiguous tensor of shape {tuple(g.shape)}")
+    norm = _norm_clip("clip_grads", gs, max_norm, norm_type, out)[0]
+    if error_if_nonfinite:
+        _finite_or_raise("clip_grads", norm)
+    return norm, out
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """``torch.nn.utils.clip_grad_norm_`` (benchmarks/train_hiv.py:198-199) in two passes over the gradients, for any optimizer: scales the
+    ``.grad`` of ``parameters`` in place by ``min(1, max_norm / (norm + 1e-6))`` and returns the norm before (fp32 device scalar, no
+    synchronisation unless ``error_if_nonfinite``, which raises BEFORE anything is scaled).  Gradients: fp32 / bf16 / fp16, mixed, on one
+    device; two of them may not share memory."""
+    if isinstance(parameters, torch.Tensor):
+        parameters = [parameters]
+    grads = [p.grad for p in parameters if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    dense = [g if _dense(g) else g.contiguous() for g in grads]
+    if error_if_nonfinite:
+        _finite_or_raise("clip_grad_norm_", _norm_clip("clip_grad_norm_", dense, 0.0, norm_type, None)[0])
+    norm = _norm_clip("clip_grad_norm_", dense, max_norm, norm_type, dense)[0]
+    for g, d in zip(grads, dense):
+        if d is not g:
+            g.copy_(d)
+    return norm

@@ -1,0 +1,232 @@
+"""Operators against a large vocabulary: one-table embedding lookup and the softmax cross entropy of a linear map
+(csrc/embedding.hip, csrc/linear_xent.hip).  Exported by ``phc_gnn_amd.ops``.
+
+Unlike the message-passing operators they take fp32, bf16 and fp16 tensors.  Sums, softmax statistics and losses are fp32 in
+every case; gradients come in the type of their input, rounded once.  There is no CPU path."""
+from __future__ import annotations
+
+import contextlib
+import ctypes as C
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import lib as L
+
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+
+
+def on_device(dev: torch.device):
+    """Launches go to the tensors' device, whatever device is current."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _dtype_id(what: str, t: torch.Tensor) -> int:
+    try:
+        return L.DTYPE_IDS[t.dtype]
+    except KeyError:
+        raise L.PhcError(f"{what}: float32, bfloat16 or float16 expected, got {t.dtype}") from None
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A 2-D tensor the kernels can read in place: unit column stride, rows that do not overlap; anything else is copied."""
+    if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] == 1):
+        return t
+    return t.contiguous()
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return max(t.stride(0), t.shape[1])
+
+
+def _int64(what: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dtype not in (torch.int64, torch.int32):
+        raise L.PhcError(f"{what}: int64 or int32 expected, got {t.dtype}")
+    return t.to(torch.int64).contiguous()
+
+
+def _gradient_nodes(who: str, *tensors: Optional[torch.Tensor]) -> list:
+    """A leaf has ONE gradient node while any graph that ends in it lives, and autograd runs that node on the stream it was made on.  A
+    backward captured on another stream would pull that stream into the capture, which ends the process when the capture ends: refused
+    here, before anything is recorded, for graphs these operators made.  The nodes carry the stream; the caller holds them until its
+    own graph does."""
+    nodes = []
+    if not torch.is_grad_enabled():
+        return nodes
+    for t in tensors:
+        if t is None or not t.requires_grad or not t.is_leaf:
+            continue
+        node = torch.autograd.graph.get_gradient_edge(t).node
+        stream = torch.cuda.current_stream(t.device).cuda_stream
+        made_on = node.metadata.setdefault("phc_stream", stream)
+        if made_on != stream and torch.cuda.is_current_stream_capturing():
+            raise L.PhcError(f"{who}: captured into a graph while an eager result of the same parameter, made on another stream, still holds its "
+                             "autograd graph; detach or delete that result (or make it on the capture's stream) first")
+        nodes.append(node)
+    return nodes
+
+
+# ---- embedding ------------------------------------------------------------------------------------------------------------------
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale: float, pad: int):
+        lib = L.load()
+        dev = weight.device
+        w = _rows(weight)
+        V, D = w.shape
+        N = tokens.numel()
+        out = torch.empty((*tokens.shape, D), dtype=w.dtype, device=dev)
+        with on_device(dev):
+            L.check(lib.phc_embedding_fwd(L.ptr(tokens), L.ptr(w), N, V, D, _row_stride(w), L.DTYPE_IDS[w.dtype], scale, L.ptr(out),
+                                          L.stream_ptr(dev)), "phc_embedding_fwd")
+        L.maybe_check_indices(dev)
+        ctx.save_for_backward(tokens)
+        ctx.meta = (V, D, w.dtype, scale, pad)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        lib = L.load()
+        (tokens,) = ctx.saved_tensors
+        V, D, dtype, scale, pad = ctx.meta
+        dev = tokens.device
+        N = tokens.numel()
+        dy = _rows(dout.to(dtype).reshape(N, D))
+        dw = torch.empty((V, D), dtype=dtype, device=dev)
+        ws_bytes = lib.phc_embedding_bwd_ws_bytes(N, V, D)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        with on_device(dev):
+            L.check(lib.phc_embedding_bwd(L.ptr(tokens), L.ptr(dy), N, V, D, _row_stride(dy), L.DTYPE_IDS[dtype], scale, pad, L.ptr(dw),
+                                          L.ptr(ws), ws_bytes, L.stream_ptr(dev)), "phc_embedding_bwd")
+        return None, dw, None, None
+
+
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[tokens]``: ``weight`` [V, D], ``tokens`` int64 / int32 of any shape -> [*tokens.shape, D] in the weight's type.
+
+    The gradient of ``weight`` is dense, ``scale`` times the sum of the rows' gradients per token in a fixed order (bitwise
+    reproducible), zero in row ``padding_idx``.  A token outside [0, V) reads row 0, counts as 0 in the gradient and is reported by
+    ``phc_gnn_amd.check_indices()``, like the encoders' feature values."""
+    dev = L.require_device(tokens, weight)
+    _dtype_id("embedding: weight", weight)
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise L.PhcError(f"embedding: weight [V, D] expected, got {tuple(weight.shape)}")
+    nodes = _gradient_nodes("embedding", weight)
+    V = weight.shape[0]
+    pad = -1
+    if padding_idx is not None:
+        if not -V <= padding_idx < V:
+            raise L.PhcError(f"embedding: padding_idx {padding_idx} outside the {V} rows")
+        pad = int(padding_idx) % V
+    out = _EmbeddingFn.apply(_int64("embedding: tokens", tokens), weight, float(scale), pad)
+    del nodes
+    return out
+
+
+# ---- softmax cross entropy of a linear map ----------------------------------------------------------------------------------------
+def _xent_desc(x, w, bias, target, ignore_index, reduction, stat, lse, piece):
+    d = L.LinearXentDesc()
+    d.N, d.D = x.shape
+    d.V = w.shape[0]
+    d.ldx, d.ldw = _row_stride(x), _row_stride(w)
+    d.ignore_index, d.piece = ignore_index, piece
+    d.dtype, d.reduction = L.DTYPE_IDS[x.dtype], reduction
+    d.x, d.W, d.bias, d.target = L.ptr(x), L.ptr(w), L.ptr(bias), L.ptr(target)
+    d.lse, d.stat = L.ptr(lse), L.ptr(stat)
+    return d
+
+
+def _xent_workspace(lib, d, backward: int, dev) -> torch.Tensor:
+    n = lib.phc_linear_xent_ws_bytes(C.byref(d), backward)
+    if n == 0:
+        raise L.PhcError(f"linear_cross_entropy: {lib.phc_last_error().decode()}")
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    d.ws, d.ws_bytes = ws.data_ptr(), n
+    return ws
+
+
+class _LinearCrossEntropyFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index: int, reduction: int, piece: int):
+        lib = L.load()
+        dev = x.device
+        N = x.shape[0]
+        ctx.meta = (ignore_index, reduction, piece)
+        if N == 0:
+            ctx.save_for_backward(x, weight, bias)
+            if reduction == 0:
+                return torch.zeros(0, dtype=torch.float32, device=dev)
+            return torch.full((), float("nan") if reduction == 2 else 0.0, dtype=torch.float32, device=dev)
+        x_, w_ = _rows(x), _rows(weight)
+        b_ = None if bias is None else bias.contiguous()
+        loss = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
+        lse = torch.empty(N, dtype=torch.float32, device=dev)
+        stat = torch.empty(2, dtype=torch.float32, device=dev)
+        d = _xent_desc(x_, w_, b_, target, ignore_index, reduction, stat, lse, piece)
+        d.loss = L.ptr(loss)
+        ws = _xent_workspace(lib, d, 0, dev)
+        with on_device(dev):
+            L.check(lib.phc_linear_xent_fwd(C.byref(d), L.stream_ptr(dev)), "phc_linear_xent_fwd")
+        del ws
+        L.maybe_check_indices(dev)
+        ctx.save_for_backward(x_, w_, b_, target, lse, stat)
+        return loss
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dloss):
+        lib = L.load()
+        ignore_index, reduction, piece = ctx.meta
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        if len(ctx.saved_tensors) == 3:                          # no rows
+            x, w, b = ctx.saved_tensors
+            return (torch.zeros_like(x) if need_x else None, torch.zeros_like(w) if need_w else None,
+                    torch.zeros_like(b) if need_b else None, None, None, None, None)
+        x, w, b, target, lse, stat = ctx.saved_tensors
+        dev = x.device
+        g = dloss.to(torch.float32).contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+        dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
+        db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need_b else None
+        d = _xent_desc(x, w, b, target, ignore_index, reduction, stat, lse, piece)
+        d.dloss, d.dx, d.dW, d.db = L.ptr(g), L.ptr(dx), L.ptr(dw), L.ptr(db)
+        ws = _xent_workspace(lib, d, 1, dev)
+        with on_device(dev):
+            L.check(lib.phc_linear_xent_bwd(C.byref(d), L.stream_ptr(dev)), "phc_linear_xent_bwd")
+        del ws
+        return dx, dw, db, None, None, None, None
+
+
+def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                         ignore_index: int = -100, reduction: str = "mean", piece: int = 0) -> torch.Tensor:
+    """Softmax cross entropy of the logits ``x @ weight.T + bias`` against ``target``, without the logits in memory.
+
+    ``x`` [*, D] and ``weight`` [V, D] (and ``bias`` [V]) of one type (fp32, bf16, fp16), ``target`` [*] int64 / int32 -> fp32 loss: one
+    value (``reduction`` "mean", "sum") or one for each row ("none").  Rows whose target is ``ignore_index`` have loss 0 and a zero
+    gradient and stay out of the mean; the mean of no rows is NaN, as for an empty selection.  A bias of -inf takes a column out of the
+    vocabulary.  A target outside [0, V) counts as 0 and is reported by ``phc_gnn_amd.check_indices()``.
+
+    The backward computes the logits again, ``piece`` columns of the vocabulary at a time (0: as many as keep a piece's gradients in the
+    last-level cache; its workspace grows with ``piece``).  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
+    dev = L.require_device(x, weight, target, bias)
+    _dtype_id("linear_cross_entropy: x", x)
+    if weight.dim() != 2 or x.dim() < 1 or weight.shape[0] < 1 or weight.shape[1] < 1 or x.shape[-1] != weight.shape[1]:
+        raise L.PhcError(f"linear_cross_entropy: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
+        raise L.PhcError(f"linear_cross_entropy: x, weight and bias of one type expected, got {x.dtype}, {weight.dtype}"
+                         + ("" if bias is None else f", {bias.dtype}"))
+    if bias is not None and tuple(bias.shape) != (weight.shape[0],):
+        raise L.PhcError(f"linear_cross_entropy: bias {tuple(bias.shape)} does not fit {weight.shape[0]} columns")
+    if tuple(target.shape) != tuple(x.shape[:-1]):
+        raise L.PhcError(f"linear_cross_entropy: target {tuple(target.shape)} does not fit x {tuple(x.shape)}")
+    if reduction not in _REDUCTIONS:
+        raise L.PhcError(f"linear_cross_entropy: unknown reduction '{reduction}' (known: {sorted(_REDUCTIONS)})")
+    if piece < 0:
+        raise L.PhcError(f"linear_cross_entropy: piece {piece}")
+    nodes = _gradient_nodes("linear_cross_entropy", x, weight, bias)
+    t = _int64("linear_cross_entropy: target", target).reshape(-1)
+    loss = _LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, bias, t, int(ignore_index), _REDUCTIONS[reduction], int(piece))
+    del nodes
+    return loss.reshape(target.shape) if reduction == "none" else loss
