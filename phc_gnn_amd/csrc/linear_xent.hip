@@ -20,7 +20,46 @@
 
 namespace phc {
 
-constexpr int XT_BK = 64;                      // k per step: 128 bytes of a row = one line of LDS
+constexpr int XT_BK = 64;                      // k per step: 128 bytes of a k-contiguous row = one line of LDS
+
+// ---- rows that count --------------------------------------------------------------------------------------------------------------------
+// Rows whose target is ignored cost nothing: the others are numbered in order ("packed" rows), and every product runs over those.
+struct XRows {
+    int *count;                // rows that count
+    int *from;                 // [packed row] -> row
+    int *to;                   // [row] -> packed row, -1 for the ignored ones
+    int *target;               // [packed row] -> column, checked
+};
+
+__global__ __launch_bounds__(1024) void xent_rows_that_count_kernel(const long long *__restrict__ target, long long ignore, int N, long long V,
+                                                                   int *err, XRows r) {
+    __shared__ int wsum[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int carry = 0;
+    for (int base = 0; base < N; base += 1024) {
+        const int i = base + threadIdx.x;
+        const long long t = i < N ? target[i] : ignore;
+        const bool kept = t != ignore;
+        const unsigned long long m = __ballot(kept);
+        if (lane == 0) wsum[wave] = __popcll(m);
+        __syncthreads();
+        int before = carry, total = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) before += wsum[w];
+            total += wsum[w];
+        }
+        const int at = before + __popcll(m & ((1ull << lane) - 1));
+        if (i < N) r.to[i] = kept ? at : -1;
+        if (kept) {
+            r.from[at] = i;
+            r.target[at] = (int)checked_index(t, V, err, PHC_IDX_ERR_TARGET);
+        }
+        carry += total;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *r.count = carry;
+}
 
 // ---- operand layout -------------------------------------------------------------------------------------------------------------------
 struct XPlanes {
@@ -34,60 +73,69 @@ __device__ __forceinline__ void split3(float a, bf16_t &h, bf16_t &m, bf16_t &l)
     l = (bf16_t)(r - (float)m);
 }
 
-// value -> the operand planes (one for 16-bit types, three for fp32)
-template <typename TIN>
-__device__ __forceinline__ void put_planes(const XPlanes &o, size_t at, TIN v) {
+// W consecutive values -> the operand planes (one for 16-bit types, three for fp32)
+template <typename TIN, int W>
+__device__ __forceinline__ void put_planes(const XPlanes &o, size_t at, const TIN (&v)[W]) {
     if constexpr (sizeof(TIN) == 4) {
-        bf16_t h, m, l;
-        split3(v, h, m, l);
-        static_cast<bf16_t *>(o.p[0])[at] = h;
-        static_cast<bf16_t *>(o.p[1])[at] = m;
-        static_cast<bf16_t *>(o.p[2])[at] = l;
+        Pack<bf16_t, W> h, m, l;
+#pragma unroll
+        for (int i = 0; i < W; ++i) split3(v[i], h.v[i], m.v[i], l.v[i]);
+        *reinterpret_cast<Pack<bf16_t, W> *>(static_cast<bf16_t *>(o.p[0]) + at) = h;
+        *reinterpret_cast<Pack<bf16_t, W> *>(static_cast<bf16_t *>(o.p[1]) + at) = m;
+        *reinterpret_cast<Pack<bf16_t, W> *>(static_cast<bf16_t *>(o.p[2]) + at) = l;
     } else {
-        static_cast<TIN *>(o.p[0])[at] = v;
+        Pack<TIN, W> q;
+#pragma unroll
+        for (int i = 0; i < W; ++i) q.v[i] = v[i];
+        *reinterpret_cast<Pack<TIN, W> *>(static_cast<TIN *>(o.p[0]) + at) = q;
     }
 }
 
-// rows [R, C] -> operand rows [R, Cp], columns behind C zero
+// Rows [R, C] -> operand rows [., Cp] (8 columns a thread), columns behind C zero.  `to`: row i goes to packed row to[i]; an ignored one
+// has its row of `zero` (dense [R, C], may be null) cleared instead; the packed rows behind `count` up to a whole step are zero.
 template <typename TIN>
-__global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ src, long long ld, long long R, int C, int Cp, XPlanes out) {
-    const long long total = R * (long long)Cp;
+__global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ src, long long ld, long long R, int C, int Cp, int vec,
+                                                       const int *__restrict__ to, const int *__restrict__ count, TIN *__restrict__ zero, XPlanes out) {
+    const int per = Cp / 8;
+    const long long total = (R + (to ? XT_BK : 0)) * (long long)per;
     for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
-        const long long r = e / Cp;
-        const int c = (int)(e - r * Cp);
-        put_planes<TIN>(out, (size_t)e, c < C ? src[r * ld + c] : (TIN)0.f);
-    }
-}
-
-// rows [R, C] -> operand columns [C, Rp], rows behind R zero; `target`: a row whose target is ignored counts as zero, whatever it
-// holds (its d is zero, and zero times a NaN is none)
-template <typename TIN>
-__global__ __launch_bounds__(256) void xent_transpose_kernel(const TIN *__restrict__ src, long long ld, long long R, int C, long long Rp,
-                                                            const long long *__restrict__ target, long long ignore, XPlanes out) {
-    __shared__ TIN tile[64][65];
-    const long long r0 = (long long)blockIdx.x * 64;
-    const int c0 = (int)blockIdx.y * 64;
-    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-        const long long r = r0 + i;
-        const int c = c0 + (threadIdx.x & 63);
-        TIN v = (TIN)0.f;
-        if (r < R && c < C && !(target && target[r] == ignore)) v = src[r * ld + c];
-        tile[i][threadIdx.x & 63] = v;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x >> 6; i < 64; i += 4) {
-        const int c = c0 + i;
-        const long long r = r0 + (threadIdx.x & 63);
-        if (c < C && r < Rp) put_planes<TIN>(out, (size_t)c * Rp + r, tile[threadIdx.x & 63][i]);
+        const long long r = e / per;
+        const int c = (int)(e - r * per) * 8;
+        TIN v[8];
+        long long at = r;
+        bool fill = false;
+        if (to) {
+            if (r >= R) {                                         // rows behind the last one
+                at = *count + (r - R);
+                fill = true;
+                if (at >= (*count + XT_BK - 1) / XT_BK * XT_BK) continue;
+            } else {
+                at = to[r];
+                if (at < 0) {
+                    if (zero)
+                        for (int k = c; k < c + 8 && k < C; ++k) zero[r * C + k] = (TIN)0.f;
+                    continue;
+                }
+            }
+        }
+        if (!fill && vec && c + 8 <= C) {
+            constexpr int H = 16 / sizeof(TIN);                   // 16-byte loads
+#pragma unroll
+            for (int k = 0; k < 8; k += H) {
+                const Pack<TIN, H> q = *reinterpret_cast<const Pack<TIN, H> *>(src + r * ld + c + k);
+#pragma unroll
+                for (int j = 0; j < H; ++j) v[k + j] = q.v[j];
+            }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = !fill && c + k < C ? src[r * ld + c + k] : (TIN)0.f;
+        }
+        put_planes<TIN, 8>(out, (size_t)at * Cp + c, v);
     }
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------------
-template <int N>
-__device__ __forceinline__ void xt_wait_vm() {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void xt_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void xt_wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 // One LDS-DMA instruction: every lane's 16 bytes at base + voff land at LDS byte address lds + 16 lane.  In asm because hipcc orders its
 // builtin against every later LDS read with s_waitcnt vmcnt(0), which would drain the prefetch; the loop's own waits order it.  M0 is
@@ -98,6 +146,13 @@ __device__ __forceinline__ void xt_dma16(unsigned lds, unsigned voff, const void
                  : "=&s"(keep)
                  : "s"(lds), "v"(voff), "s"(base)
                  : "memory");
+}
+
+// (the same in all lanes; hipcc must know it)
+__device__ __forceinline__ const char *uniform(const char *p) {
+    const unsigned long long v = reinterpret_cast<unsigned long long>(p);
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+    return reinterpret_cast<const char *>(((unsigned long long)hi << 32) | lo);
 }
 
 template <typename T>
@@ -113,36 +168,53 @@ struct Mfma16<f16_t> {
     static __device__ __forceinline__ f32x4_t mul(frag a, frag b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
-enum XEpilogue { XE_STATS, XE_DLOGITS, XE_OUT };
+typedef __attribute__((ext_vector_type(4))) short s16x4_t;
+typedef __attribute__((ext_vector_type(8))) short s16x8_t;
+typedef __attribute__((address_space(3))) const char lds_char;
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
+typedef __attribute__((address_space(3))) const s16x8_t lds_s16x8;
+
+enum XEpilogue { XE_STATS, XE_DLOGITS, XE_DX, XE_DW };
 
 struct XGemm {
     const char *A[6], *B[6];       // operand planes of each segment of the k loop
     int segments;                  // 1, or 6 for fp32 inputs
-    int ksteps;                    // steps of XT_BK per segment
+    long long K;                   // valid k (XE_DW: the count of packed rows instead)
     unsigned lda, ldb;             // row strides in bytes
-    long long rowsA, rowsB;        // valid m, n
-    int tilesM, tilesN, splits;
+    int rowsA;                     // valid m
+    int rowsB;                     // valid n (where n are the packed rows: at most)
+    int colsA;                     // A held as [k][m]: readable columns
+    int tilesM, tilesN, max_blocks;
+    int split_k;                   // k that the number of splits goes by
+    const int *count;              // packed rows
     // XE_STATS / XE_DLOGITS
-    const void *bias;              // fp32 or the operand's type (bias_f32), of this piece; may be null
-    int bias_f32;
-    const long long *target;       // [rowsB]
-    long long ignore, first_v, vocab;     // piece begins at first_v
-    int *err;
-    float *part_max, *part_sum;    // [parts][rowsB]
-    float *target_logit;           // [rowsB]
-    const float *lse, *row_rel;    // [rowsB]
-    XPlanes d, dT;                 // [rowsB][ldd] and [m][lddT]
-    long long ldd, lddT;
+    const void *bias;              // fp32 or the operand's type, of this piece; may be null
+    const int *target;             // [packed rows]
+    int first_v;                   // the piece begins here
+    float *part_max, *part_sum;    // [tilesM][N]
+    float *target_logit;           // [packed rows]
+    const float *lse, *rel;        // [packed rows]
+    XPlanes d;                     // [packed rows][ldd]
+    int ldd;
     float d_scale;                 // 16-bit d are stored times this
     float *db_part;                // [tilesN * WN][rowsA] or null
-    // XE_OUT
-    const float *row_scale;        // [rowsB] or null
-    const float *scale;            // one value, or null
+    int N;
+    // XE_DX / XE_DW
+    const float *scale;            // one value
     float out_scale;
+    const int *row_of;             // XE_DX: packed row -> output row
     void *out;                     // element (n, m) at n * ldo + m
-    long long ldo, slab;           // slab: elements between the splits' partial outputs (fp32), 0 = final output in its own type
-    int accumulate, out_dtype, out_vec;
+    int ldo;
+    float *slabs;                  // fp32 partial outputs [split][rows][ldo]
+    int accumulate, pieces, out_vec;
 };
+
+// Work of a product over `tiles` output tiles: the k loop is split where the tiles alone do not fill the card, never below 4 steps.
+__host__ __device__ inline int xt_splits(int tiles, int steps, int max_blocks) {
+    int s = tiles > 0 ? max_blocks / tiles : 1;
+    if (s > steps / 4) s = steps / 4;
+    return s < 1 ? 1 : s > 64 ? 64 : s;
+}
 
 // Tile order: the workgroups of an XCD take neighbouring tiles (blockIdx goes round-robin over the 8 XCDs), in bands of 8 m-tiles, so
 // that the tiles in flight on an XCD share operand rows in its L2.
@@ -157,44 +229,108 @@ __device__ __forceinline__ void xt_tile_of(unsigned b, int tilesM, int tilesN, i
     tn = (int)(in / height);
 }
 
+// One operand's side of the tile: T rows (m or n) by XT_BK of k, in LDS either as it is read k-contiguous, [T][64], or, where memory holds
+// it as [k][m], as [64][T] with the transposing LDS read.  16-byte pieces of an LDS row are stored at piece ^ f(row), which spreads the
+// banks of the 8 (16) rows that a quarter wavefront reads together.
+template <int T, bool TR, bool PAIR>
+struct XSide {
+    static constexpr int PIECES = TR ? T / 8 : 8;                       // per LDS row
+    static constexpr int ROWS_PER_DMA = 64 / PIECES;
+    static __device__ __forceinline__ int f(int row) {
+        if constexpr (TR) return ((row & 3) << 1) ^ (((row >> 3) & 1) << 3);
+        else return PAIR ? (row & 3) | ((row >> 1) & 4) : row & 7;
+    }
+    // m (n) of row rho of fragment i.  PAIR: two fragments give a lane 8 consecutive m (it holds rows 4 g .. 4 g + 3 of each).
+    static __device__ __forceinline__ int index(int i, int rho) {
+        return PAIR ? (i >> 1) * 32 + (rho >> 2) * 8 + (i & 1) * 4 + (rho & 3) : i * 16 + rho;
+    }
+    // fragment i (from `first` on) of half kk of the step
+    template <typename frag>
+    static __device__ __forceinline__ frag read(lds_char *tile, int first, int i, int kk, int lane) {
+        const int rho = lane & 15, g = lane >> 4;
+        if constexpr (TR) {
+            const int k = kk * 32 + g * 8 + (rho >> 2), piece = ((first + i * 16) >> 3) + ((rho >> 1) & 1);
+            lds_char *at = tile + k * (T * 2) + ((piece ^ f(k)) << 4) + (rho & 1) * 8;          // f(k + 4) = f(k)
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at);
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 4 * (T * 2)));
+            return __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const int row = first + index(i, rho);
+            return __builtin_bit_cast(frag, *(lds_s16x8 *)(tile + row * 128 + (((kk * 4 + g) ^ f(row)) << 4)));
+        }
+    }
+};
+
 template <typename T, int EPI, bool WIDE, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     typedef typename Mfma16<T>::frag frag;
     constexpr int NW = WM * WN, TM = WM * FM * 16, TN = WN * FN * 16;
-    constexpr int LOADS = (TM + TN) / 8 / NW;                   // LDS-DMA instructions per wavefront and step (8 rows each)
-    static_assert((TM / 8) % LOADS == 0, "a wavefront loads rows of one operand");
+    constexpr bool A_TR = EPI == XE_DX || EPI == XE_DW, B_TR = EPI == XE_DW, PAIR = EPI == XE_DLOGITS;
+    typedef XSide<TM, A_TR, PAIR> SA;
+    typedef XSide<TN, B_TR, false> SB;
+    constexpr int LOADS = (TM + TN) / 8 / NW;                   // LDS-DMA instructions per wavefront and step (1 KiB each)
+    static_assert((TM / 8) % LOADS == 0, "a wavefront loads one operand");
     constexpr unsigned BUF = (TM + TN) * 128;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    const unsigned tiles = (unsigned)a.tilesM * a.tilesN;
-    const int split = (int)(blockIdx.x / tiles);
+
+    // what there is to do goes by the rows that count
+    const int count = *a.count;
+    const int rowsB = EPI == XE_DW ? a.rowsB : count;
+    const int tilesN = (rowsB + TN - 1) / TN, tiles = a.tilesM * tilesN;
+    const int ksteps = EPI == XE_DW ? (count + XT_BK - 1) / XT_BK : (int)((a.K + XT_BK - 1) / XT_BK);
+    int split = 0, splits = 1, tile = blockIdx.x;
+    if constexpr (EPI == XE_DX || EPI == XE_DW) {
+        splits = xt_splits(tiles, a.segments * (EPI == XE_DW ? ksteps : a.split_k / XT_BK), a.max_blocks);
+        if (tiles > 0) {
+            split = tile / tiles;
+            tile -= split * tiles;
+        }
+    }
+    if (tiles == 0 || (EPI == XE_STATS || EPI == XE_DLOGITS ? tile >= tiles : split >= splits)) return;
     int tm, tn;
-    xt_tile_of(blockIdx.x % tiles, a.tilesM, a.tilesN, tm, tn);
+    xt_tile_of(tile, a.tilesM, tilesN, tm, tn);
+    const int steps = a.segments * ksteps;
+    const int s0 = (int)((long long)steps * split / splits), n_steps = (int)((long long)steps * (split + 1) / splits) - s0;
 
-    // this split's share of the steps
-    const int steps = a.segments * a.ksteps;
-    const int s0 = (int)((long long)steps * split / a.splits), s1 = (int)((long long)steps * (split + 1) / a.splits);
-
-    // loader: the wavefront's rows of its operand; 16-byte pieces of a row are stored at piece ^ (row & 7) (bank spread for the reads)
+    // loader
     const bool loads_a = wave * LOADS < TM / 8;
-    const long long row0 = loads_a ? (long long)tm * TM : (long long)tn * TN;
-    const long long rows = loads_a ? a.rowsA : a.rowsB;
     const unsigned ld = loads_a ? a.lda : a.ldb;
+    const bool tr = loads_a ? A_TR : B_TR;
+    const long long at0 = loads_a ? (long long)tm * TM : (long long)tn * TN;
+    const int dma0 = wave * LOADS - (loads_a ? 0 : TM / 8);     // this wavefront's first instruction of its operand
+    // memory rows behind an operand's end repeat its last one: their results are dropped, or the other operand has zeros there
+    const int rows = tr ? (EPI == XE_DW ? 0x7fffffff : (int)a.K) : loads_a ? a.rowsA : rowsB;
+    auto offset = [&](int q, int first, int limit) -> unsigned {
+        if (tr) {
+            const int per = loads_a ? SA::PIECES : SB::PIECES, row = (dma0 + q) * (64 / per) + lane / per;
+            const int f = loads_a ? XSide<TM, true, false>::f(row) : XSide<TN, true, false>::f(row);
+            const int col = min((int)at0 + ((lane % per) ^ f) * 8, (loads_a ? a.colsA : (int)(a.ldb / 2)) - 8);
+            return (unsigned)min(row, limit - 1 - first) * ld + (unsigned)col * 2;
+        }
+        const int row = (dma0 + q) * 8 + (lane >> 3);
+        const int f = loads_a ? XSide<TM, false, PAIR>::f(row) : XSide<TN, false, false>::f(row);
+        return (unsigned)min(row, limit - 1 - first) * ld + ((lane & 7) ^ f) * 16;
+    };
     unsigned voff[LOADS];
 #pragma unroll
-    for (int q = 0; q < LOADS; ++q) {
-        const int r = (wave * LOADS + q) * 8 - (loads_a ? 0 : TM) + (lane >> 3);
-        const long long row = min(row0 + r, rows - 1) - row0;   // rows behind the operand repeat its last one; their results are dropped
-        voff[q] = (unsigned)row * ld + (((lane & 7) ^ (r & 7)) << 4);
-    }
-    const unsigned lds0 = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem;
-    const unsigned lds_wave = lds0 + wave * LOADS * 1024;
-    auto issue = [&](int s, int buf) {
-        const int seg = s / a.ksteps, k = s - seg * a.ksteps;
-        const char *base = (loads_a ? a.A[seg] : a.B[seg]) + row0 * ld + (size_t)k * (XT_BK * 2);
+    for (int q = 0; q < LOADS; ++q) voff[q] = offset(q, tr ? 0 : (int)at0, tr ? XT_BK : rows);
+    const unsigned lds_wave = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem + wave * LOADS * 1024;
+    int seg = s0 / (ksteps > 0 ? ksteps : 1), kst = s0 - seg * ksteps;          // the step that is loaded next
+    auto issue = [&](int buf) {
+        const char *base = uniform((loads_a ? a.A[seg] : a.B[seg]) + (tr ? (size_t)kst * XT_BK * ld : (size_t)at0 * ld + (size_t)kst * (XT_BK * 2)));
+        if (A_TR && EPI != XE_DW && tr && (kst + 1) * XT_BK > rows) {           // the last rows of k
 #pragma unroll
-        for (int q = 0; q < LOADS; ++q) xt_dma16(lds_wave + buf * BUF + q * 1024, voff[q], base);
+            for (int q = 0; q < LOADS; ++q) xt_dma16(lds_wave + buf * BUF + q * 1024, offset(q, kst * XT_BK, rows), base);
+        } else {
+#pragma unroll
+            for (int q = 0; q < LOADS; ++q) xt_dma16(lds_wave + buf * BUF + q * 1024, voff[q], base);
+        }
+        if (++kst == ksteps) {
+            kst = 0;
+            ++seg;
+        }
     };
 
     f32x4_t acc[FM][FN];
@@ -203,146 +339,185 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
-    const int fr = lane & 15, fg = lane >> 4;
-    if (s0 < s1) issue(s0, 0);
-    for (int s = s0; s < s1; ++s) {
-        const int buf = (s - s0) & 1;
-        xt_wait_lds();                                          // this wavefront's reads of the other buffer are done
-        xt_wait_vm<0>();                                        // and its loads into this one
+    // Two LDS buffers, two halves of a step.  While the products of one half run, the fragments of the next are read; the one barrier of a
+    // step stands between them: behind it the next step's buffer is complete, and this step's buffer, read to its end, is loaded anew.
+    lds_char *lds = (lds_char *)smem;
+    const int ma = wm * FM * 16, nb = wn * FN * 16;
+    if (n_steps > 0) {
+        frag fa[2][FM], fb[2][FN];
+        issue(0);
+        xt_wait_all();
         __builtin_amdgcn_s_barrier();
-        if (s + 1 < s1) issue(s + 1, buf ^ 1);
-        const char *la = smem + buf * BUF, *lb = la + TM * 128;
+        if (n_steps > 1) issue(1);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            frag fa[FM], fb[FN];
-            const int piece = ((kk * 4 + fg) ^ (fr & 7)) << 4;
+        for (int j = 0; j < FN; ++j) fb[0][j] = SB::template read<frag>(lds + TM * 128, nb, j, 0, lane);
 #pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = *reinterpret_cast<const frag *>(la + (wm * FM * 16 + i * 16 + fr) * 128 + piece);
+        for (int i = 0; i < FM; ++i) fa[0][i] = SA::template read<frag>(lds, ma, i, 0, lane);
+        for (int t = 0; t < n_steps; ++t) {
+            lds_char *cur = lds + (t & 1) * BUF, *nxt = lds + ((t & 1) ^ 1) * BUF;
 #pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = *reinterpret_cast<const frag *>(lb + (wn * FN * 16 + j * 16 + fr) * 128 + piece);
+            for (int j = 0; j < FN; ++j) fb[1][j] = SB::template read<frag>(cur + TM * 128, nb, j, 1, lane);
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+            for (int i = 0; i < FM; ++i) {
+                fa[1][i] = SA::template read<frag>(cur, ma, i, 1, lane);
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Mfma16<T>::mul(fa[i], fb[j], acc[i][j]);
+                for (int j = 0; j < FN; ++j) acc[i][j] = Mfma16<T>::mul(fa[0][i], fb[0][j], acc[i][j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            xt_wait_all();
+            __builtin_amdgcn_s_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            if (t + 2 < n_steps) issue(t & 1);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[0][j] = SB::template read<frag>(nxt + TM * 128, nb, j, 0, lane);      // (behind the last step: read, not used)
+#pragma unroll
+            for (int i = 0; i < FM; ++i) {
+                fa[0][i] = SA::template read<frag>(nxt, ma, i, 0, lane);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = Mfma16<T>::mul(fa[1][i], fb[1][j], acc[i][j]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 
-    // element (i, j, r): m = mbase + i * 16 + r, n = nbase + j * 16
-    const long long mbase = (long long)tm * TM + wm * FM * 16 + fg * 4;
-    const long long nbase = (long long)tn * TN + wn * FN * 16 + fr;
+    // a lane holds m = m_of(i) + r (r = 0 .. 3) of n = n0 + 16 j
+    const int fr = lane & 15, fg = lane >> 4;
+    const int m_base = tm * TM + ma, n0 = tn * TN + nb + fr;
+    auto m_of = [&](int i) { return m_base + SA::index(i, fg * 4); };
     if constexpr (EPI == XE_STATS || EPI == XE_DLOGITS) {
+        typedef std::conditional_t<WIDE, float, T> TB;
         float bias[FM][4];
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const long long m = mbase + i * 16 + r;
+                const int m = m_of(i) + r;
                 float b = 0.f;
-                if (a.bias && m < a.rowsA) b = a.bias_f32 ? static_cast<const float *>(a.bias)[m] : to_f32(static_cast<const T *>(a.bias)[m]);
+                if (a.bias && m < a.rowsA) b = to_f32(static_cast<const TB *>(a.bias)[m]);
                 bias[i][r] = m < a.rowsA ? b : -INFINITY;       // columns behind the vocabulary: exp 0
             }
-        float dbs[FM][4] = {};
+        if constexpr (EPI == XE_STATS) {
+            float mx[FN], sum[FN];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const long long n = nbase + j * 16;
-            const bool in = n < a.rowsB;
-            const long long t = a.target[in ? n : 0];
-            const bool kept = in && t != a.ignore;
-            const long long hit = (kept ? (EPI == XE_STATS ? checked_index(t, a.vocab, fg == 0 && tm == 0 ? a.err : nullptr, PHC_IDX_ERR_TARGET)
-                                                          : safe_index(t, a.vocab))
-                                        : -1) - a.first_v - mbase;          // target's m, counted from this lane's first
-            if constexpr (EPI == XE_STATS) {
-                float mx = -INFINITY;
+            for (int j = 0; j < FN; ++j) {
+                const int n = n0 + j * 16;
+                const int hit = n < rowsB ? a.target[n] - a.first_v : -1;
+                mx[j] = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float l = acc[i][j][r] + bias[i][r];
                         acc[i][j][r] = l;
-                        mx = fmaxf(mx, l);
-                        if (hit == i * 16 + r) a.target_logit[n] = l;
+                        mx[j] = fmaxf(mx[j], l);
+                        if (hit == m_of(i) + r) a.target_logit[n] = l;
                     }
-                mx = fmaxf(mx, __shfl_xor(mx, 16));
-                mx = fmaxf(mx, __shfl_xor(mx, 32));
-                const float shift = mx == -INFINITY ? 0.f : mx;             // nothing but -inf: every exponential is 0
-                float sum = 0.f;
+                mx[j] = fmaxf(mx[j], __shfl_xor(mx[j], 16));
+                mx[j] = fmaxf(mx[j], __shfl_xor(mx[j], 32));
+                const float shift = mx[j] == -INFINITY ? 0.f : mx[j];       // nothing but -inf: every exponential is 0
+                sum[j] = 0.f;
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sum += WIDE ? expf(acc[i][j][r] - shift) : __expf(acc[i][j][r] - shift);
-                sum += __shfl_xor(sum, 16);
-                sum += __shfl_xor(sum, 32);
-                if (in && fg == 0) {
-                    const size_t at = (size_t)(tm * WM + wm) * a.rowsB + n;
-                    a.part_max[at] = mx;
-                    a.part_sum[at] = sum;
+                    for (int r = 0; r < 4; ++r) sum[j] += WIDE ? expf(acc[i][j][r] - shift) : __expf(acc[i][j][r] - shift);
+                sum[j] += __shfl_xor(sum[j], 16);
+                sum[j] += __shfl_xor(sum[j], 32);
+            }
+            // the wavefronts along m, through LDS
+            __syncthreads();
+            float2 *meet = reinterpret_cast<float2 *>(smem);                // [WM][TN]
+            if (fg == 0)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) meet[wm * TN + nb + j * 16 + fr] = make_float2(mx[j], sum[j]);
+            __syncthreads();
+            for (int c = threadIdx.x; c < TN; c += NW * 64) {
+                const int n = tn * TN + c;
+                if (n >= rowsB) continue;
+                float m = meet[c].x, s = meet[c].y;
+#pragma unroll
+                for (int w = 1; w < WM; ++w) {
+                    const float2 o = meet[w * TN + c];
+                    const float top = fmaxf(m, o.x), shift = top == -INFINITY ? 0.f : top;
+                    s = s * expf(m - shift) + o.y * expf(o.x - shift);
+                    m = top;
                 }
-            } else {
-                const float lse = in ? a.lse[n] : 0.f, rel = in ? a.row_rel[n] : 0.f;
+                a.part_max[(size_t)tm * a.N + n] = m;
+                a.part_sum[(size_t)tm * a.N + n] = s;
+            }
+        } else {
+            const int n_end = (count + XT_BK - 1) / XT_BK * XT_BK;          // zero rows up to a whole step of the weight gradient's k
+            float dbs[FM][4] = {};
 #pragma unroll
-                for (int i = 0; i < FM; ++i) {
+            for (int j = 0; j < FN; ++j) {
+                const int n = n0 + j * 16;
+                const bool in = n < count;
+                const int hit = in ? a.target[n] - a.first_v : -1;
+                const float lse = in ? a.lse[n] : 0.f, rel = in ? a.rel[n] : 0.f;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float l = acc[i][j][r] + bias[i][r];
+                for (int i = 0; i < FM; i += 2) {
+                    TB d[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const int ii = i + e / 4, r = e % 4, m = m_of(ii) + r;
+                        const float l = acc[ii][j][r] + bias[ii][r];
                         const float p = WIDE ? expf(l - lse) : __expf(l - lse);
-                        const long long m = mbase + i * 16 + r;
-                        const float d = kept && m < a.rowsA ? p - (hit == i * 16 + r ? 1.f : 0.f) : 0.f;
-                        const float dr = kept && m < a.rowsA ? d * rel : 0.f;
-                        dbs[i][r] += dr;
-                        if (in && m < a.ldd) put_planes<std::conditional_t<WIDE, float, T>>(a.d, (size_t)n * a.ldd + m, (std::conditional_t<WIDE, float, T>)(d * a.d_scale));
-                        if (m < a.rowsA && n < a.lddT) put_planes<std::conditional_t<WIDE, float, T>>(a.dT, (size_t)m * a.lddT + n, (std::conditional_t<WIDE, float, T>)(dr * a.d_scale));
+                        const float v = in && m < a.rowsA ? (p - (hit == m ? 1.f : 0.f)) * rel : 0.f;
+                        dbs[ii][r] += v;
+                        d[e] = (TB)(v * a.d_scale);
                     }
+                    if (n < n_end && m_of(i) < a.ldd) put_planes<TB, 8>(a.d, (size_t)n * a.ldd + m_of(i), d);
                 }
             }
-        }
-        if (EPI == XE_DLOGITS && a.db_part) {
+            if (a.db_part) {
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+                for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float v = dbs[i][r];
+                    for (int r = 0; r < 4; ++r) {
+                        float v = dbs[i][r];
 #pragma unroll
-                    for (int x = 1; x < 16; x <<= 1) v += __shfl_xor(v, x);
-                    const long long m = mbase + i * 16 + r;
-                    if (fr == 0 && m < a.rowsA) a.db_part[(size_t)(tn * WN + wn) * a.rowsA + m] = v;
-                }
+                        for (int x = 1; x < 16; x <<= 1) v += __shfl_xor(v, x);
+                        const int m = m_of(i) + r;
+                        if (fr == 0 && m < a.rowsA) a.db_part[(size_t)(tn * WN + wn) * a.rowsA + m] = v;
+                    }
+            }
         }
     } else {
-        const float s = a.out_scale * (a.scale ? *a.scale : 1.f);
+        typedef std::conditional_t<WIDE, float, T> TO;
+        const float s = a.out_scale * *a.scale;
+        const bool final = splits == 1 && (EPI == XE_DW || a.pieces == 1);
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
-            const long long n = nbase + j * 16;
-            if (n >= a.rowsB) continue;
-            const float sn = a.row_scale ? a.row_scale[n] * s : s;
-            const bool zero = a.row_scale && a.row_scale[n] == 0.f;         // (a row without a gradient: 0 whatever the operands hold)
+            const int n = n0 + j * 16;
+            if (n >= rowsB) continue;
+            const size_t row = final && EPI == XE_DX ? a.row_of[n] : n;
 #pragma unroll
             for (int i = 0; i < FM; ++i) {
-                const long long m = mbase + i * 16;
+                const int m = m_of(i);
                 float v[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] = zero ? 0.f : acc[i][j][r] * sn;
-                const size_t at = (size_t)n * a.ldo + m;
-                if (a.slab || a.out_dtype == PHC_DTYPE_F32) {
-                    float *o = static_cast<float *>(a.out) + (a.slab ? (size_t)split * a.slab : 0) + at;
-                    if (a.out_vec && m + 4 <= a.rowsA) {
-                        float4 q = make_float4(v[0], v[1], v[2], v[3]);
+                for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * s;
+                if (final) {
+                    TO *o = static_cast<TO *>(a.out) + row * a.ldo + m;
+                    if (a.out_vec && m + 4 <= a.rowsA) store_pack<TO, 4>(o, v);
+                    else
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (m + r < a.rowsA) o[r] = from_f32<TO>(v[r]);
+                } else {
+                    float *o = a.slabs + ((size_t)split * rowsB + row) * a.ldo + m;
+                    if (a.ldo % 4 == 0 && m + 4 <= a.rowsA) {
                         if (a.accumulate) {
-                            const float4 p = *reinterpret_cast<const float4 *>(o);
-                            q.x += p.x, q.y += p.y, q.z += p.z, q.w += p.w;
+                            float p[4];
+                            load_pack<float, 4>(o, p);
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) v[r] += p[r];
                         }
-                        *reinterpret_cast<float4 *>(o) = q;
+                        store_pack<float, 4>(o, v);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             if (m + r < a.rowsA) o[r] = a.accumulate ? o[r] + v[r] : v[r];
                     }
-                } else {
-                    T *o = static_cast<T *>(a.out) + at;
-                    if (a.out_vec && m + 4 <= a.rowsA) store_pack<T, 4>(o, v);
-                    else
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (m + r < a.rowsA) o[r] = from_f32<T>(v[r]);
                 }
             }
         }
@@ -350,14 +525,15 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------------------------------------
-// A workgroup joins the parts of 64 rows: 16 wavefronts share the parts, then one adds them up.
-__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int parts,
-                                                        long long N, const float *__restrict__ target_logit,
-                                                        const long long *__restrict__ target, long long ignore, float *__restrict__ lse,
+// A workgroup joins the parts of 16 rows: 64 lane groups share the parts, then one adds them up.
+__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int parts, int N,
+                                                        const int *__restrict__ count, const float *__restrict__ target_logit,
+                                                        const int *__restrict__ from, float *__restrict__ lse, float *__restrict__ row_loss,
                                                         float *__restrict__ loss) {
-    __shared__ float sm[16][64], ss[16][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const long long n = (long long)blockIdx.x * 64 + lane;
+    __shared__ float sm[64][16], ss[64][16];
+    const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
+    const int n = blockIdx.x * 16 + c, kept = *count;
+    if (blockIdx.x * 16 >= kept) return;
     float mx = -INFINITY, sum = 0.f;
     auto join = [&](float m, float s) {
         const float top = fmaxf(mx, m);
@@ -365,110 +541,119 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
         sum = sum * expf(mx - shift) + s * expf(m - shift);
         mx = top;
     };
-    if (n < N)
-        for (int p = wave; p < parts; p += 16) join(part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
-    sm[wave][lane] = mx;
-    ss[wave][lane] = sum;
+    if (n < kept)
+        for (int p = group; p < parts; p += 64) join(part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
+    sm[group][c] = mx;
+    ss[group][c] = sum;
     __syncthreads();
-    if (wave == 0 && n < N) {
-        for (int w = 1; w < 16; ++w) join(sm[w][lane], ss[w][lane]);
+    if (group == 0 && n < kept) {
+        for (int w = 1; w < 64; ++w) join(sm[w][c], ss[w][c]);
         const float l = mx + logf(sum);
         lse[n] = l;
-        loss[n] = target[n] == ignore ? 0.f : l - target_logit[n];
+        row_loss[n] = l - target_logit[n];
+        if (loss) loss[from[n]] = l - target_logit[n];
     }
 }
 
-// sum of the rows' losses and the number of rows that count -> out[0] = sum or mean, stat = {sum, count}
-__global__ __launch_bounds__(1024) void xent_reduce_kernel(const float *__restrict__ rows, const long long *__restrict__ target, long long ignore,
-                                                          long long N, int mean, float *__restrict__ out, float *__restrict__ stat) {
-    __shared__ double red[16], cnt[16];
-    double s = 0.0, c = 0.0;
-    for (long long i = threadIdx.x; i < N; i += 1024) {
-        if (target[i] == ignore) continue;
-        s += (double)rows[i];
-        c += 1.0;
-    }
+// sum of the rows' losses -> out[0] = sum or mean, stat = {sum, rows that count}; per row (out is null): zeros for the ignored rows
+__global__ __launch_bounds__(1024) void xent_reduce_kernel(const float *__restrict__ row_loss, const int *__restrict__ count, const int *__restrict__ to,
+                                                          int N, int mean, float *__restrict__ out, float *__restrict__ loss, float *__restrict__ stat) {
+    __shared__ double red[16];
+    const int kept = *count;
+    double s = 0.0;
+    for (int i = threadIdx.x; i < kept; i += 1024) s += (double)row_loss[i];
+    if (loss)
+        for (int i = threadIdx.x; i < N; i += 1024)
+            if (to[i] < 0) loss[i] = 0.f;
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        s += __shfl_xor(s, d);
-        c += __shfl_xor(c, d);
-    }
-    if ((threadIdx.x & 63) == 0) {
-        red[threadIdx.x >> 6] = s;
-        cnt[threadIdx.x >> 6] = c;
-    }
+    for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) {
-            s += red[w];
-            c += cnt[w];
-        }
-        if (out) out[0] = (float)(mean ? s / c : s);          // (no row counts: the mean of nothing is NaN)
+        for (int w = 1; w < 16; ++w) s += red[w];
+        if (out) out[0] = (float)(mean ? s / (double)kept : s);          // (no row counts: the mean of nothing is NaN)
         stat[0] = (float)s;
-        stat[1] = (float)c;
+        stat[1] = (float)kept;
     }
 }
 
-// g_i of every row: row_scale = g_i (dx), top = max |g_i|, row_rel = g_i / top (what the 16-bit d of the weight gradient carry)
-__global__ __launch_bounds__(1024) void xent_scales_kernel(const float *__restrict__ dloss, int per_row, int mean, const float *__restrict__ stat,
-                                                          const long long *__restrict__ target, long long ignore, long long N,
-                                                          float *__restrict__ row_scale, float *__restrict__ row_rel, float *__restrict__ top) {
+// g_i of every packed row: top = max |g_i|, rel = g_i / top (what the rows of d carry; top goes to the products' outputs)
+__global__ __launch_bounds__(1024) void xent_scales_kernel(const float *__restrict__ dloss, int per_row, int mean, const int *__restrict__ count,
+                                                          const int *__restrict__ from, float *__restrict__ rel, float *__restrict__ top) {
     __shared__ float red[16];
-    const float count = stat[1];
-    auto g_of = [&](long long i) {
-        if (target[i] == ignore) return 0.f;
-        const float g = per_row ? dloss[i] : dloss[0];
-        return mean ? g / count : g;
-    };
+    const int kept = *count;
+    auto g_of = [&](int i) { return per_row ? dloss[from[i]] : mean ? dloss[0] / (float)kept : dloss[0]; };
     float m = 0.f;
-    for (long long i = threadIdx.x; i < N; i += 1024) m = fmaxf(m, fabsf(g_of(i)));
+    for (int i = threadIdx.x; i < kept; i += 1024) m = fmaxf(m, fabsf(g_of(i)));
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     for (int w = 0; w < 16; ++w) m = fmaxf(m, red[w]);
     if (threadIdx.x == 0) *top = m;
-    for (long long i = threadIdx.x; i < N; i += 1024) {
+    for (int i = threadIdx.x; i < kept; i += 1024) {
         const float g = g_of(i);
-        row_scale[i] = g;
-        row_rel[i] = g == 0.f ? 0.f : g / m;
+        rel[i] = g == 0.f ? 0.f : g / m;
     }
 }
 
-// out[i] = sum over the slabs, in order
+// The splits' partial outputs in order.  dx: rows go back to their places; dW: nothing to do where one split wrote the result.
 template <typename T>
-__global__ __launch_bounds__(256) void xent_sum_slabs_kernel(const float *__restrict__ slabs, long long slab, int n, long long count,
-                                                            const float *__restrict__ scale, T *__restrict__ out) {
-    const float f = scale ? *scale : 1.f;
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < count; e += (long long)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void xent_sum_slabs_kernel(const float *__restrict__ slabs, const int *__restrict__ count, int rows_static, int tilesM,
+                                                            int TN, int split_steps, int segments, int max_blocks, int D, int pieces,
+                                                            const int *__restrict__ row_of, T *__restrict__ out) {
+    const int rows = row_of ? *count : rows_static;
+    const int steps = segments * (row_of ? split_steps : (*count + XT_BK - 1) / XT_BK);
+    const int n = xt_splits(tilesM * ((rows + TN - 1) / TN), steps, max_blocks);
+    if (n == 1 && (!row_of || pieces == 1)) return;
+    const long long total = (long long)rows * D;
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
         float v = slabs[e];
-        for (int s = 1; s < n; ++s) v += slabs[(size_t)s * slab + e];
-        out[e] = from_f32<T>(v * f);
+        for (int s = 1; s < n; ++s) v += slabs[(size_t)s * total + e];
+        const long long r = e / D;
+        out[row_of ? (long long)row_of[r] * D + (e - r * D) : e] = from_f32<T>(v);
     }
+}
+
+// db[v] = top sum over the tiles along n of their partial sums
+template <typename T>
+__global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ part, const int *__restrict__ count, int TN, int WN, int nv,
+                                                     const float *__restrict__ top, T *__restrict__ db) {
+    const int v = blockIdx.x * 256 + threadIdx.x;
+    if (v >= nv) return;
+    const int n = (*count + TN - 1) / TN * WN;
+    float s = 0.f;
+    for (int i = 0; i < n; ++i) s += part[(size_t)i * nv + v];
+    db[v] = from_f32<T>(s * *top);
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------------
 static long long round_up(long long v, long long m) { return (v + m - 1) / m * m; }
 static long long ceil_div(long long v, long long m) { return (v + m - 1) / m; }
 
-constexpr long long XT_PIECE_BYTES = 256ll << 20;      // both orders of a piece's d together: what the Infinity Cache holds
+constexpr long long XT_PIECE_BYTES = 128ll << 20;      // a piece's d: half of the Infinity Cache, W and x beside it
+
+// Tiles of 256 x 256 by 8 wavefronts (one workgroup on a CU) or 128 x 128 by 4 (two)
+struct Tile256 {
+    static constexpr int WM = 2, WN = 4, FM = 8, FN = 4, SIZE = 256, BLOCKS = 256;
+};
+struct Tile128 {
+    static constexpr int WM = 2, WN = 2, FM = 4, FN = 4, SIZE = 128, BLOCKS = 512;
+};
 
 struct XPlan {
     bool wide;                 // fp32 inputs
     int planes, segments;
     long long Kp, Np, piece, pieces;
-    bool pack_x, pack_w;
-    long long parts;
-    int splits_dx, splits_dw;
+    bool pack_w;
+    bool big_fwd, big_d, big_dx, big_dw;       // 256 x 256 tiles
+    long long wcols;           // readable columns of W's operand rows
 };
 
-constexpr int TILE = 128;
-
-static int splits_for(long long tiles, long long steps) {
-    // enough workgroups for the 256 CUs twice over, at least 8 steps each
-    long long s = ceil_div(512, tiles);
-    if (s > steps / 8) s = steps / 8;
-    return (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+static bool big_tiles(long long m, long long n, bool splits) {
+    // the large tile needs fewer operand bytes per product, and fills the card only with enough of them
+    const long long t = ceil_div(m, 256) * ceil_div(n, 256);
+    return m > 128 && n > 128 && (splits ? t >= 32 : t >= 192);
 }
 
 static XPlan make_plan(const phc_linear_xent_desc *d) {
@@ -478,54 +663,61 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     p.segments = p.wide ? 6 : 1;
     p.Kp = round_up(d->D, XT_BK);
     p.Np = round_up(d->N, XT_BK);
-    // an operand is read where it lies when its rows are whole steps and 16-byte aligned
-    p.pack_x = p.wide || d->D % XT_BK || d->ldx % 8 || !aligned_to(d->x, 16);
+    // W is read where it lies when its rows are whole steps and 16-byte aligned
     p.pack_w = p.wide || d->D % XT_BK || d->ldw % 8 || !aligned_to(d->W, 16);
-    p.parts = ceil_div(d->V, TILE) * 2;
-    long long piece = XT_PIECE_BYTES / (4 * p.planes * (d->N > 0 ? d->N : 1)) / 256 * 256;
+    p.wcols = p.Kp;
+    long long piece = XT_PIECE_BYTES / (2 * p.planes * (d->N > 0 ? d->N : 1)) / 256 * 256;
     if (piece < 2048) piece = 2048;
     if (d->piece > 0) piece = round_up(d->piece, 64);
     if (piece >= d->V) piece = round_up(d->V, 64);
     p.pieces = ceil_div(d->V, piece);
     p.piece = d->piece > 0 ? piece : round_up(ceil_div(d->V, p.pieces), 64);
     p.pieces = ceil_div(d->V, p.piece);
-    p.splits_dx = splits_for(ceil_div(d->D, TILE) * ceil_div(d->N, TILE), p.segments * (p.piece / XT_BK));
-    p.splits_dw = splits_for(ceil_div(d->D, TILE) * ceil_div(p.piece, TILE), p.segments * (p.Np / XT_BK));
+    p.big_fwd = big_tiles(d->V, d->N, false);
+    p.big_d = big_tiles(p.piece, d->N, false);
+    p.big_dx = big_tiles(d->D, d->N, true);
+    p.big_dw = big_tiles(d->D, p.piece, true);
     return p;
 }
 
+static size_t slab_floats(long long rows, long long D, bool big, bool keeps) {
+    // splits exist only while tiles * splits stays within the blocks of one launch
+    const size_t tile = big ? Tile256::SIZE : Tile128::SIZE, blocks = big ? Tile256::BLOCKS : Tile128::BLOCKS;
+    const size_t most = blocks * tile * tile;
+    const size_t all = (size_t)rows * D;
+    return keeps ? (all > most ? all : most) : most;
+}
+
 struct XWs {
-    XPlanes x{}, w{}, xT{}, wT{}, dl{}, dlT{};
-    float *part_max = nullptr, *part_sum = nullptr, *target_logit = nullptr, *rows = nullptr;
-    float *row_scale = nullptr, *row_rel = nullptr, *top = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr, *db_part = nullptr;
+    XRows rows{};
+    XPlanes x{}, w{}, dl{};
+    float *part_max = nullptr, *part_sum = nullptr, *target_logit = nullptr, *row_loss = nullptr;
+    float *rel = nullptr, *top = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr, *db_part = nullptr;
     size_t bytes;
     XWs(const phc_linear_xent_desc *d, const XPlan &p, bool backward, void *ws) {
         Carve c(ws);
         auto planes = [&](XPlanes &o, size_t count) {
             for (int i = 0; i < p.planes; ++i) o.p[i] = c.take<unsigned short>(count);
         };
-        if (p.pack_x) planes(x, (size_t)d->N * p.Kp);
+        rows.count = c.take<int>(1);
+        rows.from = c.take<int>(d->N);
+        rows.to = c.take<int>(d->N);
+        rows.target = c.take<int>(d->N);
+        planes(x, (size_t)p.Np * p.Kp);
         if (p.pack_w) planes(w, (size_t)(backward ? p.piece : d->V) * p.Kp);
         if (!backward) {
-            part_max = c.take<float>((size_t)p.parts * d->N);
-            part_sum = c.take<float>((size_t)p.parts * d->N);
+            const size_t parts = ceil_div(d->V, p.big_fwd ? 256 : 128);
+            part_max = c.take<float>(parts * d->N);
+            part_sum = c.take<float>(parts * d->N);
             target_logit = c.take<float>(d->N);
-            rows = c.take<float>(d->N);
+            row_loss = c.take<float>(d->N);
         } else {
-            row_scale = c.take<float>(d->N);
-            row_rel = c.take<float>(d->N);
+            rel = c.take<float>(d->N);
             top = c.take<float>(1);
-            planes(dl, (size_t)d->N * p.piece);
-            planes(dlT, (size_t)p.piece * p.Np);
-            if (d->dx) {
-                planes(wT, (size_t)d->D * p.piece);
-                if (p.splits_dx > 1 || p.pieces > 1) dx_slabs = c.take<float>((size_t)p.splits_dx * d->N * d->D);
-            }
-            if (d->dW) {
-                planes(xT, (size_t)d->D * p.Np);
-                if (p.splits_dw > 1) dw_slabs = c.take<float>((size_t)p.splits_dw * p.piece * d->D);
-            }
-            if (d->db) db_part = c.take<float>((size_t)ceil_div(d->N, TILE) * 2 * p.piece);
+            planes(dl, (size_t)p.Np * p.piece);
+            if (d->dx) dx_slabs = c.take<float>(slab_floats(d->N, d->D, p.big_dx, p.pieces > 1));
+            if (d->dW) dw_slabs = c.take<float>(slab_floats(p.piece, d->D, p.big_dw, false));
+            if (d->db) db_part = c.take<float>((size_t)(p.big_d ? ceil_div(d->N, 256) * Tile256::WN : ceil_div(d->N, 128) * Tile128::WN) * p.piece);
         }
         bytes = c.used;
     }
@@ -536,26 +728,18 @@ static unsigned flat_grid(long long n) {
     return (unsigned)(b < 1 ? 1 : b > 8192 ? 8192 : b);
 }
 
-static void pack(const phc_linear_xent_desc *d, const void *src, long long ld, long long R, int C, long long Cp, const XPlanes &out, hipStream_t s) {
-    const dim3 g(flat_grid(R * Cp));
-    if (d->dtype == PHC_DTYPE_F32)
-        PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_pack_kernel<float>), g, dim3(256), 0, s, static_cast<const float *>(src), ld, R, C, (int)Cp, out);
-    else if (d->dtype == PHC_DTYPE_BF16)
-        PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_pack_kernel<bf16_t>), g, dim3(256), 0, s, static_cast<const bf16_t *>(src), ld, R, C, (int)Cp, out);
-    else
-        PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_pack_kernel<f16_t>), g, dim3(256), 0, s, static_cast<const f16_t *>(src), ld, R, C, (int)Cp, out);
+template <typename T>
+static void pack_as(const void *src, long long ld, long long R, long long C, long long Cp, const XRows *rows, void *zero, const XPlanes &out, hipStream_t s) {
+    const int vec = aligned_to(src, 16) && (ld * sizeof(T)) % 16 == 0;
+    PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_pack_kernel<T>), dim3(flat_grid((R + (rows ? XT_BK : 0)) * (Cp / 8))), dim3(256), 0, s, static_cast<const T *>(src), ld,
+                  R, (int)C, (int)Cp, vec, rows ? (const int *)rows->to : (const int *)nullptr, rows ? (const int *)rows->count : (const int *)nullptr,
+                  static_cast<T *>(zero), out);
 }
-
-static void transpose(const phc_linear_xent_desc *d, const void *src, long long ld, long long R, int C, long long Rp, const long long *target,
-                      const XPlanes &out, hipStream_t s) {
-    const dim3 g((unsigned)ceil_div(Rp, 64), (unsigned)ceil_div(C, 64));
-    const long long ig = d->ignore_index;
-    if (d->dtype == PHC_DTYPE_F32)
-        PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_transpose_kernel<float>), g, dim3(256), 0, s, static_cast<const float *>(src), ld, R, C, Rp, target, ig, out);
-    else if (d->dtype == PHC_DTYPE_BF16)
-        PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_transpose_kernel<bf16_t>), g, dim3(256), 0, s, static_cast<const bf16_t *>(src), ld, R, C, Rp, target, ig, out);
-    else
-        PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_transpose_kernel<f16_t>), g, dim3(256), 0, s, static_cast<const f16_t *>(src), ld, R, C, Rp, target, ig, out);
+static void pack(int dtype, const void *src, long long ld, long long R, long long C, long long Cp, const XRows *rows, void *zero, const XPlanes &out,
+                 hipStream_t s) {
+    if (dtype == PHC_DTYPE_F32) pack_as<float>(src, ld, R, C, Cp, rows, zero, out, s);
+    else if (dtype == PHC_DTYPE_BF16) pack_as<bf16_t>(src, ld, R, C, Cp, rows, zero, out, s);
+    else pack_as<f16_t>(src, ld, R, C, Cp, rows, zero, out, s);
 }
 
 static void set_planes(const XPlan &p, const XPlanes &A, const XPlanes &B, XGemm *g) {
@@ -567,31 +751,44 @@ static void set_planes(const XPlan &p, const XPlanes &A, const XPlanes &B, XGemm
     }
 }
 
-template <typename T, int EPI, bool WIDE>
+template <typename T, int EPI, bool WIDE, typename TILE>
 static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
-    constexpr int WM = 2, WN = 2, FM = 4, FN = 4, LDS = 2 * (WM * FM + WN * FN) * 16 * 128;
-    g.tilesM = (int)ceil_div(g.rowsA, WM * FM * 16);
-    g.tilesN = (int)ceil_div(g.rowsB, WN * FN * 16);
-    if (!ensure_dynamic_lds(xent_gemm_kernel<T, EPI, WIDE, WM, WN, FM, FN>, LDS)) return false;
-    PHC_LAUNCH_AS(kid, (xent_gemm_kernel<T, EPI, WIDE, WM, WN, FM, FN>), dim3((unsigned)(g.tilesM * g.tilesN * g.splits)), dim3(WM * WN * 64), LDS, s, g);
+    constexpr int LDS = 4 * TILE::SIZE * 128;
+    g.tilesM = (int)ceil_div(g.rowsA, TILE::SIZE);
+    g.tilesN = (int)ceil_div(g.rowsB, TILE::SIZE);
+    g.max_blocks = TILE::BLOCKS;
+    auto kernel = xent_gemm_kernel<T, EPI, WIDE, TILE::WM, TILE::WN, TILE::FM, TILE::FN>;
+    if (!ensure_dynamic_lds(kernel, LDS)) return false;
+    long long blocks = (long long)g.tilesM * g.tilesN;
+    if ((EPI == XE_DX || EPI == XE_DW) && blocks < TILE::BLOCKS) blocks = TILE::BLOCKS;
+    PHC_LAUNCH_AS(kid, kernel, dim3((unsigned)blocks), dim3(TILE::WM * TILE::WN * 64), LDS, s, g);
     return true;
 }
 template <int EPI>
-static bool gemm(const phc_linear_xent_desc *d, int kid, XGemm &g, hipStream_t s) {
-    if (d->dtype == PHC_DTYPE_F32) return launch_gemm<bf16_t, EPI, true>(kid, g, s);
-    if (d->dtype == PHC_DTYPE_BF16) return launch_gemm<bf16_t, EPI, false>(kid, g, s);
-    return launch_gemm<f16_t, EPI, false>(kid, g, s);
+static int gemm(const phc_linear_xent_desc *d, int kid, bool big, XGemm &g, hipStream_t s) {
+    bool ok;
+    if (d->dtype == PHC_DTYPE_F32) ok = big ? launch_gemm<bf16_t, EPI, true, Tile256>(kid, g, s) : launch_gemm<bf16_t, EPI, true, Tile128>(kid, g, s);
+    else if (d->dtype == PHC_DTYPE_BF16) ok = big ? launch_gemm<bf16_t, EPI, false, Tile256>(kid, g, s) : launch_gemm<bf16_t, EPI, false, Tile128>(kid, g, s);
+    else ok = big ? launch_gemm<f16_t, EPI, false, Tile256>(kid, g, s) : launch_gemm<f16_t, EPI, false, Tile128>(kid, g, s);
+    PHC_REQUIRE(ok, PHC_ERR_LAUNCH, "phc_linear_xent: the runtime refused the kernel's LDS size");
+    return PHC_OK;
 }
 
-static void sum_slabs(const phc_linear_xent_desc *d, int kid, const float *slabs, long long slab, int n, long long count, const float *scale, void *out,
-                      hipStream_t s) {
-    const dim3 g(flat_grid(count));
-    if (d->dtype == PHC_DTYPE_F32)
-        PHC_LAUNCH_AS(kid, (xent_sum_slabs_kernel<float>), g, dim3(256), 0, s, slabs, slab, n, count, scale, static_cast<float *>(out));
-    else if (d->dtype == PHC_DTYPE_BF16)
-        PHC_LAUNCH_AS(kid, (xent_sum_slabs_kernel<bf16_t>), g, dim3(256), 0, s, slabs, slab, n, count, scale, static_cast<bf16_t *>(out));
-    else
-        PHC_LAUNCH_AS(kid, (xent_sum_slabs_kernel<f16_t>), g, dim3(256), 0, s, slabs, slab, n, count, scale, static_cast<f16_t *>(out));
+template <typename T>
+static void sum_slabs_as(int kid, const float *slabs, const XGemm &g, int tile, int pieces, void *out, hipStream_t s) {
+    PHC_LAUNCH_AS(kid, (xent_sum_slabs_kernel<T>), dim3(flat_grid((long long)g.rowsB * g.ldo)), dim3(256), 0, s, slabs, g.count, g.rowsB, g.tilesM, tile,
+                  g.split_k / XT_BK, g.segments, g.max_blocks, g.ldo, pieces, g.row_of, static_cast<T *>(out));
+}
+static void sum_slabs(int dtype, int kid, const float *slabs, const XGemm &g, int tile, int pieces, void *out, hipStream_t s) {
+    if (dtype == PHC_DTYPE_F32) sum_slabs_as<float>(kid, slabs, g, tile, pieces, out, s);
+    else if (dtype == PHC_DTYPE_BF16) sum_slabs_as<bf16_t>(kid, slabs, g, tile, pieces, out, s);
+    else sum_slabs_as<f16_t>(kid, slabs, g, tile, pieces, out, s);
+}
+
+template <typename T>
+static void db_as(const float *part, const XRows &r, int TN, int WN, int nv, const float *top, void *db, hipStream_t s) {
+    PHC_LAUNCH_AS(K_XENT_DW, (xent_db_kernel<T>), dim3((unsigned)ceil_div(nv, 256)), dim3(256), 0, s, part, (const int *)r.count, TN, WN, nv, top,
+                  static_cast<T *>(db));
 }
 
 static int xent_check(const char *who, const phc_linear_xent_desc *d) {
@@ -626,42 +823,34 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     const XPlan p = make_plan(d);
     XWs w(d, p, false, d->ws);
-    const int es = dtype_bytes(d->dtype);
-    XPlanes X{{const_cast<void *>(d->x)}}, W{{const_cast<void *>(d->W)}};
-    long long ldx = d->ldx * es, ldw = d->ldw * es;
-    if (p.pack_x) {
-        pack(d, d->x, d->ldx, d->N, (int)d->D, p.Kp, w.x, s);
-        X = w.x;
-        ldx = p.Kp * 2;
-    }
+    const int es = dtype_bytes(d->dtype), N = (int)d->N;
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_that_count_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const long long *>(d->target),
+                  (long long)d->ignore_index, N, (long long)d->V, err_word(), w.rows);
+    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &w.rows, nullptr, w.x, s);
+    XPlanes W{{const_cast<void *>(d->W)}};
     if (p.pack_w) {
-        pack(d, d->W, d->ldw, d->V, (int)d->D, p.Kp, w.w, s);
+        pack(d->dtype, d->W, d->ldw, d->V, d->D, p.Kp, nullptr, nullptr, w.w, s);
         W = w.w;
-        ldw = p.Kp * 2;
     }
     XGemm g{};
-    set_planes(p, W, X, &g);
-    g.ksteps = (int)(p.Kp / XT_BK);
-    g.lda = (unsigned)ldw;
-    g.ldb = (unsigned)ldx;
-    g.rowsA = d->V;
-    g.rowsB = d->N;
-    g.splits = 1;
+    set_planes(p, W, w.x, &g);
+    g.K = p.Kp;
+    g.lda = (unsigned)(p.pack_w ? p.Kp * 2 : d->ldw * es);
+    g.ldb = (unsigned)(p.Kp * 2);
+    g.rowsA = (int)d->V;
+    g.rowsB = g.N = N;
+    g.count = w.rows.count;
     g.bias = d->bias;
-    g.bias_f32 = p.wide;
-    g.target = reinterpret_cast<const long long *>(d->target);
-    g.ignore = d->ignore_index;
-    g.vocab = d->V;
-    g.err = err_word();
+    g.target = w.rows.target;
     g.part_max = w.part_max;
     g.part_sum = w.part_sum;
     g.target_logit = w.target_logit;
-    PHC_REQUIRE(gemm<XE_STATS>(d, K_XENT_LOGITS, g, s), PHC_ERR_LAUNCH, "phc_linear_xent_fwd: LDS size refused");
-    float *rows = d->reduction == 0 ? d->loss : w.rows;
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_kernel, dim3((unsigned)ceil_div(d->N, 64)), dim3(1024), 0, s, (const float *)w.part_max,
-                  (const float *)w.part_sum, (int)p.parts, (long long)d->N, (const float *)w.target_logit, g.target, g.ignore, d->lse, rows);
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_reduce_kernel, dim3(1), dim3(1024), 0, s, (const float *)rows, g.target, g.ignore, (long long)d->N,
-                  d->reduction == 2 ? 1 : 0, d->reduction == 0 ? (float *)nullptr : d->loss, d->stat);
+    if (int rc = gemm<XE_STATS>(d, K_XENT_LOGITS, p.big_fwd, g, s)) return rc;
+    float *loss = d->reduction == PHC_REDUCE_NONE ? d->loss : nullptr;
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_kernel, dim3((unsigned)ceil_div(N, 16)), dim3(1024), 0, s, (const float *)w.part_max, (const float *)w.part_sum,
+                  g.tilesM, N, g.count, (const float *)w.target_logit, (const int *)w.rows.from, d->lse, w.row_loss, loss);
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_reduce_kernel, dim3(1), dim3(1024), 0, s, (const float *)w.row_loss, g.count, (const int *)w.rows.to, N,
+                  d->reduction == PHC_REDUCE_MEAN ? 1 : 0, loss ? (float *)nullptr : d->loss, loss, d->stat);
     return launch_status("phc_linear_xent_fwd");
 }
 
@@ -674,95 +863,93 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     const XPlan p = make_plan(d);
     XWs w(d, p, true, d->ws);
-    const int es = dtype_bytes(d->dtype);
-    const long long *target = reinterpret_cast<const long long *>(d->target);
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_scales_kernel, dim3(1), dim3(1024), 0, s, d->dloss, d->reduction == 0 ? 1 : 0, d->reduction == 2 ? 1 : 0,
-                  (const float *)d->stat, target, (long long)d->ignore_index, (long long)d->N, w.row_scale, w.row_rel, w.top);
+    const int es = dtype_bytes(d->dtype), N = (int)d->N;
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_that_count_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const long long *>(d->target),
+                  (long long)d->ignore_index, N, (long long)d->V, (int *)nullptr, w.rows);
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_scales_kernel, dim3(1), dim3(1024), 0, s, d->dloss, d->reduction == PHC_REDUCE_NONE ? 1 : 0,
+                  d->reduction == PHC_REDUCE_MEAN ? 1 : 0, (const int *)w.rows.count, (const int *)w.rows.from, w.rel, w.top);
+    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &w.rows, d->dx, w.x, s);
     // fp16 has no normal values below 6e-5, where most probabilities of a large vocabulary lie: its d are stored times 2^14
     const float d_scale = d->dtype == PHC_DTYPE_F16 ? 16384.f : 1.f;
-    XPlanes X{{const_cast<void *>(d->x)}};
-    long long ldx = d->ldx * es;
-    if (p.pack_x) {
-        pack(d, d->x, d->ldx, d->N, (int)d->D, p.Kp, w.x, s);
-        X = w.x;
-        ldx = p.Kp * 2;
-    }
-    if (d->dW) transpose(d, d->x, d->ldx, d->N, (int)d->D, p.Np, target, w.xT, s);
+    XGemm o{};                                                   // (the last piece's dx product: its splits are joined at the end)
     for (long long v0 = 0; v0 < d->V; v0 += p.piece) {
-        const long long nv = d->V - v0 < p.piece ? d->V - v0 : p.piece, nvp = round_up(nv, XT_BK);
+        const int nv = (int)(d->V - v0 < p.piece ? d->V - v0 : p.piece), nvp = (int)round_up(nv, XT_BK);
         const char *Wv = static_cast<const char *>(d->W) + (size_t)v0 * d->ldw * es;
         XPlanes W{{const_cast<char *>(Wv)}};
-        long long ldw = d->ldw * es;
         if (p.pack_w) {
-            pack(d, Wv, d->ldw, nv, (int)d->D, p.Kp, w.w, s);
+            pack(d->dtype, Wv, d->ldw, nv, d->D, p.Kp, nullptr, nullptr, w.w, s);
             W = w.w;
-            ldw = p.Kp * 2;
         }
+        const unsigned ldw = (unsigned)(p.pack_w ? p.Kp * 2 : d->ldw * es);
         XGemm g{};
-        set_planes(p, W, X, &g);
-        g.ksteps = (int)(p.Kp / XT_BK);
-        g.lda = (unsigned)ldw;
-        g.ldb = (unsigned)ldx;
+        set_planes(p, W, w.x, &g);
+        g.K = p.Kp;
+        g.lda = ldw;
+        g.ldb = (unsigned)(p.Kp * 2);
         g.rowsA = nv;
-        g.rowsB = d->N;
-        g.splits = 1;
+        g.rowsB = g.N = N;
+        g.count = w.rows.count;
         g.bias = d->bias ? static_cast<const char *>(d->bias) + (size_t)v0 * es : nullptr;
-        g.bias_f32 = p.wide;
-        g.target = target;
-        g.ignore = d->ignore_index;
-        g.first_v = v0;
-        g.vocab = d->V;
+        g.target = w.rows.target;
+        g.first_v = (int)v0;
         g.lse = d->lse;
-        g.row_rel = w.row_rel;
+        g.rel = w.rel;
         g.d = w.dl;
-        g.dT = w.dlT;
         g.ldd = nvp;
-        g.lddT = p.Np;
         g.d_scale = d_scale;
         g.db_part = d->db ? w.db_part : nullptr;
-        PHC_REQUIRE(gemm<XE_DLOGITS>(d, K_XENT_DLOGITS, g, s), PHC_ERR_LAUNCH, "phc_linear_xent_bwd: LDS size refused");
-        if (d->db)
-            sum_slabs(d, K_XENT_DW, w.db_part, nv, (int)(ceil_div(d->N, TILE) * 2), nv, w.top, static_cast<char *>(d->db) + (size_t)v0 * es, s);
-        if (d->dx) {
-            transpose(d, Wv, d->ldw, nv, (int)d->D, nvp, nullptr, w.wT, s);
-            XGemm o{};
-            set_planes(p, w.wT, w.dl, &o);
-            o.ksteps = (int)(nvp / XT_BK);
-            o.lda = o.ldb = (unsigned)(nvp * 2);
-            o.rowsA = d->D;
-            o.rowsB = d->N;
-            o.splits = p.splits_dx;
-            o.row_scale = w.row_scale;
-            o.out_scale = 1.f / d_scale;
-            o.out = w.dx_slabs ? static_cast<void *>(w.dx_slabs) : d->dx;
-            o.ldo = d->D;
-            o.slab = w.dx_slabs ? (long long)d->N * d->D : 0;
-            o.accumulate = v0 > 0;
-            o.out_dtype = d->dtype;
-            o.out_vec = d->D % 4 == 0 && (w.dx_slabs || aligned_to(d->dx, 4 * es));
-            PHC_REQUIRE(gemm<XE_OUT>(d, K_XENT_DX, o, s), PHC_ERR_LAUNCH, "phc_linear_xent_bwd: LDS size refused");
+        if (int rc = gemm<XE_DLOGITS>(d, K_XENT_DLOGITS, p.big_d, g, s)) return rc;
+        if (d->db) {
+            const int TN = p.big_d ? 256 : 128, WN = p.big_d ? Tile256::WN : Tile128::WN;
+            char *db = static_cast<char *>(d->db) + (size_t)v0 * es;
+            if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, w.rows, TN, WN, nv, w.top, db, s);
+            else if (d->dtype == PHC_DTYPE_BF16) db_as<bf16_t>(w.db_part, w.rows, TN, WN, nv, w.top, db, s);
+            else db_as<f16_t>(w.db_part, w.rows, TN, WN, nv, w.top, db, s);
         }
-        if (d->dW) {
-            XGemm o{};
-            set_planes(p, w.xT, w.dlT, &o);
-            o.ksteps = (int)(p.Np / XT_BK);
-            o.lda = o.ldb = (unsigned)(p.Np * 2);
-            o.rowsA = d->D;
-            o.rowsB = nv;
-            o.splits = p.splits_dw;
+        if (d->dx) {
+            o = XGemm{};
+            set_planes(p, W, w.dl, &o);
+            o.K = nv;
+            o.split_k = (int)p.piece;
+            o.lda = ldw;
+            o.ldb = (unsigned)(nvp * 2);
+            o.rowsA = (int)d->D;
+            o.colsA = (int)p.wcols;
+            o.rowsB = N;
+            o.count = w.rows.count;
             o.scale = w.top;
             o.out_scale = 1.f / d_scale;
-            char *out = static_cast<char *>(d->dW) + (size_t)v0 * d->D * es;
-            o.out = w.dw_slabs ? static_cast<void *>(w.dw_slabs) : out;
-            o.ldo = d->D;
-            o.slab = w.dw_slabs ? nv * d->D : 0;
-            o.out_dtype = d->dtype;
-            o.out_vec = d->D % 4 == 0 && (w.dw_slabs || aligned_to(d->dW, 4 * es));
-            PHC_REQUIRE(gemm<XE_OUT>(d, K_XENT_DW, o, s), PHC_ERR_LAUNCH, "phc_linear_xent_bwd: LDS size refused");
-            if (w.dw_slabs) sum_slabs(d, K_XENT_DW, w.dw_slabs, o.slab, p.splits_dw, nv * d->D, nullptr, out, s);
+            o.row_of = w.rows.from;
+            o.out = d->dx;
+            o.ldo = (int)d->D;
+            o.slabs = w.dx_slabs;
+            o.accumulate = v0 > 0;
+            o.pieces = (int)p.pieces;
+            o.out_vec = d->D % 4 == 0 && aligned_to(d->dx, 4 * es);
+            if (int rc = gemm<XE_DX>(d, K_XENT_DX, p.big_dx, o, s)) return rc;
+        }
+        if (d->dW) {
+            XGemm q{};
+            set_planes(p, w.x, w.dl, &q);
+            q.lda = (unsigned)(p.Kp * 2);
+            q.ldb = (unsigned)(nvp * 2);
+            q.rowsA = (int)d->D;
+            q.colsA = (int)p.Kp;
+            q.rowsB = nv;
+            q.count = w.rows.count;
+            q.scale = w.top;
+            q.out_scale = 1.f / d_scale;
+            q.out = static_cast<char *>(d->dW) + (size_t)v0 * d->D * es;
+            q.ldo = (int)d->D;
+            q.slabs = w.dw_slabs;
+            q.pieces = 1;
+            q.out_vec = d->D % 4 == 0 && aligned_to(d->dW, 4 * es);
+            if (int rc = gemm<XE_DW>(d, K_XENT_DW, p.big_dw, q, s)) return rc;
+            if ((long long)q.tilesM * q.tilesN * 2 <= q.max_blocks)
+                sum_slabs(d->dtype, K_XENT_DW, w.dw_slabs, q, p.big_dw ? 256 : 128, 1, q.out, s);
         }
     }
-    if (d->dx && w.dx_slabs) sum_slabs(d, K_XENT_DX, w.dx_slabs, (long long)d->N * d->D, p.splits_dx, (long long)d->N * d->D, nullptr, d->dx, s);
+    if (d->dx) sum_slabs(d->dtype, K_XENT_DX, w.dx_slabs, o, p.big_dx ? 256 : 128, (int)p.pieces, d->dx, s);
     return launch_status("phc_linear_xent_bwd");
 }
 

@@ -25,8 +25,8 @@ def _formula(x, w, b, t, reduction, up, ignore=-100):
 
     Logits: exact products of the inputs added in fp32, d + 1 roundings of at most 2^-24 of the sum of magnitudes A (for fp32 inputs the
     split's dropped terms add 3 * 2^-25 A and there are six sums: 7 (d + 1) + 2 in all is above it).  exp: relative error of the argument's error
-    plus 2^-24 (|argument| + 4) of its own rounding.  d is rounded to the operand type (half a step; fp16's are stored times 2^14, so
-    their subnormal step is 2^-24 / 2^14; fp32 is split to 2^-25).  A gradient is a sum of K products in fp32: K roundings of 2^-24 of the sum
+    plus 2^-24 (|argument| + 4) of its own rounding.  d g / max |g| is rounded to the operand type (half a step; fp16's are stored times 2^14,
+    so their subnormal half step is 2^-25 / 2^14; fp32 is split to 2^-25).  A gradient is a sum of K products in fp32: K roundings of 2^-24 of the sum
     of magnitudes (six sums for fp32 inputs), a few more of the scales, and the rounding to its type."""
     X, W = x.double(), w.double()
     n, d = X.shape
@@ -62,18 +62,16 @@ def _formula(x, w, b, t, reduction, up, ignore=-100):
     D[~kept] = 0
     half = torch.finfo(x.dtype).eps / 2 if not wide else 2.0 ** -25
     tiny = 2.0 ** -39 if x.dtype == torch.float16 else 2.0 ** -130
-    e_d = p * (ez + e_lse[:, None] + ((z - lse[:, None]).abs().clamp(max=110) + 6) * U32) + D.abs() * (half + 4 * U32) + tiny
-    e_d[~kept] = 0
-    top = g.abs().max()
-    e_dw = e_d * g.abs()[:, None] + (D * g[:, None]).abs() * 4 * U32 + (tiny * top if x.dtype == torch.float16 else 0)
-    e_dw[~kept] = 0
+    e_d = p * (ez + e_lse[:, None] + ((z - lse[:, None]).abs().clamp(max=110) + 6) * U32) + D.abs() * (half + 4 * U32)
+    e_dg = e_d * g.abs()[:, None] + (D * g[:, None]).abs() * 4 * U32 + tiny * g.abs().max()
+    e_dg[~kept] = 0
     final = torch.finfo(x.dtype).eps / 2
     ftiny = {torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -134, torch.float32: 2.0 ** -149}[x.dtype]
     DG = D * g[:, None]
     dx, dw, db = DG @ W, DG.t() @ X, DG.sum(dim=0)
-    b_dx = (e_d * g.abs()[:, None]) @ W.abs() + DG.abs() @ W.abs() * (sums * (v + 2) + 8) * U32 + dx.abs() * final * 1.01 + ftiny
-    b_dw = e_dw.t() @ X.abs() + DG.t().abs() @ X.abs() * (sums * (n + 2) + 8) * U32 + dw.abs() * final * 1.01 + ftiny
-    b_db = e_dw.sum(dim=0) + DG.abs().sum(dim=0) * (n + 8) * U32 + db.abs() * final * 1.01 + ftiny
+    b_dx = e_dg @ W.abs() + DG.abs() @ W.abs() * (sums * (v + 2) + 8) * U32 + dx.abs() * final * 1.01 + ftiny
+    b_dw = e_dg.t() @ X.abs() + DG.t().abs() @ X.abs() * (sums * (n + 2) + 8) * U32 + dw.abs() * final * 1.01 + ftiny
+    b_db = e_dg.sum(dim=0) + DG.abs().sum(dim=0) * (n + 8) * U32 + db.abs() * final * 1.01 + ftiny
     return (out, dx, dw, db), (e_out * 1.01, b_dx * 1.01, b_dw * 1.01, b_db * 1.01)
 
 
