@@ -1236,11 +1236,11 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
  * x [N, D] (rows ldx apart), W [V, D] (rows ldw apart), bias [V] or NULL, target int64 [N].  A target outside [0, V) counts as 0 and
  * sets PHC_IDX_ERR_TARGET.  A bias of -inf takes a column out.  fp32 operands are expected to be finite: they are multiplied as sums of
  * three 16-bit terms (accuracy of fp32).  Bitwise reproducible.
- *   fwd writes loss ([N], or one value for sum and mean; the mean of no rows is NaN), stat {sum, rows that count} and lse (room for N
- *   values: logsumexp of the rows that count, in their order);
- *   bwd reads the forward's lse and dloss (fp32, [N] or one value), and writes whichever of dx [N, D], dW [V, D], db [V]
+ *   fwd writes loss ([N], or one value for sum and mean; the mean of no rows is NaN) and state (phc_linear_xent_state_bytes(N) bytes,
+ *   256-byte aligned: the rows that count and their logsumexp);
+ *   bwd reads that state and dloss (fp32, [N] or one value), and writes whichever of dx [N, D], dW [V, D], db [V]
  *   (dense, of the inputs' type) is not NULL.  Rows that do not count have a zero gradient, whatever x holds there.
- * The backward walks the vocabulary in pieces of `piece` columns (0: chosen so that a piece's gradients fit the last-level cache).
+ * The backward walks the vocabulary in pieces of `piece` columns (0: as many as half a GiB of scratch holds).
  * N, V, ldx, ldw <= 2^22, D <= 2^20, all >= 1.  ws: phc_linear_xent_ws_bytes(desc, backward) bytes, 256-byte aligned, scratch. */
 #define PHC_REDUCE_NONE 0
 #define PHC_REDUCE_SUM 1
@@ -1250,12 +1250,14 @@ typedef struct phc_linear_xent_desc {
     int32_t dtype, reduction;
     const void *x, *W, *bias;
     const int64_t *target;
-    float *loss, *lse, *stat;
+    float *loss;
+    void *state;
     const float *dloss;
     void *dx, *dW, *db;
     void *ws;
     size_t ws_bytes;
 } phc_linear_xent_desc;                     /* the struct is HOST memory, its pointers device memory */
+size_t phc_linear_xent_state_bytes(int64_t N);
 size_t phc_linear_xent_ws_bytes(const phc_linear_xent_desc *desc, int backward);
 int phc_linear_xent_fwd(const phc_linear_xent_desc *desc, void *stream);
 int phc_linear_xent_bwd(const phc_linear_xent_desc *desc, void *stream);

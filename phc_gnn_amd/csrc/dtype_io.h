@@ -36,6 +36,25 @@ __device__ __forceinline__ void store_pack(T *p, const float (&in)[W]) {
     *reinterpret_cast<Pack<T, W> *>(p) = q;
 }
 
+// ... at any element-aligned address (the hardware takes unaligned global accesses)
+template <typename T, int W>
+struct __attribute__((packed, aligned(sizeof(T)))) LoosePack {
+    T v[W];
+};
+template <typename T, int W>
+__device__ __forceinline__ void load_loose(const T *p, float (&out)[W]) {
+    const LoosePack<T, W> q = *reinterpret_cast<const LoosePack<T, W> *>(p);
+#pragma unroll
+    for (int i = 0; i < W; ++i) out[i] = to_f32(q.v[i]);
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_loose(T *p, const float (&in)[W]) {
+    LoosePack<T, W> q;
+#pragma unroll
+    for (int i = 0; i < W; ++i) q.v[i] = from_f32<T>(in[i]);
+    *reinterpret_cast<LoosePack<T, W> *>(p) = q;
+}
+
 inline int dtype_bytes(int dtype) { return dtype == PHC_DTYPE_F32 ? 4 : (dtype == PHC_DTYPE_BF16 || dtype == PHC_DTYPE_F16) ? 2 : 0; }
 inline bool aligned_to(const void *p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 

@@ -33,29 +33,41 @@ struct XRows {
 
 __global__ __launch_bounds__(1024) void xent_rows_that_count_kernel(const long long *__restrict__ target, long long ignore, int N, long long V,
                                                                    int *err, XRows r) {
+    constexpr int PER = 8;                     // a wavefront takes 8 x 64 consecutive rows at a time
     __shared__ int wsum[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int carry = 0;
-    for (int base = 0; base < N; base += 1024) {
-        const int i = base + threadIdx.x;
-        const long long t = i < N ? target[i] : ignore;
-        const bool kept = t != ignore;
-        const unsigned long long m = __ballot(kept);
-        if (lane == 0) wsum[wave] = __popcll(m);
+    for (int base = 0; base < N; base += 1024 * PER) {
+        const int i0 = base + wave * 64 * PER + lane;
+        long long t[PER];
+        unsigned long long m[PER];
+        int mine = 0;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) t[q] = i0 + q * 64 < N ? target[i0 + q * 64] : ignore;
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            m[q] = __ballot(t[q] != ignore);
+            mine += __popcll(m[q]);
+        }
+        if (lane == 0) wsum[wave] = mine;
         __syncthreads();
-        int before = carry, total = 0;
+        int at = carry;
 #pragma unroll
         for (int w = 0; w < 16; ++w) {
-            if (w < wave) before += wsum[w];
-            total += wsum[w];
+            if (w < wave) at += wsum[w];
+            carry += wsum[w];
         }
-        const int at = before + __popcll(m & ((1ull << lane) - 1));
-        if (i < N) r.to[i] = kept ? at : -1;
-        if (kept) {
-            r.from[at] = i;
-            r.target[at] = (int)checked_index(t, V, err, PHC_IDX_ERR_TARGET);
+#pragma unroll
+        for (int q = 0; q < PER; ++q) {
+            const int i = i0 + q * 64, k = at + __popcll(m[q] & ((1ull << lane) - 1));
+            const bool kept = t[q] != ignore;
+            if (i < N) r.to[i] = kept ? k : -1;
+            if (kept) {
+                r.from[k] = i;
+                r.target[k] = (int)checked_index(t[q], V, err, PHC_IDX_ERR_TARGET);
+            }
+            at += __popcll(m[q]);
         }
-        carry += total;
         __syncthreads();
     }
     if (threadIdx.x == 0) *r.count = carry;
@@ -174,6 +186,14 @@ typedef __attribute__((address_space(3))) const char lds_char;
 typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 typedef __attribute__((address_space(3))) const s16x8_t lds_s16x8;
 
+// (maximum, sum of exponentials below it) of two parts of a row; a part of nothing but -inf has sum 0
+__device__ __forceinline__ void xt_join(float &mx, float &sum, float m, float s) {
+    const float top = fmaxf(mx, m);
+    const float shift = top == -INFINITY ? 0.f : top;
+    sum = sum * expf(mx - shift) + s * expf(m - shift);
+    mx = top;
+}
+
 enum XEpilogue { XE_STATS, XE_DLOGITS, XE_DX, XE_DW };
 
 struct XGemm {
@@ -187,6 +207,7 @@ struct XGemm {
     int tilesM, tilesN, max_blocks;
     int split_k;                   // k that the number of splits goes by
     const int *count;              // packed rows
+    int pick;                      // launched with both tile sizes: the one that fits the rows that count does the work
     // XE_STATS / XE_DLOGITS
     const void *bias;              // fp32 or the operand's type, of this piece; may be null
     const int *target;             // [packed rows]
@@ -206,8 +227,11 @@ struct XGemm {
     void *out;                     // element (n, m) at n * ldo + m
     int ldo;
     float *slabs;                  // fp32 partial outputs [split][rows][ldo]
-    int accumulate, pieces, out_vec;
+    int accumulate, pieces;
 };
+
+// 256 x 256 tiles need half the operand bytes of 128 x 128 ones per product, and fill the card only with enough of them.
+__host__ __device__ inline bool xt_big(int m, int n) { return m > 128 && n > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
 
 // Work of a product over `tiles` output tiles: the k loop is split where the tiles alone do not fill the card, never below 4 steps.
 __host__ __device__ inline int xt_splits(int tiles, int steps, int max_blocks) {
@@ -277,6 +301,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 
     // what there is to do goes by the rows that count
     const int count = *a.count;
+    if ((EPI == XE_STATS || EPI == XE_DLOGITS) && a.pick && xt_big(a.rowsA, count) != (TM == 256)) return;
     const int rowsB = EPI == XE_DW ? a.rowsB : count;
     const int tilesN = (rowsB + TN - 1) / TN, tiles = a.tilesM * tilesN;
     const int ksteps = EPI == XE_DW ? (count + XT_BK - 1) / XT_BK : (int)((a.K + XT_BK - 1) / XT_BK);
@@ -437,9 +462,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 #pragma unroll
                 for (int w = 1; w < WM; ++w) {
                     const float2 o = meet[w * TN + c];
-                    const float top = fmaxf(m, o.x), shift = top == -INFINITY ? 0.f : top;
-                    s = s * expf(m - shift) + o.y * expf(o.x - shift);
-                    m = top;
+                    xt_join(m, s, o.x, o.y);
                 }
                 a.part_max[(size_t)tm * a.N + n] = m;
                 a.part_sum[(size_t)tm * a.N + n] = s;
@@ -498,21 +521,21 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
                 for (int r = 0; r < 4; ++r) v[r] = acc[i][j][r] * s;
                 if (final) {
                     TO *o = static_cast<TO *>(a.out) + row * a.ldo + m;
-                    if (a.out_vec && m + 4 <= a.rowsA) store_pack<TO, 4>(o, v);
+                    if (m + 4 <= a.rowsA) store_loose<TO, 4>(o, v);
                     else
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
                             if (m + r < a.rowsA) o[r] = from_f32<TO>(v[r]);
                 } else {
                     float *o = a.slabs + ((size_t)split * rowsB + row) * a.ldo + m;
-                    if (a.ldo % 4 == 0 && m + 4 <= a.rowsA) {
+                    if (m + 4 <= a.rowsA) {
                         if (a.accumulate) {
                             float p[4];
-                            load_pack<float, 4>(o, p);
+                            load_loose<float, 4>(o, p);
 #pragma unroll
                             for (int r = 0; r < 4; ++r) v[r] += p[r];
                         }
-                        store_pack<float, 4>(o, v);
+                        store_loose<float, 4>(o, v);
                     } else {
 #pragma unroll
                         for (int r = 0; r < 4; ++r)
@@ -524,9 +547,183 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     }
 }
 
+// ---- a few rows -------------------------------------------------------------------------------------------------------------------------
+// Up to 64 rows (scoring a few tokens): W is read once and everything else is small, so the launch is W's bytes at the memory's rate and
+// latency.  A workgroup takes 64 columns; its four wavefronts share the k (their loads are all in flight at once) and meet in LDS.  W and x go
+// from memory straight into matrix operands: lane (rho, g) loads 16 bytes of row rho at k = g * 16 bytes, the same for both operands, so any
+// order of k inside a step will do.  fp32 on the fp32 matrix instructions (4 k each): their rate is enough beside W's bytes.
+struct XFew {
+    const void *W, *x, *bias;
+    long long ldw, ldx;            // elements
+    int N, V, D;
+    const long long *target;
+    long long ignore;
+    int *err;
+    float *part_max, *part_sum;    // [64-column group][16 NF]
+    float *target_logit;           // [row]
+};
+
+template <typename T>
+struct XFewStep {                  // 16-bit: 8 k of each of 4 lane groups
+    static constexpr int PER = 8, K = 32;
+    typedef typename Mfma16<T>::frag frag;
+    static __device__ __forceinline__ f32x4_t mul(frag a, frag b, f32x4_t c) { return Mfma16<T>::mul(a, b, c); }
+};
+template <>
+struct XFewStep<float> {
+    static constexpr int PER = 4, K = 16;
+    typedef f32x4_t frag;
+    static __device__ __forceinline__ f32x4_t mul(frag a, frag b, f32x4_t c) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], b[q], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// 16 bytes at an element-aligned address, zeros behind the row's end
+template <typename T, typename frag>
+__device__ __forceinline__ frag few_load(const T *p, int left) {
+    constexpr int PER = 16 / sizeof(T);
+    LoosePack<T, PER> q = {};
+    if (left >= PER) q = *reinterpret_cast<const LoosePack<T, PER> *>(p);
+    else if (left > 0)
+#pragma unroll
+        for (int e = 0; e < PER; ++e)
+            if (e < left) q.v[e] = p[e];
+    return __builtin_bit_cast(frag, q);
+}
+
+template <typename T, int NF>
+__global__ __launch_bounds__(256) void xent_few_kernel(XFew a) {
+    typedef XFewStep<T> S;
+    typedef typename S::frag frag;
+    constexpr int UNROLL = NF > 2 ? 2 : 4;
+    __shared__ f32x4_t meet[4][4][NF][64];
+    __shared__ float2 top[4][NF * 16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
+    const int v0 = blockIdx.x * 64;
+    const T *w[4], *x[NF];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = static_cast<const T *>(a.W) + (long long)min(v0 + i * 16 + fr, a.V - 1) * a.ldw + fg * S::PER;
+#pragma unroll
+    for (int j = 0; j < NF; ++j) x[j] = static_cast<const T *>(a.x) + (long long)min(j * 16 + fr, a.N - 1) * a.ldx + fg * S::PER;
+    f32x4_t acc[4][NF];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = wave * S::K; k0 < a.D; k0 += 4 * UNROLL * S::K) {
+        frag fw[UNROLL][4], fx[UNROLL][NF];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = k0 + u * 4 * S::K;
+            const int left = a.D - k - fg * S::PER;              // elements of the rows from this lane's on
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fw[u][i] = few_load<T, frag>(w[i] + k, left);
+#pragma unroll
+            for (int j = 0; j < NF; ++j) fx[u][j] = few_load<T, frag>(x[j] + k, left);
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < NF; ++j) acc[i][j] = S::mul(fw[u][i], fx[u][j], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) meet[wave][i][j][lane] = acc[i][j];
+    __syncthreads();
+    // wavefront w: columns v0 + 16 w ..; a lane holds columns 4 fg .. 4 fg + 3 of row fr
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+        f32x4_t l = meet[0][wave][j][lane];
+#pragma unroll
+        for (int q = 1; q < 4; ++q) l += meet[q][wave][j][lane];
+        const int n = j * 16 + fr;
+        const long long t = n < a.N ? a.target[n] : a.ignore;
+        const int hit = t == a.ignore ? -1 : (int)checked_index(t, a.V, blockIdx.x == 0 ? a.err : nullptr, PHC_IDX_ERR_TARGET);
+        float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int v = v0 + wave * 16 + fg * 4 + r;
+            if (v >= a.V) {
+                l[r] = -INFINITY;
+                continue;
+            }
+            if (a.bias) l[r] += to_f32(static_cast<const T *>(a.bias)[v]);
+            mx = fmaxf(mx, l[r]);
+            if (hit == v) a.target_logit[n] = l[r];
+        }
+        mx = fmaxf(mx, __shfl_xor(mx, 16));
+        mx = fmaxf(mx, __shfl_xor(mx, 32));
+        const float shift = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sum += sizeof(T) == 4 ? expf(l[r] - shift) : __expf(l[r] - shift);
+        sum += __shfl_xor(sum, 16);
+        sum += __shfl_xor(sum, 32);
+        if (fg == 0) top[wave][n] = make_float2(mx, sum);
+    }
+    __syncthreads();
+    if (threadIdx.x < NF * 16) {
+        float m = top[0][threadIdx.x].x, s = top[0][threadIdx.x].y;
+#pragma unroll
+        for (int q = 1; q < 4; ++q) xt_join(m, s, top[q][threadIdx.x].x, top[q][threadIdx.x].y);
+        a.part_max[(size_t)blockIdx.x * NF * 16 + threadIdx.x] = m;
+        a.part_sum[(size_t)blockIdx.x * NF * 16 + threadIdx.x] = s;
+    }
+}
+
+// joins the column groups' parts; losses, their reduction and the state for the backward: one workgroup, rows in the lanes of a wavefront
+__global__ __launch_bounds__(1024) void xent_few_finish_kernel(XFew a, int parts, int cols, int reduction, XRows rows, float *__restrict__ lse,
+                                                              float *__restrict__ loss) {
+    __shared__ float sm[1024], ss[1024];
+    const int c = threadIdx.x % cols, group = threadIdx.x / cols, groups = 1024 / cols;
+    float mx = -INFINITY, sum = 0.f;
+    for (int p = group; p < parts; p += groups) xt_join(mx, sum, a.part_max[(size_t)p * cols + c], a.part_sum[(size_t)p * cols + c]);
+    sm[threadIdx.x] = mx;
+    ss[threadIdx.x] = sum;
+    for (int half = groups / 2; half >= 1; half /= 2) {              // (groups is a power of two)
+        __syncthreads();
+        if (group < half) {
+            xt_join(mx, sum, sm[threadIdx.x + half * cols], ss[threadIdx.x + half * cols]);
+            sm[threadIdx.x] = mx;
+            ss[threadIdx.x] = sum;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x >= 64) return;
+    const int n = threadIdx.x;
+    const long long t = n < a.N ? a.target[n] : a.ignore;
+    const bool kept = t != a.ignore;
+    const unsigned long long m = __ballot(kept);
+    float l = 0.f;
+    if (kept) {
+        const float e = sm[n] + logf(ss[n]);
+        l = e - a.target_logit[n];
+        const int at = __popcll(m & ((1ull << n) - 1));
+        rows.from[at] = n;
+        rows.to[n] = at;
+        rows.target[at] = (int)safe_index(t, a.V);
+        lse[at] = e;
+    } else if (n < a.N) {
+        rows.to[n] = -1;
+    }
+    if (n == 0) *rows.count = __popcll(m);
+    if (reduction == PHC_REDUCE_NONE) {
+        if (n < a.N) loss[n] = l;
+        return;
+    }
+    double s = (double)l;
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
+    if (n == 0) loss[0] = (float)(reduction == PHC_REDUCE_MEAN ? s / (double)__popcll(m) : s);
+}
+
 // ---- rows -------------------------------------------------------------------------------------------------------------------------------
 // A workgroup joins the parts of 16 rows: 64 lane groups share the parts, then one adds them up.
-__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int parts, int N,
+__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int V, int N,
                                                         const int *__restrict__ count, const float *__restrict__ target_logit,
                                                         const int *__restrict__ from, float *__restrict__ lse, float *__restrict__ row_loss,
                                                         float *__restrict__ loss) {
@@ -534,20 +731,15 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int n = blockIdx.x * 16 + c, kept = *count;
     if (blockIdx.x * 16 >= kept) return;
+    const int parts = xt_big(V, kept) ? (V + 255) / 256 : (V + 127) / 128;
     float mx = -INFINITY, sum = 0.f;
-    auto join = [&](float m, float s) {
-        const float top = fmaxf(mx, m);
-        const float shift = top == -INFINITY ? 0.f : top;
-        sum = sum * expf(mx - shift) + s * expf(m - shift);
-        mx = top;
-    };
     if (n < kept)
-        for (int p = group; p < parts; p += 64) join(part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
+        for (int p = group; p < parts; p += 64) xt_join(mx, sum, part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
     sm[group][c] = mx;
     ss[group][c] = sum;
     __syncthreads();
     if (group == 0 && n < kept) {
-        for (int w = 1; w < 64; ++w) join(sm[w][c], ss[w][c]);
+        for (int w = 1; w < 64; ++w) xt_join(mx, sum, sm[w][c], ss[w][c]);
         const float l = mx + logf(sum);
         lse[n] = l;
         row_loss[n] = l - target_logit[n];
@@ -555,25 +747,25 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
     }
 }
 
-// sum of the rows' losses -> out[0] = sum or mean, stat = {sum, rows that count}; per row (out is null): zeros for the ignored rows
+// sum of the rows' losses -> out[0] = sum or mean; per row (out is null): zeros for the ignored rows
 __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float *__restrict__ row_loss, const int *__restrict__ count, const int *__restrict__ to,
-                                                          int N, int mean, float *__restrict__ out, float *__restrict__ loss, float *__restrict__ stat) {
+                                                          int N, int mean, float *__restrict__ out, float *__restrict__ loss) {
     __shared__ double red[16];
+    if (loss) {
+        for (int i = threadIdx.x; i < N; i += 1024)
+            if (to[i] < 0) loss[i] = 0.f;
+        return;
+    }
     const int kept = *count;
     double s = 0.0;
     for (int i = threadIdx.x; i < kept; i += 1024) s += (double)row_loss[i];
-    if (loss)
-        for (int i = threadIdx.x; i < N; i += 1024)
-            if (to[i] < 0) loss[i] = 0.f;
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; ++w) s += red[w];
-        if (out) out[0] = (float)(mean ? s / (double)kept : s);          // (no row counts: the mean of nothing is NaN)
-        stat[0] = (float)s;
-        stat[1] = (float)kept;
+        out[0] = (float)(mean ? s / (double)kept : s);          // (no row counts: the mean of nothing is NaN)
     }
 }
 
@@ -615,23 +807,31 @@ __global__ __launch_bounds__(256) void xent_sum_slabs_kernel(const float *__rest
     }
 }
 
-// db[v] = top sum over the tiles along n of their partial sums
+// db[v] = top sum over the row tiles' partial sums, in order: 16 columns a workgroup, 16 lane groups share the parts
 template <typename T>
-__global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ part, const int *__restrict__ count, int TN, int WN, int nv,
+__global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ part, const int *__restrict__ count, int nv,
                                                      const float *__restrict__ top, T *__restrict__ db) {
-    const int v = blockIdx.x * 256 + threadIdx.x;
-    if (v >= nv) return;
-    const int n = (*count + TN - 1) / TN * WN;
+    __shared__ float meet[16][16];
+    const int c = threadIdx.x & 15, group = threadIdx.x >> 4, v = blockIdx.x * 16 + c;
+    const int n = xt_big(nv, *count) ? (*count + 255) / 256 * 4 : (*count + 127) / 128 * 2;
     float s = 0.f;
-    for (int i = 0; i < n; ++i) s += part[(size_t)i * nv + v];
-    db[v] = from_f32<T>(s * *top);
+    if (v < nv)
+        for (int i = group; i < n; i += 16) s += part[(size_t)i * nv + v];
+    meet[group][c] = s;
+    __syncthreads();
+    if (group == 0 && v < nv) {
+        for (int w = 1; w < 16; ++w) s += meet[w][c];
+        db[v] = from_f32<T>(s * *top);
+    }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------------------
 static long long round_up(long long v, long long m) { return (v + m - 1) / m * m; }
 static long long ceil_div(long long v, long long m) { return (v + m - 1) / m; }
 
-constexpr long long XT_PIECE_BYTES = 128ll << 20;      // a piece's d: half of the Infinity Cache, W and x beside it
+// A piece's d.  Pieces are for memory alone: at N = 8192, V = 131072, D = 2048 (bf16) pieces of 8192, 16384, 32768 and all columns took 14.4,
+// 14.3, 14.3 and 14.3 ms, smaller ones cost (4096: 15.8 ms).
+constexpr long long XT_PIECE_BYTES = 512ll << 20;
 
 // Tiles of 256 x 256 by 8 wavefronts (one workgroup on a CU) or 128 x 128 by 4 (two)
 struct Tile256 {
@@ -646,15 +846,13 @@ struct XPlan {
     int planes, segments;
     long long Kp, Np, piece, pieces;
     bool pack_w;
-    bool big_fwd, big_d, big_dx, big_dw;       // 256 x 256 tiles
+    bool big_fwd, big_d;       // 256 x 256 tiles, if enough rows count (known on the device alone)
+    bool big_dx, big_dw;       // 256 x 256 tiles
     long long wcols;           // readable columns of W's operand rows
 };
 
-static bool big_tiles(long long m, long long n, bool splits) {
-    // the large tile needs fewer operand bytes per product, and fills the card only with enough of them
-    const long long t = ceil_div(m, 256) * ceil_div(n, 256);
-    return m > 128 && n > 128 && (splits ? t >= 32 : t >= 192);
-}
+// dx and dW split their k loop: few large tiles do
+static bool big_split(long long m, long long n) { return m > 128 && n > 128 && ceil_div(m, 256) * ceil_div(n, 256) >= 32; }
 
 static XPlan make_plan(const phc_linear_xent_desc *d) {
     XPlan p;
@@ -673,10 +871,10 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     p.pieces = ceil_div(d->V, piece);
     p.piece = d->piece > 0 ? piece : round_up(ceil_div(d->V, p.pieces), 64);
     p.pieces = ceil_div(d->V, p.piece);
-    p.big_fwd = big_tiles(d->V, d->N, false);
-    p.big_d = big_tiles(p.piece, d->N, false);
-    p.big_dx = big_tiles(d->D, d->N, true);
-    p.big_dw = big_tiles(d->D, p.piece, true);
+    p.big_fwd = xt_big((int)d->V, (int)d->N);
+    p.big_d = xt_big((int)p.piece, (int)d->N);
+    p.big_dx = big_split(d->D, d->N);
+    p.big_dw = big_split(d->D, p.piece);
     return p;
 }
 
@@ -688,8 +886,23 @@ static size_t slab_floats(long long rows, long long D, bool big, bool keeps) {
     return keeps ? (all > most ? all : most) : most;
 }
 
-struct XWs {
+// what the forward hands to the backward
+struct XState {
     XRows rows{};
+    float *lse = nullptr;
+    size_t bytes;
+    XState(long long N, void *state) {
+        Carve c(state);
+        rows.count = c.take<int>(1);
+        rows.from = c.take<int>(N);
+        rows.to = c.take<int>(N);
+        rows.target = c.take<int>(N);
+        lse = c.take<float>(N);
+        bytes = c.used;
+    }
+};
+
+struct XWs {
     XPlanes x{}, w{}, dl{};
     float *part_max = nullptr, *part_sum = nullptr, *target_logit = nullptr, *row_loss = nullptr;
     float *rel = nullptr, *top = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr, *db_part = nullptr;
@@ -699,14 +912,10 @@ struct XWs {
         auto planes = [&](XPlanes &o, size_t count) {
             for (int i = 0; i < p.planes; ++i) o.p[i] = c.take<unsigned short>(count);
         };
-        rows.count = c.take<int>(1);
-        rows.from = c.take<int>(d->N);
-        rows.to = c.take<int>(d->N);
-        rows.target = c.take<int>(d->N);
         planes(x, (size_t)p.Np * p.Kp);
         if (p.pack_w) planes(w, (size_t)(backward ? p.piece : d->V) * p.Kp);
         if (!backward) {
-            const size_t parts = ceil_div(d->V, p.big_fwd ? 256 : 128);
+            const size_t parts = ceil_div(d->V, 128);
             part_max = c.take<float>(parts * d->N);
             part_sum = c.take<float>(parts * d->N);
             target_logit = c.take<float>(d->N);
@@ -717,7 +926,7 @@ struct XWs {
             planes(dl, (size_t)p.Np * p.piece);
             if (d->dx) dx_slabs = c.take<float>(slab_floats(d->N, d->D, p.big_dx, p.pieces > 1));
             if (d->dW) dw_slabs = c.take<float>(slab_floats(p.piece, d->D, p.big_dw, false));
-            if (d->db) db_part = c.take<float>((size_t)(p.big_d ? ceil_div(d->N, 256) * Tile256::WN : ceil_div(d->N, 128) * Tile128::WN) * p.piece);
+            if (d->db) db_part = c.take<float>((size_t)(ceil_div(d->N, 256) * Tile256::WN) * p.piece);          // (4 parts of each 256 rows, either size)
         }
         bytes = c.used;
     }
@@ -767,6 +976,12 @@ static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
 template <int EPI>
 static int gemm(const phc_linear_xent_desc *d, int kid, bool big, XGemm &g, hipStream_t s) {
     bool ok;
+    if ((EPI == XE_STATS || EPI == XE_DLOGITS) && big && !g.pick) {
+        // Enough rows for large tiles, if they count, which the device alone knows: both sizes are launched, one of them ends at once
+        // (4 us; 13 568 rows of which 15 % count against 5000 columns would fill 160 of the 256 CUs with large tiles).
+        g.pick = 1;
+        if (int rc = gemm<EPI>(d, kid, false, g, s)) return rc;
+    }
     if (d->dtype == PHC_DTYPE_F32) ok = big ? launch_gemm<bf16_t, EPI, true, Tile256>(kid, g, s) : launch_gemm<bf16_t, EPI, true, Tile128>(kid, g, s);
     else if (d->dtype == PHC_DTYPE_BF16) ok = big ? launch_gemm<bf16_t, EPI, false, Tile256>(kid, g, s) : launch_gemm<bf16_t, EPI, false, Tile128>(kid, g, s);
     else ok = big ? launch_gemm<f16_t, EPI, false, Tile256>(kid, g, s) : launch_gemm<f16_t, EPI, false, Tile128>(kid, g, s);
@@ -786,9 +1001,34 @@ static void sum_slabs(int dtype, int kid, const float *slabs, const XGemm &g, in
 }
 
 template <typename T>
-static void db_as(const float *part, const XRows &r, int TN, int WN, int nv, const float *top, void *db, hipStream_t s) {
-    PHC_LAUNCH_AS(K_XENT_DW, (xent_db_kernel<T>), dim3((unsigned)ceil_div(nv, 256)), dim3(256), 0, s, part, (const int *)r.count, TN, WN, nv, top,
+static void db_as(const float *part, const XRows &r, int nv, const float *top, void *db, hipStream_t s) {
+    PHC_LAUNCH_AS(K_XENT_DW, (xent_db_kernel<T>), dim3((unsigned)ceil_div(nv, 16)), dim3(256), 0, s, part, (const int *)r.count, nv, top,
                   static_cast<T *>(db));
+}
+
+constexpr int XT_FEW = 64;
+static bool few_rows(const phc_linear_xent_desc *d) { return d->N <= XT_FEW; }
+
+template <typename T>
+static void launch_few(const XFew &f, hipStream_t s) {
+    const dim3 grid((unsigned)ceil_div(f.V, 64));
+    if (f.N <= 16) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 1>), grid, dim3(256), 0, s, f);
+    else if (f.N <= 32) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 2>), grid, dim3(256), 0, s, f);
+    else PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 4>), grid, dim3(256), 0, s, f);
+}
+
+static int forward_few(const phc_linear_xent_desc *d, const XState &st, hipStream_t s) {
+    const int cols = d->N <= 16 ? 16 : d->N <= 32 ? 32 : 64, parts = (int)ceil_div(d->V, 64);
+    Carve c(d->ws);
+    XFew f{d->W, d->x, d->bias, d->ldw, d->ldx, (int)d->N, (int)d->V, (int)d->D, reinterpret_cast<const long long *>(d->target), d->ignore_index, err_word()};
+    f.part_max = c.take<float>((size_t)parts * cols);
+    f.part_sum = c.take<float>((size_t)parts * cols);
+    f.target_logit = c.take<float>(cols);
+    if (d->dtype == PHC_DTYPE_F32) launch_few<float>(f, s);
+    else if (d->dtype == PHC_DTYPE_BF16) launch_few<bf16_t>(f, s);
+    else launch_few<f16_t>(f, s);
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_few_finish_kernel, dim3(1), dim3(1024), 0, s, f, parts, cols, d->reduction, st.rows, st.lse, d->loss);
+    return launch_status("phc_linear_xent_fwd");
 }
 
 static int xent_check(const char *who, const phc_linear_xent_desc *d) {
@@ -800,7 +1040,7 @@ static int xent_check(const char *who, const phc_linear_xent_desc *d) {
                 "%s: N=%lld, V=%lld, D=%lld or a row stride is beyond 2^22, 2^22, 2^20, 2^22", who, (long long)d->N, (long long)d->V, (long long)d->D);
     PHC_REQUIRE(d->ldx >= d->D && d->ldw >= d->D, PHC_ERR_INVALID_ARG, "%s: row stride below the row length", who);
     PHC_REQUIRE(d->piece >= 0, PHC_ERR_INVALID_ARG, "%s: piece %lld", who, (long long)d->piece);
-    PHC_REQUIRE(d->x && d->W && d->target && d->lse && d->stat, PHC_ERR_INVALID_ARG, "%s: null pointer", who);
+    PHC_REQUIRE(d->x && d->W && d->target && d->state && aligned_to(d->state, 256), PHC_ERR_INVALID_ARG, "%s: null pointer, or a state that is not 256-byte aligned", who);
     return PHC_OK;
 }
 
@@ -810,8 +1050,11 @@ using namespace phc;
 
 extern "C" {
 
+size_t phc_linear_xent_state_bytes(int64_t N) { return N < 0 || N > (1 << 22) ? 0 : XState(N, nullptr).bytes; }
+
 size_t phc_linear_xent_ws_bytes(const phc_linear_xent_desc *d, int backward) {
     if (xent_check("phc_linear_xent_ws_bytes", d)) return 0;
+    if (!backward && few_rows(d)) return (size_t)ceil_div(d->V, 64) * 64 * 2 * sizeof(float) + 2048;
     return XWs(d, make_plan(d), backward != 0, nullptr).bytes + 256;
 }
 
@@ -821,12 +1064,14 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     PHC_REQUIRE(d->ws && aligned_to(d->ws, 256) && d->ws_bytes >= phc_linear_xent_ws_bytes(d, 0), PHC_ERR_WORKSPACE,
                 "phc_linear_xent_fwd: workspace of %zu bytes, %zu needed", (size_t)d->ws_bytes, phc_linear_xent_ws_bytes(d, 0));
     hipStream_t s = static_cast<hipStream_t>(stream);
+    const XState st(d->N, d->state);
+    if (few_rows(d)) return forward_few(d, st, s);
     const XPlan p = make_plan(d);
     XWs w(d, p, false, d->ws);
     const int es = dtype_bytes(d->dtype), N = (int)d->N;
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_that_count_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const long long *>(d->target),
-                  (long long)d->ignore_index, N, (long long)d->V, err_word(), w.rows);
-    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &w.rows, nullptr, w.x, s);
+                  (long long)d->ignore_index, N, (long long)d->V, err_word(), st.rows);
+    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &st.rows, nullptr, w.x, s);
     XPlanes W{{const_cast<void *>(d->W)}};
     if (p.pack_w) {
         pack(d->dtype, d->W, d->ldw, d->V, d->D, p.Kp, nullptr, nullptr, w.w, s);
@@ -839,18 +1084,18 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     g.ldb = (unsigned)(p.Kp * 2);
     g.rowsA = (int)d->V;
     g.rowsB = g.N = N;
-    g.count = w.rows.count;
+    g.count = st.rows.count;
     g.bias = d->bias;
-    g.target = w.rows.target;
+    g.target = st.rows.target;
     g.part_max = w.part_max;
     g.part_sum = w.part_sum;
     g.target_logit = w.target_logit;
     if (int rc = gemm<XE_STATS>(d, K_XENT_LOGITS, p.big_fwd, g, s)) return rc;
     float *loss = d->reduction == PHC_REDUCE_NONE ? d->loss : nullptr;
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_kernel, dim3((unsigned)ceil_div(N, 16)), dim3(1024), 0, s, (const float *)w.part_max, (const float *)w.part_sum,
-                  g.tilesM, N, g.count, (const float *)w.target_logit, (const int *)w.rows.from, d->lse, w.row_loss, loss);
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_reduce_kernel, dim3(1), dim3(1024), 0, s, (const float *)w.row_loss, g.count, (const int *)w.rows.to, N,
-                  d->reduction == PHC_REDUCE_MEAN ? 1 : 0, loss ? (float *)nullptr : d->loss, loss, d->stat);
+                  (int)d->V, N, g.count, (const float *)w.target_logit, (const int *)st.rows.from, st.lse, w.row_loss, loss);
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_reduce_kernel, dim3(1), dim3(1024), 0, s, (const float *)w.row_loss, g.count, (const int *)st.rows.to, N,
+                  d->reduction == PHC_REDUCE_MEAN ? 1 : 0, loss ? (float *)nullptr : d->loss, loss);
     return launch_status("phc_linear_xent_fwd");
 }
 
@@ -863,12 +1108,11 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
     hipStream_t s = static_cast<hipStream_t>(stream);
     const XPlan p = make_plan(d);
     XWs w(d, p, true, d->ws);
+    const XState st(d->N, d->state);
     const int es = dtype_bytes(d->dtype), N = (int)d->N;
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_that_count_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const long long *>(d->target),
-                  (long long)d->ignore_index, N, (long long)d->V, (int *)nullptr, w.rows);
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_scales_kernel, dim3(1), dim3(1024), 0, s, d->dloss, d->reduction == PHC_REDUCE_NONE ? 1 : 0,
-                  d->reduction == PHC_REDUCE_MEAN ? 1 : 0, (const int *)w.rows.count, (const int *)w.rows.from, w.rel, w.top);
-    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &w.rows, d->dx, w.x, s);
+                  d->reduction == PHC_REDUCE_MEAN ? 1 : 0, (const int *)st.rows.count, (const int *)st.rows.from, w.rel, w.top);
+    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &st.rows, d->dx, w.x, s);
     // fp16 has no normal values below 6e-5, where most probabilities of a large vocabulary lie: its d are stored times 2^14
     const float d_scale = d->dtype == PHC_DTYPE_F16 ? 16384.f : 1.f;
     XGemm o{};                                                   // (the last piece's dx product: its splits are joined at the end)
@@ -888,11 +1132,11 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         g.ldb = (unsigned)(p.Kp * 2);
         g.rowsA = nv;
         g.rowsB = g.N = N;
-        g.count = w.rows.count;
+        g.count = st.rows.count;
         g.bias = d->bias ? static_cast<const char *>(d->bias) + (size_t)v0 * es : nullptr;
-        g.target = w.rows.target;
+        g.target = st.rows.target;
         g.first_v = (int)v0;
-        g.lse = d->lse;
+        g.lse = st.lse;
         g.rel = w.rel;
         g.d = w.dl;
         g.ldd = nvp;
@@ -900,11 +1144,10 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         g.db_part = d->db ? w.db_part : nullptr;
         if (int rc = gemm<XE_DLOGITS>(d, K_XENT_DLOGITS, p.big_d, g, s)) return rc;
         if (d->db) {
-            const int TN = p.big_d ? 256 : 128, WN = p.big_d ? Tile256::WN : Tile128::WN;
             char *db = static_cast<char *>(d->db) + (size_t)v0 * es;
-            if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, w.rows, TN, WN, nv, w.top, db, s);
-            else if (d->dtype == PHC_DTYPE_BF16) db_as<bf16_t>(w.db_part, w.rows, TN, WN, nv, w.top, db, s);
-            else db_as<f16_t>(w.db_part, w.rows, TN, WN, nv, w.top, db, s);
+            if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, st.rows, nv, w.top, db, s);
+            else if (d->dtype == PHC_DTYPE_BF16) db_as<bf16_t>(w.db_part, st.rows, nv, w.top, db, s);
+            else db_as<f16_t>(w.db_part, st.rows, nv, w.top, db, s);
         }
         if (d->dx) {
             o = XGemm{};
@@ -916,16 +1159,15 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             o.rowsA = (int)d->D;
             o.colsA = (int)p.wcols;
             o.rowsB = N;
-            o.count = w.rows.count;
+            o.count = st.rows.count;
             o.scale = w.top;
             o.out_scale = 1.f / d_scale;
-            o.row_of = w.rows.from;
+            o.row_of = st.rows.from;
             o.out = d->dx;
             o.ldo = (int)d->D;
             o.slabs = w.dx_slabs;
             o.accumulate = v0 > 0;
             o.pieces = (int)p.pieces;
-            o.out_vec = d->D % 4 == 0 && aligned_to(d->dx, 4 * es);
             if (int rc = gemm<XE_DX>(d, K_XENT_DX, p.big_dx, o, s)) return rc;
         }
         if (d->dW) {
@@ -936,14 +1178,13 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             q.rowsA = (int)d->D;
             q.colsA = (int)p.Kp;
             q.rowsB = nv;
-            q.count = w.rows.count;
+            q.count = st.rows.count;
             q.scale = w.top;
             q.out_scale = 1.f / d_scale;
             q.out = static_cast<char *>(d->dW) + (size_t)v0 * d->D * es;
             q.ldo = (int)d->D;
             q.slabs = w.dw_slabs;
             q.pieces = 1;
-            q.out_vec = d->D % 4 == 0 && aligned_to(d->dW, 4 * es);
             if (int rc = gemm<XE_DW>(d, K_XENT_DW, p.big_dw, q, s)) return rc;
             if ((long long)q.tilesM * q.tilesN * 2 <= q.max_blocks)
                 sum_slabs(d->dtype, K_XENT_DW, w.dw_slabs, q, p.big_dw ? 256 : 128, 1, q.out, s);

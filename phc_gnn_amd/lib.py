@@ -46,7 +46,7 @@ class LinearXentDesc(C.Structure):
     """phc_linear_xent_desc (include/phc_hip.h)."""
     _fields_ = [("N", _L), ("V", _L), ("D", _L), ("ldx", _L), ("ldw", _L), ("ignore_index", _L), ("piece", _L),
                 ("dtype", C.c_int32), ("reduction", C.c_int32), ("x", _P), ("W", _P), ("bias", _P), ("target", _P),
-                ("loss", _P), ("lse", _P), ("stat", _P), ("dloss", _P), ("dx", _P), ("dW", _P), ("db", _P), ("ws", _P), ("ws_bytes", _S)]
+                ("loss", _P), ("state", _P), ("dloss", _P), ("dx", _P), ("dW", _P), ("db", _P), ("ws", _P), ("ws_bytes", _S)]
 
 
 class DownstreamNorm(C.Structure):
@@ -320,6 +320,7 @@ SIGNATURES = {
     "phc_embedding_fwd": (_I, [_P, _P, _L, _L, _L, _L, _I, C.c_float, _P, _P]),
     "phc_embedding_bwd_ws_bytes": (_S, [_L, _L, _L]),
     "phc_embedding_bwd": (_I, [_P, _P, _L, _L, _L, _L, _I, C.c_float, _L, _P, _P, _S, _P]),
+    "phc_linear_xent_state_bytes": (_S, [_L]),
     "phc_linear_xent_ws_bytes": (_S, [C.POINTER(LinearXentDesc), _I]),
     "phc_linear_xent_fwd": (_I, [C.POINTER(LinearXentDesc), _P]),
     "phc_linear_xent_bwd": (_I, [C.POINTER(LinearXentDesc), _P]),

@@ -126,7 +126,7 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
 
 
 # ---- softmax cross entropy of a linear map ----------------------------------------------------------------------------------------
-def _xent_desc(x, w, bias, target, ignore_index, reduction, stat, lse, piece):
+def _xent_desc(x, w, bias, target, ignore_index, reduction, state, piece):
     d = L.LinearXentDesc()
     d.N, d.D = x.shape
     d.V = w.shape[0]
@@ -134,7 +134,7 @@ def _xent_desc(x, w, bias, target, ignore_index, reduction, stat, lse, piece):
     d.ignore_index, d.piece = ignore_index, piece
     d.dtype, d.reduction = L.DTYPE_IDS[x.dtype], reduction
     d.x, d.W, d.bias, d.target = L.ptr(x), L.ptr(w), L.ptr(bias), L.ptr(target)
-    d.lse, d.stat = L.ptr(lse), L.ptr(stat)
+    d.state = L.ptr(state)
     return d
 
 
@@ -162,16 +162,15 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         x_, w_ = _rows(x), _rows(weight)
         b_ = None if bias is None else bias.contiguous()
         loss = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-        lse = torch.empty(N, dtype=torch.float32, device=dev)
-        stat = torch.empty(2, dtype=torch.float32, device=dev)
-        d = _xent_desc(x_, w_, b_, target, ignore_index, reduction, stat, lse, piece)
+        state = torch.empty(lib.phc_linear_xent_state_bytes(N), dtype=torch.uint8, device=dev)
+        d = _xent_desc(x_, w_, b_, target, ignore_index, reduction, state, piece)
         d.loss = L.ptr(loss)
         ws = _xent_workspace(lib, d, 0, dev)
         with on_device(dev):
             L.check(lib.phc_linear_xent_fwd(C.byref(d), L.stream_ptr(dev)), "phc_linear_xent_fwd")
         del ws
         L.maybe_check_indices(dev)
-        ctx.save_for_backward(x_, w_, b_, target, lse, stat)
+        ctx.save_for_backward(x_, w_, b_, target, state)
         return loss
 
     @staticmethod
@@ -184,13 +183,13 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
             x, w, b = ctx.saved_tensors
             return (torch.zeros_like(x) if need_x else None, torch.zeros_like(w) if need_w else None,
                     torch.zeros_like(b) if need_b else None, None, None, None, None)
-        x, w, b, target, lse, stat = ctx.saved_tensors
+        x, w, b, target, state = ctx.saved_tensors
         dev = x.device
         g = dloss.to(torch.float32).contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
         dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
         db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need_b else None
-        d = _xent_desc(x, w, b, target, ignore_index, reduction, stat, lse, piece)
+        d = _xent_desc(x, w, b, target, ignore_index, reduction, state, piece)
         d.dloss, d.dx, d.dW, d.db = L.ptr(g), L.ptr(dx), L.ptr(dw), L.ptr(db)
         ws = _xent_workspace(lib, d, 1, dev)
         with on_device(dev):
@@ -208,8 +207,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     gradient and stay out of the mean; the mean of no rows is NaN, as for an empty selection.  A bias of -inf takes a column out of the
     vocabulary.  A target outside [0, V) counts as 0 and is reported by ``phc_gnn_amd.check_indices()``.
 
-    The backward computes the logits again, ``piece`` columns of the vocabulary at a time (0: as many as keep a piece's gradients in the
-    last-level cache; its workspace grows with ``piece``).  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
+    The backward computes the logits again, ``piece`` columns of the vocabulary at a time (0: as many as half a GiB of scratch holds; it
+    grows with ``piece``).  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
     dev = L.require_device(x, weight, target, bias)
     _dtype_id("linear_cross_entropy: x", x)
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[0] < 1 or weight.shape[1] < 1 or x.shape[-1] != weight.shape[1]:

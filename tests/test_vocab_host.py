@@ -68,7 +68,7 @@ def _desc(lib, **kw):
     d = lib.LinearXentDesc()
     ok = 1 << 20
     for k, v in dict(dict(N=10, V=300, D=64, ldx=64, ldw=64, ignore_index=-100, piece=0, dtype=1, reduction=2, x=ok, W=ok, target=ok, loss=ok,
-                          lse=ok, stat=ok, ws=ok, ws_bytes=1 << 40), **kw).items():
+                          state=ok, ws=ok, ws_bytes=1 << 40), **kw).items():
         setattr(d, k, v)
     return d
 
@@ -77,7 +77,7 @@ def test_linear_xent_entry_points_check_their_arguments():
     lib, h = _lib()
     for kw, code in ((dict(dtype=3), -1), (dict(reduction=3), -1), (dict(N=0), -1), (dict(V=0), -1), (dict(D=0), -1), (dict(ldx=63), -1),
                      (dict(ldw=63), -1), (dict(N=1 << 23), -2), (dict(V=1 << 23), -2), (dict(ldw=1 << 23), -2), (dict(piece=-1), -1),
-                     (dict(x=None), -1), (dict(W=None), -1), (dict(target=None), -1), (dict(lse=None), -1), (dict(stat=None), -1),
+                     (dict(x=None), -1), (dict(W=None), -1), (dict(target=None), -1), (dict(state=None), -1), (dict(state=(1 << 20) + 8), -1),
                      (dict(loss=None), -1), (dict(ws=None), -3), (dict(ws=(1 << 20) + 16), -3), (dict(ws_bytes=8), -3)):
         assert h.phc_linear_xent_fwd(C.byref(_desc(lib, **kw)), None) == code, kw
     assert h.phc_linear_xent_fwd(None, None) == -1
