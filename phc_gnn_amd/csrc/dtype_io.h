@@ -36,6 +36,15 @@ __device__ __forceinline__ void store_pack(T *p, const float (&in)[W]) {
     *reinterpret_cast<Pack<T, W> *>(p) = q;
 }
 
+// (hipcc splits the store of a Pack of zeros into elements)
+template <typename T, int W>
+__device__ __forceinline__ void store_zeros(T *p) {
+    if constexpr (sizeof(T) * W == 16) *reinterpret_cast<uint4 *>(p) = make_uint4(0, 0, 0, 0);
+    else if constexpr (sizeof(T) * W == 8) *reinterpret_cast<uint2 *>(p) = make_uint2(0, 0);
+    else if constexpr (sizeof(T) * W == 4) *reinterpret_cast<unsigned *>(p) = 0;
+    else *reinterpret_cast<unsigned short *>(p) = 0;
+}
+
 // ... at any element-aligned address (the hardware takes unaligned global accesses)
 template <typename T, int W>
 struct __attribute__((packed, aligned(sizeof(T)))) LoosePack {

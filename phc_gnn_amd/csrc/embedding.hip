@@ -15,7 +15,7 @@ namespace phc {
 
 constexpr int EB_THREADS = 256;
 constexpr int EB_CHUNK = 32;              // sorted positions per chunk
-constexpr int EB_RADIX_BITS = 8;
+constexpr int EB_RADIX_BITS = 9;           // (two passes up to 262144 rows)
 constexpr int EB_BINS = 1 << EB_RADIX_BITS;
 constexpr int EB_SORT_ITEMS = 8;          // keys per thread and sort tile
 constexpr int EB_SORT_TILE = EB_THREADS * EB_SORT_ITEMS;
@@ -41,44 +41,55 @@ __global__ __launch_bounds__(EB_THREADS) void embedding_fwd_kernel(const long lo
 }
 
 // ---- stable radix sort of (token, position) -------------------------------------------------------------------------------------------
-// One pass: tile histograms, one scan over [digit][tile], stable scatter.  Inside a tile a wavefront ranks its 64 keys by comparing
-// digits with ballots (peers = lanes with the same digit); the wavefronts' counts are then added in order.
-__global__ __launch_bounds__(EB_THREADS) void embedding_keys_kernel(const long long *__restrict__ tokens, long long N, long long V,
-                                                                    int *__restrict__ keys, int *__restrict__ pos) {
-    for (long long i = (long long)blockIdx.x * EB_THREADS + threadIdx.x; i < N; i += (long long)gridDim.x * EB_THREADS) {
-        keys[i] = (int)safe_index(tokens[i], V);
-        pos[i] = (int)i;
+// Digits of at most 9 bits, as many passes as the vocabulary's bits need.  A wavefront ranks its 64 keys by comparing digits with ballots
+// (peers = lanes with the same digit); the counts of its earlier keys stand in LDS.  Up to EB_LDS_SORT positions one workgroup sorts in
+// LDS, in one launch; beyond that every pass is tile histograms, one scan over [digit][tile] and a stable scatter.
+
+// rank of this lane's key among the wavefront's keys of the same digit; `count` (this wavefront's, per digit) is moved on
+__device__ __forceinline__ int eb_rank(int digit, bool in, int bits, int *count) {
+    unsigned long long peers = __ballot(in);
+    for (int b = 0; b < bits; ++b) {
+        const unsigned long long m = __ballot((digit >> b) & 1);
+        peers &= ((digit >> b) & 1) ? m : ~m;
     }
+    const int below = __popcll(peers & ((1ull << (threadIdx.x & 63)) - 1));
+    const int before = in ? count[digit] : 0;
+    __builtin_amdgcn_wave_barrier();
+    if (in && below == 0) count[digit] = before + __popcll(peers);
+    __builtin_amdgcn_wave_barrier();
+    return before + below;
 }
 
-__global__ __launch_bounds__(EB_THREADS) void embedding_hist_kernel(const int *__restrict__ keys, int N, int shift, int tiles,
-                                                                   int *__restrict__ hist) {
-    __shared__ int bins[EB_BINS];
-    bins[threadIdx.x] = 0;
-    __syncthreads();
-    const int base = blockIdx.x * EB_SORT_TILE;
-    for (int j = 0; j < EB_SORT_ITEMS; ++j) {
-        const int i = base + j * EB_THREADS + threadIdx.x;
-        if (i < N) atomicAdd(&bins[(keys[i] >> shift) & (EB_BINS - 1)], 1);
-    }
-    __syncthreads();
-    hist[threadIdx.x * tiles + blockIdx.x] = bins[threadIdx.x];
-}
-
-// exclusive scan of n counts, in place, by one workgroup
-__global__ __launch_bounds__(1024) void embedding_scan_kernel(int *__restrict__ a, int n) {
-    __shared__ int wsum[16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int carry = 0;
-    for (int base = 0; base < n; base += 1024 * 4) {
-        const int i0 = base + threadIdx.x * 4;
-        int v[4], s = 0;
+// One workgroup, everything in LDS: a thread holds PER keys of its wavefront's consecutive 64 PER.
+template <int PER>
+__global__ __launch_bounds__(1024) void embedding_sort_lds_kernel(const long long *__restrict__ tokens, int N, long long V, int bits, int passes,
+                                                                 int *__restrict__ keys_out, int *__restrict__ pos_out) {
+    constexpr int WAVES = 16, CAP = 1024 * PER;
+    extern __shared__ int smem[];
+    int *lkeys = smem;                                            // [CAP]
+    int(*count)[EB_BINS] = reinterpret_cast<int(*)[EB_BINS]>(smem + CAP);      // [WAVES]
+    int *wsum = smem + CAP + WAVES * EB_BINS;                     // [WAVES]
+    unsigned short *lpos = reinterpret_cast<unsigned short *>(wsum + WAVES);   // [CAP]
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, base = wave * 64 * PER + lane;
+    int key[PER], pos[PER];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = i0 + j < n ? a[i0 + j] : 0;
-            s += v[j];
-        }
-        int inc = s;
+    for (int j = 0; j < PER; ++j) {
+        const int i = base + j * 64;
+        key[j] = i < N ? (int)safe_index(tokens[i], V) : 0;
+        pos[j] = i;
+    }
+    const int width = (bits + passes - 1) / passes, mask = (1 << width) - 1;
+    for (int p = 0; p < passes; ++p) {
+        for (int b = lane; b < EB_BINS; b += 64) count[wave][b] = 0;
+        int rank[PER];
+#pragma unroll
+        for (int j = 0; j < PER; ++j) rank[j] = eb_rank((key[j] >> (p * width)) & mask, base + j * 64 < N, width, count[wave]);
+        __syncthreads();
+        // exclusive starts: digits in order, the wavefronts of a digit in order (a thread has one digit: EB_BINS <= 1024)
+        int total = 0;
+        if (threadIdx.x < EB_BINS)
+            for (int w = 0; w < WAVES; ++w) total += count[w][threadIdx.x];
+        int inc = total;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(inc, d);
@@ -86,71 +97,147 @@ __global__ __launch_bounds__(1024) void embedding_scan_kernel(int *__restrict__ 
         }
         if (lane == 63) wsum[wave] = inc;
         __syncthreads();
-        int before = carry, total = 0;
-#pragma unroll
-        for (int w = 0; w < 16; ++w) {
-            if (w < wave) before += wsum[w];
-            total += wsum[w];
+        if (threadIdx.x < EB_BINS) {
+            int run = inc - total;
+            for (int w = 0; w < wave; ++w) run += wsum[w];
+            for (int w = 0; w < WAVES; ++w) {
+                const int c = count[w][threadIdx.x];
+                count[w][threadIdx.x] = run;
+                run += c;
+            }
         }
-        int run = before + inc - s;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (i0 + j < n) a[i0 + j] = run;
-            run += v[j];
-        }
-        carry += total;
         __syncthreads();
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (base + j * 64 >= N) continue;
+            const int o = count[wave][(key[j] >> (p * width)) & mask] + rank[j];
+            lkeys[o] = key[j];
+            lpos[o] = (unsigned short)pos[j];
+        }
+        __syncthreads();
+        if (p == passes - 1) break;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int i = base + j * 64;
+            if (i < N) {
+                key[j] = lkeys[i];
+                pos[j] = lpos[i];
+            }
+        }
+        __syncthreads();
+    }
+    for (int i = threadIdx.x; i < N; i += 1024) {
+        keys_out[i] = lkeys[i];
+        pos_out[i] = lpos[i];
     }
 }
 
-__global__ __launch_bounds__(EB_THREADS) void embedding_scatter_kernel(const int *__restrict__ keys, const int *__restrict__ pos, int N,
-                                                                      int shift, int tiles, const int *__restrict__ offs,
-                                                                      int *__restrict__ keys_out, int *__restrict__ pos_out) {
-    constexpr int WAVES = EB_THREADS / 64;
-    __shared__ int wcount[WAVES][EB_BINS];       // keys of a digit met by each wavefront: then the wavefront's start in the output
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int b = lane; b < EB_BINS; b += 64) wcount[wave][b] = 0;
+// The first pass reads the tokens themselves (keys == nullptr); positions are then the indices.
+__device__ __forceinline__ int eb_key(const int *keys, const long long *tokens, long long V, int i) {
+    return keys ? keys[i] : (int)safe_index(tokens[i], V);
+}
+
+__global__ __launch_bounds__(EB_THREADS) void embedding_hist_kernel(const int *__restrict__ keys, const long long *__restrict__ tokens, long long V,
+                                                                   int N, int shift, int mask, int *__restrict__ hist) {
+    __shared__ int bins[EB_BINS];
+    for (int b = threadIdx.x; b < EB_BINS; b += EB_THREADS) bins[b] = 0;
     __syncthreads();
-    const int base = blockIdx.x * EB_SORT_TILE + wave * (64 * EB_SORT_ITEMS);      // a wavefront owns consecutive keys
-    int digit[EB_SORT_ITEMS], rank[EB_SORT_ITEMS];
+    const int base = blockIdx.x * EB_SORT_TILE;
 #pragma unroll
     for (int j = 0; j < EB_SORT_ITEMS; ++j) {
-        const int i = base + j * 64 + lane;
-        const bool in = i < N;
-        digit[j] = in ? (keys[i] >> shift) & (EB_BINS - 1) : -1;
-        unsigned long long peers = __ballot(in);
-#pragma unroll
-        for (int b = 0; b < EB_RADIX_BITS; ++b) {
-            const unsigned long long m = __ballot((digit[j] >> b) & 1);
-            peers &= ((digit[j] >> b) & 1) ? m : ~m;
-        }
-        const int below = __popcll(peers & ((1ull << lane) - 1));
-        const int before = in ? wcount[wave][digit[j]] : 0;
-        rank[j] = before + below;
-        __builtin_amdgcn_wave_barrier();
-        if (in && below == 0) wcount[wave][digit[j]] = before + __popcll(peers);
-        __builtin_amdgcn_wave_barrier();
+        const int i = base + j * EB_THREADS + threadIdx.x;
+        if (i < N) atomicAdd(&bins[(eb_key(keys, tokens, V, i) >> shift) & mask], 1);
     }
     __syncthreads();
-    {
-        const int b = threadIdx.x;
-        int run = offs[b * tiles + blockIdx.x];
+    for (int b = threadIdx.x; b < EB_BINS; b += EB_THREADS) hist[(size_t)blockIdx.x * EB_BINS + b] = bins[b];
+}
+
+// hist [tile][digit] -> the first place of every (tile, digit) in the output: digits in order, the tiles of a digit in order.  One workgroup;
+// 1024 / EB_BINS thread groups share the tiles.
+__global__ __launch_bounds__(1024) void embedding_scan_kernel(int *__restrict__ hist, int tiles) {
+    constexpr int GROUPS = 1024 / EB_BINS, AHEAD = 16;
+    __shared__ int sums[GROUPS][EB_BINS], wsum[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = threadIdx.x % EB_BINS, g = threadIdx.x / EB_BINS;
+    const int each = (tiles + GROUPS - 1) / GROUPS, t0 = min(g * each, tiles), t1 = min(t0 + each, tiles);
+    int mine = 0;
+    for (int t = t0; t < t1; t += AHEAD) {
+        int v[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) v[q] = t + q < t1 ? hist[(size_t)(t + q) * EB_BINS + b] : 0;
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) mine += v[q];
+    }
+    sums[g][b] = mine;
+    __syncthreads();
+    int total = 0;
+    if (g == 0)
+        for (int k = 0; k < GROUPS; ++k) total += sums[k][b];
+    int inc = total;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(inc, d);
+        if (lane >= d) inc += o;
+    }
+    if (lane == 63) wsum[wave] = inc;
+    __syncthreads();
+    if (g == 0) {
+        int run = inc - total;
+        for (int w = 0; w < wave; ++w) run += wsum[w];
+        for (int k = 0; k < GROUPS; ++k) {
+            const int c = sums[k][b];
+            sums[k][b] = run;
+            run += c;
+        }
+    }
+    __syncthreads();
+    int run = sums[g][b];
+    for (int t = t0; t < t1; t += AHEAD) {
+        int v[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) v[q] = t + q < t1 ? hist[(size_t)(t + q) * EB_BINS + b] : 0;
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            if (t + q < t1) hist[(size_t)(t + q) * EB_BINS + b] = run;
+            run += v[q];
+        }
+    }
+}
+
+__global__ __launch_bounds__(EB_THREADS) void embedding_scatter_kernel(const int *__restrict__ keys, const long long *__restrict__ tokens, long long V,
+                                                                      const int *__restrict__ pos, int N, int shift, int width,
+                                                                      const int *__restrict__ offs, int *__restrict__ keys_out,
+                                                                      int *__restrict__ pos_out) {
+    constexpr int WAVES = EB_THREADS / 64;
+    __shared__ int count[WAVES][EB_BINS];        // keys of a digit met by each wavefront: then the wavefront's start in the output
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, mask = (1 << width) - 1;
+    for (int b = lane; b < EB_BINS; b += 64) count[wave][b] = 0;
+    const int base = blockIdx.x * EB_SORT_TILE + wave * (64 * EB_SORT_ITEMS) + lane;      // a wavefront owns consecutive keys
+    int key[EB_SORT_ITEMS], at[EB_SORT_ITEMS], rank[EB_SORT_ITEMS];
+#pragma unroll
+    for (int j = 0; j < EB_SORT_ITEMS; ++j) {
+        const int i = base + j * 64;
+        key[j] = i < N ? eb_key(keys, tokens, V, i) : 0;
+        at[j] = i < N && keys ? pos[i] : i;
+    }
+#pragma unroll
+    for (int j = 0; j < EB_SORT_ITEMS; ++j) rank[j] = eb_rank((key[j] >> shift) & mask, base + j * 64 < N, width, count[wave]);
+    __syncthreads();
+    for (int b = threadIdx.x; b < EB_BINS; b += EB_THREADS) {
+        int run = offs[(size_t)blockIdx.x * EB_BINS + b];
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) {
-            const int c = wcount[w][b];
-            wcount[w][b] = run;
+            const int c = count[w][b];
+            count[w][b] = run;
             run += c;
         }
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < EB_SORT_ITEMS; ++j) {
-        const int i = base + j * 64 + lane;
-        if (i < N) {
-            const int o = wcount[wave][digit[j]] + rank[j];
-            keys_out[o] = keys[i];
-            pos_out[o] = pos[i];
-        }
+        if (base + j * 64 >= N) continue;
+        const int o = count[wave][(key[j] >> shift) & mask] + rank[j];
+        keys_out[o] = key[j];
+        pos_out[o] = at[j];
     }
 }
 
@@ -179,76 +266,124 @@ __global__ __launch_bounds__(EB_THREADS) void embedding_bwd_kernel(const int *__
             if (threadIdx.x == 0) n_empty = __popcll(m);
         }
         __syncthreads();
-        float z[W] = {};
         for (int e = threadIdx.x >> 6; e < n_empty; e += EB_THREADS / 64) {
             T *dst = dW + (size_t)empty_rows[e] * D;
-            for (int c = (threadIdx.x & 63) * W; c < D; c += 64 * W) store_pack<T, W>(dst + c, z);
+            for (int c = (threadIdx.x & 63) * W; c < D; c += 64 * W) store_zeros<T, W>(dst + c);
         }
         return;
     }
-    const int slab_cols = W << lg;
+    // the chunk's keys and positions, one in front and one behind: by the group's lanes, for all of them
+    extern __shared__ int staged[];                                // [groups of the workgroup][EB_CHUNK + 2 keys | EB_CHUNK positions]
+    const int slab_cols = W << lg, lanes = 1 << lg, me = threadIdx.x & (lanes - 1);
+    int *skeys = staged + (threadIdx.x >> lg) * (2 * EB_CHUNK + 2), *spos = skeys + EB_CHUNK + 2;
     const int slabs = (D + slab_cols - 1) / slab_cols;
     const long long group = ((long long)blockIdx.x * EB_THREADS + threadIdx.x) >> lg;
     const int chunk = (int)(group / slabs);
-    const int col = (int)(group % slabs) * slab_cols + (threadIdx.x & ((1 << lg) - 1)) * W;
+    const int col = (int)(group % slabs) * slab_cols + me * W;
     const long long first = (long long)chunk * EB_CHUNK;
-    if (first >= N || col >= D) return;
-    const int begin = (int)first, end = min(begin + EB_CHUNK, N);
+    const int begin = (int)min(first, (long long)N), n = min(EB_CHUNK, N - begin);
+    for (int i = me; i < EB_CHUNK + 2; i += lanes) {
+        const int at = begin + i - 1;
+        skeys[i] = at >= 0 && at < N ? keys[at] : -1;
+        if (i < EB_CHUNK) spos[i] = begin + i < N ? pos[begin + i] : 0;
+    }
+    __syncthreads();
+    if (n <= 0 || col >= D) return;
     float acc[W] = {};
-    int key = keys[begin];
-    bool from_before = begin > 0 && keys[begin - 1] == key;        // the run started in an earlier chunk
-    for (int i = begin; i < end; ++i) {
-        float v[W];
-        load_pack<T, W>(dy + (long long)pos[i] * ldy + col, v);
+    int key = skeys[1];
+    bool from_before = skeys[0] == key;                         // the run started in an earlier chunk
+    constexpr int AHEAD = 8;                                       // rows in flight
+    for (int i0 = 0; i0 < n; i0 += AHEAD) {
+        Pack<T, W> row[AHEAD];
 #pragma unroll
-        for (int q = 0; q < W; ++q) acc[q] += v[q];
-        const int next = i + 1 < N ? keys[i + 1] : -1;
-        if (next == key && i + 1 < end) continue;
-        if (from_before || next == key) {
-            // part of a crossing run: slot 0 = a run that came from before, slot 1 = one that starts here and goes on
-            float *p = partial + ((size_t)chunk * 2 + (from_before ? 0 : 1)) * D + col;
+        for (int q = 0; q < AHEAD; ++q)                            // (behind the chunk's end: its last row again, not used)
+            row[q] = *reinterpret_cast<const Pack<T, W> *>(dy + (long long)spos[min(i0 + q, n - 1)] * ldy + col);
 #pragma unroll
-            for (int q = 0; q < W; ++q) p[q] = acc[q];
-        } else if (key != pad) {
+        for (int q = 0; q < AHEAD; ++q) {
+            if (i0 + q >= n) break;
 #pragma unroll
-            for (int q = 0; q < W; ++q) acc[q] *= scale;
-            store_pack<T, W>(dW + (size_t)key * D + col, acc);
+            for (int c = 0; c < W; ++c) acc[c] += to_f32(row[q].v[c]);
+            const int next = skeys[i0 + q + 2];
+            if (next == key && i0 + q + 1 < n) continue;
+            if (from_before || next == key) {
+                // part of a crossing run: slot 0 = a run that came from before, slot 1 = one that starts here and goes on
+                store_pack<float, W>(partial + ((size_t)chunk * 2 + (from_before ? 0 : 1)) * D + col, acc);
+            } else if (key != pad) {
+#pragma unroll
+                for (int c = 0; c < W; ++c) acc[c] *= scale;
+                store_pack<T, W>(dW + (size_t)key * D + col, acc);
+            }
+#pragma unroll
+            for (int c = 0; c < W; ++c) acc[c] = 0.f;
+            from_before = false;
+            key = next;
         }
-#pragma unroll
-        for (int q = 0; q < W; ++q) acc[q] = 0.f;
-        from_before = false;
-        key = next;
     }
 }
 
-// the crossing run that starts in a chunk: its parts in order
+// The crossing runs that start in EB_JOIN neighbouring chunks: their parts in order.  A workgroup takes those chunks and a column slab; its
+// lane groups share a run's parts (group g the g-th stretch of them) and their sums are added in order.
+constexpr int EB_JOIN = 4;
 template <typename T, int W>
 __global__ __launch_bounds__(EB_THREADS) void embedding_join_kernel(const int *__restrict__ keys, int N, int D, float scale, int pad, int lg,
-                                                                   int chunks, const float *__restrict__ partial, T *__restrict__ dW) {
-    const int slab_cols = W << lg;
-    const int slabs = (D + slab_cols - 1) / slab_cols;
-    const long long group = ((long long)blockIdx.x * EB_THREADS + threadIdx.x) >> lg;
-    const int chunk = (int)(group / slabs);
-    const int col = (int)(group % slabs) * slab_cols + (threadIdx.x & ((1 << lg) - 1)) * W;
-    if (chunk + 1 >= chunks || col >= D) return;                     // (the last chunk's runs end in it)
-    const int last = (chunk + 1) * EB_CHUNK - 1;
-    const int key = keys[last];
-    if (keys[last + 1] != key || key == pad) return;                 // no run crosses this chunk's end
-    const int begin = chunk * EB_CHUNK;
-    if (keys[begin] == key && begin > 0 && keys[begin - 1] == key) return;      // ... or it started in an earlier chunk
-    float acc[W];
-#pragma unroll
-    for (int q = 0; q < W; ++q) acc[q] = partial[((size_t)chunk * 2 + 1) * D + col + q];
-    for (int c = chunk + 1; c < chunks && keys[c * EB_CHUNK] == key; ++c) {
-#pragma unroll
-        for (int q = 0; q < W; ++q) acc[q] += partial[(size_t)c * 2 * D + col + q];
+                                                                   int chunks, int slabs, const float *__restrict__ partial, T *__restrict__ dW) {
+    __shared__ float meet[EB_THREADS * W];
+    const int first = (int)(blockIdx.x / slabs) * EB_JOIN, count = min(EB_JOIN, chunks - 1 - first);     // (the last chunk's runs end in it)
+    const int lanes = 1 << lg, me = threadIdx.x & (lanes - 1), g = threadIdx.x >> lg, groups = EB_THREADS >> lg;
+    const int col = (int)(blockIdx.x % slabs) * (W << lg) + me * W;
+    // which of the chunks start a crossing run (the same answer in every wavefront)
+    bool starts = false;
+    if ((int)(threadIdx.x & 63) < count) {
+        const int begin = (first + (threadIdx.x & 63)) * EB_CHUNK, key = keys[begin + EB_CHUNK - 1];
+        starts = keys[begin + EB_CHUNK] == key && key != pad && !(keys[begin] == key && begin > 0 && keys[begin - 1] == key);
     }
+    unsigned long long todo = __ballot(starts);
+    for (; todo; todo &= todo - 1) {
+        const int chunk = first + __builtin_ctzll(todo), last = (chunk + 1) * EB_CHUNK - 1, key = keys[last];
+        int lo = last + 1, hi = N;                                   // the run's end
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (keys[mid] <= key) lo = mid + 1; else hi = mid;
+        }
+        const int parts = (lo - 1) / EB_CHUNK - chunk;               // in the chunks behind this one
+        const int each = (parts + groups - 1) / groups, p0 = min(g * each, parts), p1 = min(p0 + each, parts);
+        float acc[W] = {};
+        if (col < D) {
+            const float *src = partial + (size_t)(chunk + 1) * 2 * D + col;
+            constexpr int AHEAD = 8;
+            for (int p = p0; p < p1; p += AHEAD) {
+                float v[AHEAD][W];
 #pragma unroll
-    for (int q = 0; q < W; ++q) acc[q] *= scale;
-    store_pack<T, W>(dW + (size_t)key * D + col, acc);
+                for (int q = 0; q < AHEAD; ++q) load_pack<float, W>(src + (size_t)min(p + q, p1 - 1) * 2 * D, v[q]);
+#pragma unroll
+                for (int q = 0; q < AHEAD; ++q)
+                    if (p + q < p1)
+#pragma unroll
+                        for (int c = 0; c < W; ++c) acc[c] += v[q][c];
+            }
+        }
+        __syncthreads();                                             // (the run before has been read)
+#pragma unroll
+        for (int c = 0; c < W; ++c) meet[c * EB_THREADS + threadIdx.x] = acc[c];
+        __syncthreads();
+        if (g == 0 && col < D) {
+            float sum[W];
+            load_pack<float, W>(partial + ((size_t)chunk * 2 + 1) * D + col, sum);
+            for (int k = 0; k < min(groups, parts); ++k)
+#pragma unroll
+                for (int c = 0; c < W; ++c) sum[c] += meet[c * EB_THREADS + k * lanes + me];
+#pragma unroll
+            for (int c = 0; c < W; ++c) sum[c] *= scale;
+            store_pack<T, W>(dW + (size_t)key * D + col, sum);
+        }
+    }
 }
 
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
+constexpr int EB_LDS_SORT = 16384;
+template <int PER>
+constexpr size_t eb_lds_sort_bytes() { return (size_t)1024 * PER * 6 + 16 * EB_BINS * 4 + 16 * 4; }
+
 struct EmbeddingWs {
     int *keys[2], *pos[2], *hist;
     float *partial;
@@ -257,14 +392,44 @@ struct EmbeddingWs {
         Carve c(ws);
         const long long tiles = (N + EB_SORT_TILE - 1) / EB_SORT_TILE, chunks = (N + EB_CHUNK - 1) / EB_CHUNK;
         for (int i = 0; i < 2; ++i) {
-            keys[i] = c.take<int>(N);
-            pos[i] = c.take<int>(N);
+            const bool used = i == 0 || N > EB_LDS_SORT;
+            keys[i] = c.take<int>(used ? N : 0);
+            pos[i] = c.take<int>(used ? N : 0);
         }
-        hist = c.take<int>(tiles * EB_BINS);
+        hist = c.take<int>(N > EB_LDS_SORT ? tiles * EB_BINS : 0);
         partial = c.take<float>((size_t)chunks * 2 * D);
         bytes = c.used;
     }
 };
+
+template <int PER>
+static bool sort_lds(const int64_t *tokens, int N, int64_t V, int bits, int passes, const EmbeddingWs &w, hipStream_t s) {
+    if (!ensure_dynamic_lds(embedding_sort_lds_kernel<PER>, eb_lds_sort_bytes<PER>())) return false;
+    PHC_LAUNCH_AS(K_EMBEDDING_SORT, (embedding_sort_lds_kernel<PER>), dim3(1), dim3(1024), eb_lds_sort_bytes<PER>(), s,
+                  reinterpret_cast<const long long *>(tokens), N, (long long)V, bits, passes, w.keys[0], w.pos[0]);
+    return true;
+}
+
+// sorted (token, position) in keys[side], pos[side]; -1: a launch was refused
+static int sort_tokens(const int64_t *tokens, int N, int64_t V, const EmbeddingWs &w, hipStream_t s) {
+    int bits = 1;
+    while ((1ll << bits) < V) ++bits;
+    const int passes = (bits + EB_RADIX_BITS - 1) / EB_RADIX_BITS, width = (bits + passes - 1) / passes;
+    if (N <= 2048) return sort_lds<2>(tokens, N, V, bits, passes, w, s) ? 0 : -1;
+    if (N <= 6144) return sort_lds<6>(tokens, N, V, bits, passes, w, s) ? 0 : -1;
+    if (N <= EB_LDS_SORT) return sort_lds<16>(tokens, N, V, bits, passes, w, s) ? 0 : -1;
+    const int tiles = (N + EB_SORT_TILE - 1) / EB_SORT_TILE, mask = (1 << width) - 1;
+    const long long *t = reinterpret_cast<const long long *>(tokens);
+    int side = 1;
+    for (int p = 0; p < passes; ++p, side ^= 1) {
+        const int *keys = p ? w.keys[side] : nullptr, *pos = p ? w.pos[side] : nullptr;
+        PHC_LAUNCH_AS(K_EMBEDDING_SORT, embedding_hist_kernel, dim3(tiles), dim3(EB_THREADS), 0, s, keys, t, (long long)V, N, p * width, mask, w.hist);
+        PHC_LAUNCH_AS(K_EMBEDDING_SORT, embedding_scan_kernel, dim3(1), dim3(1024), 0, s, w.hist, tiles);
+        PHC_LAUNCH_AS(K_EMBEDDING_SORT, embedding_scatter_kernel, dim3(tiles), dim3(EB_THREADS), 0, s, keys, t, (long long)V, pos, N, p * width, width,
+                      (const int *)w.hist, w.keys[side ^ 1], w.pos[side ^ 1]);
+    }
+    return side;
+}
 
 // lanes per row: the smallest power of two that covers a row in one go, at most a wavefront
 static int lane_group(int D, int W) {
@@ -292,15 +457,16 @@ static void launch_fwd(const int64_t *tokens, const void *weight, int64_t N, int
 template <typename T, int W>
 static void launch_bwd(const EmbeddingWs &w, int side, const void *dy, int64_t N, int64_t V, int64_t ldy, int D, float scale, int pad,
                        void *dW, hipStream_t s) {
-    const int lg = lane_group(D, W);
+    const int lg = lane_group(D, W) < 3 ? 3 : lane_group(D, W);          // (8 lanes at least: a group stages 66 words)
     const long long slabs = (D + (W << lg) - 1) / (W << lg), chunks = (N + EB_CHUNK - 1) / EB_CHUNK;
     const long long cb = (((chunks * slabs) << lg) + EB_THREADS - 1) / EB_THREADS, zb = (V + 63) / 64;
-    PHC_LAUNCH_AS(K_EMBEDDING_BWD, (embedding_bwd_kernel<T, W>), dim3((unsigned)(cb + zb)), dim3(EB_THREADS), 0, s, (const int *)w.keys[side],
+    PHC_LAUNCH_AS(K_EMBEDDING_BWD, (embedding_bwd_kernel<T, W>), dim3((unsigned)(cb + zb)), dim3(EB_THREADS),
+                  (EB_THREADS >> lg) * (2 * EB_CHUNK + 2) * sizeof(int), s, (const int *)w.keys[side],
                (const int *)w.pos[side], static_cast<const T *>(dy), (long long)ldy, (int)N, (int)V, D, scale, pad, lg, (int)cb,
                static_cast<T *>(dW), w.partial);
     if (chunks > 1)
-        PHC_LAUNCH_AS(K_EMBEDDING_BWD, (embedding_join_kernel<T, W>), dim3((unsigned)cb), dim3(EB_THREADS), 0, s, (const int *)w.keys[side], (int)N, D, scale, pad,
-                   lg, (int)chunks, (const float *)w.partial, static_cast<T *>(dW));
+        PHC_LAUNCH_AS(K_EMBEDDING_BWD, (embedding_join_kernel<T, W>), dim3((unsigned)((chunks + EB_JOIN - 2) / EB_JOIN * slabs)), dim3(EB_THREADS), 0, s, (const int *)w.keys[side],
+                      (int)N, D, scale, pad, lg, (int)chunks, (int)slabs, (const float *)w.partial, static_cast<T *>(dW));
 }
 
 }  // namespace phc
@@ -364,18 +530,8 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
     const int pad = padding_idx >= 0 && padding_idx < V ? (int)padding_idx : -1;
     int side = 0;
     if (N > 0) {
-        const int tiles = (int)((N + EB_SORT_TILE - 1) / EB_SORT_TILE);
-        const unsigned kb = (unsigned)((N + EB_THREADS - 1) / EB_THREADS);
-        PHC_LAUNCH_AS(K_EMBEDDING_SORT, embedding_keys_kernel, dim3(kb < 4096 ? kb : 4096), dim3(EB_THREADS), 0, s, reinterpret_cast<const long long *>(tokens),
-                   (long long)N, (long long)V, w.keys[0], w.pos[0]);
-        int bits = 0;
-        while ((1ll << bits) < V) ++bits;
-        for (int shift = 0; shift < bits; shift += EB_RADIX_BITS, side ^= 1) {
-            PHC_LAUNCH_AS(K_EMBEDDING_SORT, embedding_hist_kernel, dim3(tiles), dim3(EB_THREADS), 0, s, (const int *)w.keys[side], (int)N, shift, tiles, w.hist);
-            PHC_LAUNCH_AS(K_EMBEDDING_SORT, embedding_scan_kernel, dim3(1), dim3(1024), 0, s, w.hist, tiles * EB_BINS);
-            PHC_LAUNCH_AS(K_EMBEDDING_SORT, embedding_scatter_kernel, dim3(tiles), dim3(EB_THREADS), 0, s, (const int *)w.keys[side], (const int *)w.pos[side],
-                       (int)N, shift, tiles, (const int *)w.hist, w.keys[side ^ 1], w.pos[side ^ 1]);
-        }
+        side = sort_tokens(tokens, (int)N, V, w, s);
+        PHC_REQUIRE(side >= 0, PHC_ERR_LAUNCH, "phc_embedding_bwd: the runtime refused the sort's LDS size");
     }
     const int width = pack_width(dtype_bytes(dtype), D, ldy, dy ? dy : dW, dW);
     EB_DISPATCH(launch_bwd, dtype, width, w, side, dy, N, V, ldy, (int)D, scale, pad, dW, s);

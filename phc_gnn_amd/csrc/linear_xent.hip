@@ -149,15 +149,24 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ 
 // ---- the product ----------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void xt_wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
-// One LDS-DMA instruction: every lane's 16 bytes at base + voff land at LDS byte address lds + 16 lane.  In asm because hipcc orders its
-// builtin against every later LDS read with s_waitcnt vmcnt(0), which would drain the prefetch; the loop's own waits order it.  M0 is
-// the DMA's LDS base, saved and restored inside the statement.
-__device__ __forceinline__ void xt_dma16(unsigned lds, unsigned voff, const void *base) {
+// Eight LDS-DMA instructions: every lane's 16 bytes at base + voff[q] land at LDS byte address lds + 1024 q + 16 lane.  In asm because hipcc
+// orders its builtin against every later LDS read with s_waitcnt vmcnt(0), which would drain the prefetch; the loop's own waits order
+// them.  M0 is the DMA's LDS base, saved and restored inside the statement.
+__device__ __forceinline__ void xt_dma8(unsigned lds, const unsigned (&voff)[8], const void *base) {
     unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep)
-                 : "s"(lds), "v"(voff), "s"(base)
-                 : "memory");
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %10\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %10\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %10\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %10\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %6, %10\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %7, %10\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %8, %10\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %9, %10\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "v"(voff[4]), "v"(voff[5]), "v"(voff[6]), "v"(voff[7]), "s"(base)
+        : "memory", "scc");
 }
 
 // (the same in all lanes; hipcc must know it)
@@ -231,7 +240,9 @@ struct XGemm {
 };
 
 // 256 x 256 tiles need half the operand bytes of 128 x 128 ones per product, and fill the card only with enough of them.
-__host__ __device__ inline bool xt_big(int m, int n) { return m > 128 && n > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= 192; }
+__host__ __device__ inline bool xt_big(int m, int n) {
+    return m > 128 && n > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= 192;
+}
 
 // Work of a product over `tiles` output tiles: the k loop is split where the tiles alone do not fill the card, never below 4 steps.
 __host__ __device__ inline int xt_splits(int tiles, int steps, int max_blocks) {
@@ -293,7 +304,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     typedef XSide<TM, A_TR, PAIR> SA;
     typedef XSide<TN, B_TR, false> SB;
     constexpr int LOADS = (TM + TN) / 8 / NW;                   // LDS-DMA instructions per wavefront and step (1 KiB each)
-    static_assert((TM / 8) % LOADS == 0, "a wavefront loads one operand");
+    static_assert(FN <= FM, "a group of products for each n fragment's read");
+    static_assert(LOADS == 8 && (TM / 8) % LOADS == 0, "a wavefront loads 8 KiB of one operand");
     constexpr unsigned BUF = (TM + TN) * 128;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -341,20 +353,25 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     unsigned voff[LOADS];
 #pragma unroll
     for (int q = 0; q < LOADS; ++q) voff[q] = offset(q, tr ? 0 : (int)at0, tr ? XT_BK : rows);
-    const unsigned lds_wave = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem + wave * LOADS * 1024;
-    int seg = s0 / (ksteps > 0 ? ksteps : 1), kst = s0 - seg * ksteps;          // the step that is loaded next
+    const unsigned lds_wave = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem + wave * LOADS * 1024);
+    // the step that is loaded next
+    const unsigned k_bytes = tr ? XT_BK * ld : XT_BK * 2;
+    int seg = __builtin_amdgcn_readfirstlane(s0 / (ksteps > 0 ? ksteps : 1)), kst = __builtin_amdgcn_readfirstlane(s0 - seg * ksteps);
+    auto plane = [&]() { return uniform((loads_a ? a.A[seg] : a.B[seg]) + (tr ? 0 : (size_t)at0 * ld) + (size_t)kst * k_bytes); };
+    const char *base = plane();
     auto issue = [&](int buf) {
-        const char *base = uniform((loads_a ? a.A[seg] : a.B[seg]) + (tr ? (size_t)kst * XT_BK * ld : (size_t)at0 * ld + (size_t)kst * (XT_BK * 2)));
         if (A_TR && EPI != XE_DW && tr && (kst + 1) * XT_BK > rows) {           // the last rows of k
+            unsigned last[LOADS];
 #pragma unroll
-            for (int q = 0; q < LOADS; ++q) xt_dma16(lds_wave + buf * BUF + q * 1024, offset(q, kst * XT_BK, rows), base);
+            for (int q = 0; q < LOADS; ++q) last[q] = offset(q, kst * XT_BK, rows);
+            xt_dma8(lds_wave + buf * BUF, last, base);
         } else {
-#pragma unroll
-            for (int q = 0; q < LOADS; ++q) xt_dma16(lds_wave + buf * BUF + q * 1024, voff[q], base);
+            xt_dma8(lds_wave + buf * BUF, voff, base);
         }
+        base += k_bytes;
         if (++kst == ksteps) {
             kst = 0;
-            ++seg;
+            if (++seg < a.segments) base = plane();
         }
     };
 
@@ -364,10 +381,22 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
 
+    const int ma = wm * FM * 16, nb = wn * FN * 16;
+    auto half = [&](lds_char *tile, int kk, const frag (&a0)[FM], const frag (&b0)[FN], frag (&a1)[FM], frag (&b1)[FN], bool load, int buf = 0) {
+        if (load) issue(buf);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+            if (i < FN) b1[i] = SB::template read<frag>(tile + TM * 128, nb, i, kk, lane);
+            a1[i] = SA::template read<frag>(tile, ma, i, kk, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = Mfma16<T>::mul(a0[i], b0[j], acc[i][j]);
+            __builtin_amdgcn_sched_barrier(0);          // (hipcc would gather the reads behind the products)
+        }
+    };
+
     // Two LDS buffers, two halves of a step.  While the products of one half run, the fragments of the next are read; the one barrier of a
     // step stands between them: behind it the next step's buffer is complete, and this step's buffer, read to its end, is loaded anew.
     lds_char *lds = (lds_char *)smem;
-    const int ma = wm * FM * 16, nb = wn * FN * 16;
     if (n_steps > 0) {
         frag fa[2][FM], fb[2][FN];
         issue(0);
@@ -380,27 +409,13 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
         for (int i = 0; i < FM; ++i) fa[0][i] = SA::template read<frag>(lds, ma, i, 0, lane);
         for (int t = 0; t < n_steps; ++t) {
             lds_char *cur = lds + (t & 1) * BUF, *nxt = lds + ((t & 1) ^ 1) * BUF;
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[1][j] = SB::template read<frag>(cur + TM * 128, nb, j, 1, lane);
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                fa[1][i] = SA::template read<frag>(cur, ma, i, 1, lane);
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Mfma16<T>::mul(fa[0][i], fb[0][j], acc[i][j]);
-            }
+            half(cur, 1, fa[0], fb[0], fa[1], fb[1], false);
             __builtin_amdgcn_sched_barrier(0);
             xt_wait_all();
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
-            if (t + 2 < n_steps) issue(t & 1);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[0][j] = SB::template read<frag>(nxt + TM * 128, nb, j, 0, lane);      // (behind the last step: read, not used)
-#pragma unroll
-            for (int i = 0; i < FM; ++i) {
-                fa[0][i] = SA::template read<frag>(nxt, ma, i, 0, lane);
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = Mfma16<T>::mul(fa[1][i], fb[1][j], acc[i][j]);
-            }
+            // (behind the last step the fragments are read once more and not used)
+            half(nxt, 0, fa[1], fb[1], fa[0], fb[0], t + 2 < n_steps, t & 1);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -852,7 +867,9 @@ struct XPlan {
 };
 
 // dx and dW split their k loop: few large tiles do
-static bool big_split(long long m, long long n) { return m > 128 && n > 128 && ceil_div(m, 256) * ceil_div(n, 256) >= 32; }
+static bool big_split(long long m, long long n) {
+    return m > 128 && n > 128 && ceil_div(m, 256) * ceil_div(n, 256) >= 32;
+}
 
 static XPlan make_plan(const phc_linear_xent_desc *d) {
     XPlan p;

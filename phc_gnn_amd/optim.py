@@ -9,12 +9,13 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from array import array
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import lib as L
-from .vocab import on_device
+from .vocab import on_device, raw_stream
 
 
 # clip + Adam as ONE launch whose workgroups exchange the sums of squares inside it (csrc/optim.hip, round 6); 0 = the two launches
@@ -183,6 +184,23 @@ def _dense(t: torch.Tensor) -> bool:
     return t.is_contiguous() or torch._prims_common.is_non_overlapping_and_dense(t)
 
 
+def _one_device(who: str, tensors: Sequence[torch.Tensor]) -> torch.device:
+    dev = L.require_device(tensors[0])
+    index = dev.index
+    for t in tensors:
+        if t.get_device() != index or not t.is_cuda:
+            L.require_device(tensors[0], t)                       # (raises)
+    return dev
+
+
+def _dtype_array(who: str, tensors: Sequence[torch.Tensor]) -> array:
+    ids = L.DTYPE_IDS
+    try:
+        return array("i", [ids[t.dtype] for t in tensors])
+    except KeyError as exc:
+        raise L.PhcError(f"{who}: float32, bfloat16 or float16 expected, got {exc.args[0]}") from None
+
+
 def _norm_clip(who: str, grads: Sequence[torch.Tensor], max_norm: float, norm_type: float, out: Optional[Sequence[torch.Tensor]]):
     """{norm, coefficient} of ``grads`` as a device tensor; the scaled gradients in ``out``."""
     lib = L.load()
@@ -191,22 +209,23 @@ def _norm_clip(who: str, grads: Sequence[torch.Tensor], max_norm: float, norm_ty
         raise L.PhcError(f"{who}: norm_type {norm_type} (known: 1, 2, inf)")
     if not max_norm >= 0.0:
         raise L.PhcError(f"{who}: max_norm {max_norm}")
-    dev = L.require_device(*grads, *(out or ()))
+    dev = _one_device(who, grads) if out is None or out is grads else _one_device(who, (*grads, *out))
     n = len(grads)
-    ids = L.DTYPE_IDS
-    try:
-        dtypes = (C.c_int32 * n)(*[ids[g.dtype] for g in grads])
-        out_dtypes = None if out is None else (C.c_int32 * n)(*[ids[o.dtype] for o in out])
-    except KeyError as exc:
-        raise L.PhcError(f"{who}: float32, bfloat16 or float16 expected, got {exc.args[0]}") from None
-    numel = (C.c_int64 * n)(*[g.numel() for g in grads])
-    src = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
-    dst = None if out is None else (C.c_void_p * n)(*[o.data_ptr() for o in out])
-    ws_bytes = lib.phc_grad_norm_ws_bytes(n, numel)
+    dtypes = _dtype_array(who, grads)
+    numel, src = array("q", [g.numel() for g in grads]), array("Q", [g.data_ptr() for g in grads])
+    if out is None:
+        dst = out_dtypes = None
+    elif out is grads:
+        dst, out_dtypes = src, dtypes
+    else:
+        dst, out_dtypes = array("Q", [o.data_ptr() for o in out]), _dtype_array(who, out)
+    host = lambda a: None if a is None else a.buffer_info()[0]
+    ws_bytes = lib.phc_grad_norm_ws_bytes(n, host(numel))
     res = torch.empty(2 + ws_bytes // 4, dtype=torch.float32, device=dev)          # {norm, coefficient} | workspace
+    at = res.data_ptr()
     with on_device(dev):
-        L.check(lib.phc_grad_norm_clip(n, src, numel, dtypes, kind, float(max_norm), dst, out_dtypes, L.ptr(res), L.ptr(res) + 8, ws_bytes,
-                                       L.stream_ptr(dev)), who)
+        L.check(lib.phc_grad_norm_clip(n, host(src), host(numel), host(dtypes), kind, float(max_norm), host(dst), host(out_dtypes), at, at + 8,
+                                       ws_bytes, raw_stream(dev)), who)
     return res
 
 

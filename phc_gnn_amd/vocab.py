@@ -46,25 +46,32 @@ def _int64(what: str, t: torch.Tensor) -> torch.Tensor:
     return t.to(torch.int64).contiguous()
 
 
-def _gradient_nodes(who: str, *tensors: Optional[torch.Tensor]) -> list:
+def raw_stream(dev: torch.device) -> int:
+    """The current stream of ``dev`` as a hipStream_t (``lib.stream_ptr`` without the Python stream object)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
+
+
+def _check_capture(who: str, dev: torch.device, *tensors: Optional[torch.Tensor]) -> None:
     """A leaf has ONE gradient node while any graph that ends in it lives, and autograd runs that node on the stream it was made on.  A
     backward captured on another stream would pull that stream into the capture, which ends the process when the capture ends: refused
-    here, before anything is recorded, for graphs these operators made.  The nodes carry the stream; the caller holds them until its
-    own graph does."""
-    nodes = []
-    if not torch.is_grad_enabled():
-        return nodes
-    for t in tensors:
-        if t is None or not t.requires_grad or not t.is_leaf:
-            continue
+    here, before anything is recorded, for graphs these operators made (``_tag``)."""
+    leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    if not leaves or not torch.is_grad_enabled() or not torch.cuda.is_current_stream_capturing():
+        return
+    for t in leaves:
         node = torch.autograd.graph.get_gradient_edge(t).node
-        stream = torch.cuda.current_stream(t.device).cuda_stream
-        made_on = node.metadata.setdefault("phc_stream", stream)
-        if made_on != stream and torch.cuda.is_current_stream_capturing():
+        if node.metadata.get("phc_stream", raw_stream(dev)) != raw_stream(dev):
             raise L.PhcError(f"{who}: captured into a graph while an eager result of the same parameter, made on another stream, still holds its "
                              "autograd graph; detach or delete that result (or make it on the capture's stream) first")
-        nodes.append(node)
-    return nodes
+
+
+def _tag(out: torch.Tensor, dev: torch.device) -> torch.Tensor:
+    """Marks the leaves' gradient nodes behind ``out`` with their stream (the nodes live as long as the graph)."""
+    if out.grad_fn is not None:
+        for fn, _ in out.grad_fn.next_functions:
+            if isinstance(fn, torch._C._functions.AccumulateGrad):
+                fn.metadata.setdefault("phc_stream", raw_stream(dev))
+    return out
 
 
 # ---- embedding ------------------------------------------------------------------------------------------------------------------
@@ -79,7 +86,7 @@ class _EmbeddingFn(torch.autograd.Function):
         out = torch.empty((*tokens.shape, D), dtype=w.dtype, device=dev)
         with on_device(dev):
             L.check(lib.phc_embedding_fwd(L.ptr(tokens), L.ptr(w), N, V, D, _row_stride(w), L.DTYPE_IDS[w.dtype], scale, L.ptr(out),
-                                          L.stream_ptr(dev)), "phc_embedding_fwd")
+                                          raw_stream(dev)), "phc_embedding_fwd")
         L.maybe_check_indices(dev)
         ctx.save_for_backward(tokens)
         ctx.meta = (V, D, w.dtype, scale, pad)
@@ -99,7 +106,7 @@ class _EmbeddingFn(torch.autograd.Function):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         with on_device(dev):
             L.check(lib.phc_embedding_bwd(L.ptr(tokens), L.ptr(dy), N, V, D, _row_stride(dy), L.DTYPE_IDS[dtype], scale, pad, L.ptr(dw),
-                                          L.ptr(ws), ws_bytes, L.stream_ptr(dev)), "phc_embedding_bwd")
+                                          L.ptr(ws), ws_bytes, raw_stream(dev)), "phc_embedding_bwd")
         return None, dw, None, None
 
 
@@ -113,16 +120,14 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     _dtype_id("embedding: weight", weight)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise L.PhcError(f"embedding: weight [V, D] expected, got {tuple(weight.shape)}")
-    nodes = _gradient_nodes("embedding", weight)
+    _check_capture("embedding", dev, weight)
     V = weight.shape[0]
     pad = -1
     if padding_idx is not None:
         if not -V <= padding_idx < V:
             raise L.PhcError(f"embedding: padding_idx {padding_idx} outside the {V} rows")
         pad = int(padding_idx) % V
-    out = _EmbeddingFn.apply(_int64("embedding: tokens", tokens), weight, float(scale), pad)
-    del nodes
-    return out
+    return _tag(_EmbeddingFn.apply(_int64("embedding: tokens", tokens), weight, float(scale), pad), dev)
 
 
 # ---- softmax cross entropy of a linear map ----------------------------------------------------------------------------------------
@@ -167,7 +172,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         d.loss = L.ptr(loss)
         ws = _xent_workspace(lib, d, 0, dev)
         with on_device(dev):
-            L.check(lib.phc_linear_xent_fwd(C.byref(d), L.stream_ptr(dev)), "phc_linear_xent_fwd")
+            L.check(lib.phc_linear_xent_fwd(C.byref(d), raw_stream(dev)), "phc_linear_xent_fwd")
         del ws
         L.maybe_check_indices(dev)
         ctx.save_for_backward(x_, w_, b_, target, state)
@@ -193,7 +198,7 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         d.dloss, d.dx, d.dW, d.db = L.ptr(g), L.ptr(dx), L.ptr(dw), L.ptr(db)
         ws = _xent_workspace(lib, d, 1, dev)
         with on_device(dev):
-            L.check(lib.phc_linear_xent_bwd(C.byref(d), L.stream_ptr(dev)), "phc_linear_xent_bwd")
+            L.check(lib.phc_linear_xent_bwd(C.byref(d), raw_stream(dev)), "phc_linear_xent_bwd")
         del ws
         return dx, dw, db, None, None, None, None
 
@@ -224,8 +229,8 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise L.PhcError(f"linear_cross_entropy: unknown reduction '{reduction}' (known: {sorted(_REDUCTIONS)})")
     if piece < 0:
         raise L.PhcError(f"linear_cross_entropy: piece {piece}")
-    nodes = _gradient_nodes("linear_cross_entropy", x, weight, bias)
+    _check_capture("linear_cross_entropy", dev, x, weight, bias)
     t = _int64("linear_cross_entropy: target", target).reshape(-1)
     loss = _LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, bias, t, int(ignore_index), _REDUCTIONS[reduction], int(piece))
-    del nodes
+    _tag(loss, dev)
     return loss.reshape(target.shape) if reduction == "none" else loss
