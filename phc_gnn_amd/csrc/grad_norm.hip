@@ -38,12 +38,6 @@ __device__ __forceinline__ int gn_tensor_of(const GnTable &t, int chunk) {
     return __builtin_amdgcn_readfirstlane(__popcll(a) + __popcll(b) - 1);
 }
 
-// Accesses in flight per thread.  16-bit tensors: 4 (157 us instead of 184 for 110 M bf16 gradients clipped into fp32 ones); fp32: one, the
-// 32 wavefronts of a CU already keep the memory busy, and more only spread its open pages (1 / 2 / 4 / 8 in flight: 1208 / 1228 /
-// 1257 / 1225 us for 536 M).
-template <typename T>
-constexpr int GN_AHEAD = sizeof(T) == 2 ? 4 : 1;
-
 // elements at any element-aligned address: one 16-byte access (the hardware takes unaligned addresses)
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) Loose {
@@ -87,18 +81,8 @@ __device__ __forceinline__ double gn_block_join(double v, double *red) {
 template <int KIND, typename T>
 __device__ __forceinline__ void gn_chunk(const T *__restrict__ g, int n, GnAcc<KIND> &acc) {
     constexpr int W = 16 / sizeof(T);
-    constexpr int STEP = GN_THREADS * W, AHEAD = GN_AHEAD<T>;
     int i = threadIdx.x * W;
-    for (; i + (AHEAD - 1) * STEP + W <= n; i += AHEAD * STEP) {
-        Loose<T> q[AHEAD];
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a) q[a] = *reinterpret_cast<const Loose<T> *>(g + i + a * STEP);
-#pragma unroll
-        for (int a = 0; a < AHEAD; ++a)
-#pragma unroll
-            for (int k = 0; k < W; ++k) acc.add(to_f32(q[a].v[k]));
-    }
-    for (; i + W <= n; i += STEP) {
+    for (; i + W <= n; i += GN_THREADS * W) {
         const Loose<T> q = *reinterpret_cast<const Loose<T> *>(g + i);
 #pragma unroll
         for (int k = 0; k < W; ++k) acc.add(to_f32(q.v[k]));
@@ -137,6 +121,12 @@ __global__ __launch_bounds__(1024) void grad_norm_finish_kernel(const double *__
         norm_coef[1] = c >= 1.0 ? 1.f : (float)c;            // (NaN stays NaN, as the gradients then are)
     }
 }
+
+// Accesses in flight per thread.  From 16-bit tensors 4 (157 us instead of 184 for 110 M bf16 gradients clipped into fp32 ones); from fp32 one:
+// the 32 wavefronts of a CU already keep the memory busy, and more only spread its open pages (1 / 2 / 4 in flight: 1208 / 1224 / 1257 us for
+// 536 M; the same holds for the norm's pass, 1208 / 1211 / 1244 us).
+template <typename T>
+constexpr int GN_AHEAD = sizeof(T) == 2 ? 4 : 1;
 
 // W results at an element-aligned address, past the caches (nothing reads them soon, and the gradients still to be scaled lie there)
 template <typename U, int W>

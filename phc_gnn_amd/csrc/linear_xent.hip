@@ -106,7 +106,7 @@ __device__ __forceinline__ void put_planes(const XPlanes &o, size_t at, const TI
 // Rows [R, C] -> operand rows [., Cp] (8 columns a thread), columns behind C zero.  `to`: row i goes to packed row to[i]; an ignored one
 // has its row of `zero` (dense [R, C], may be null) cleared instead; the packed rows behind `count` up to a whole step are zero.
 template <typename TIN>
-__global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ src, long long ld, long long R, int C, int Cp, int vec,
+__global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ src, long long ld, long long R, int C, int Cp,
                                                        const int *__restrict__ to, const int *__restrict__ count, TIN *__restrict__ zero, XPlanes out) {
     const int per = Cp / 8;
     const long long total = (R + (to ? XT_BK : 0)) * (long long)per;
@@ -130,11 +130,11 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ 
                 }
             }
         }
-        if (!fill && vec && c + 8 <= C) {
-            constexpr int H = 16 / sizeof(TIN);                   // 16-byte loads
+        if (!fill && c + 8 <= C) {
+            constexpr int H = 16 / sizeof(TIN);                   // 16-byte loads, at element-aligned addresses
 #pragma unroll
             for (int k = 0; k < 8; k += H) {
-                const Pack<TIN, H> q = *reinterpret_cast<const Pack<TIN, H> *>(src + r * ld + c + k);
+                const LoosePack<TIN, H> q = *reinterpret_cast<const LoosePack<TIN, H> *>(src + r * ld + c + k);
 #pragma unroll
                 for (int j = 0; j < H; ++j) v[k + j] = q.v[j];
             }
@@ -147,6 +147,7 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ 
 }
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void xt_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void xt_wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 // Eight LDS-DMA instructions: every lane's 16 bytes at base + voff[q] land at LDS byte address lds + 1024 q + 16 lane.  In asm because hipcc
@@ -230,7 +231,8 @@ struct XGemm {
     float *db_part;                // [tilesN * WN][rowsA] or null
     int N;
     // XE_DX / XE_DW
-    const float *scale;            // one value
+    const float *top, *dloss;      // g of the products: *top, or (no top) *dloss over the rows that count
+    int mean;
     float out_scale;
     const int *row_of;             // XE_DX: packed row -> output row
     void *out;                     // element (n, m) at n * ldo + m
@@ -242,6 +244,12 @@ struct XGemm {
 // 256 x 256 tiles need half the operand bytes of 128 x 128 ones per product, and fill the card only with enough of them.
 __host__ __device__ inline bool xt_big(int m, int n) {
     return m > 128 && n > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= 192;
+}
+
+// what the products of d are multiplied by: the largest |g_i| where the rows of d carry g_i / that, else the one g
+__device__ __forceinline__ float xt_scale(const float *top, const float *dloss, int mean, int count) {
+    if (top) return *top;
+    return mean ? (count > 0 ? *dloss / (float)count : 0.f) : *dloss;
 }
 
 // Work of a product over `tiles` output tiles: the k loop is split where the tiles alone do not fill the card, never below 4 steps.
@@ -317,33 +325,31 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     const int rowsB = EPI == XE_DW ? a.rowsB : count;
     const int tilesN = (rowsB + TN - 1) / TN, tiles = a.tilesM * tilesN;
     const int ksteps = EPI == XE_DW ? (count + XT_BK - 1) / XT_BK : (int)((a.K + XT_BK - 1) / XT_BK);
-    int split = 0, splits = 1, tile = blockIdx.x;
-    if constexpr (EPI == XE_DX || EPI == XE_DW) {
-        splits = xt_splits(tiles, a.segments * (EPI == XE_DW ? ksteps : a.split_k / XT_BK), a.max_blocks);
-        if (tiles > 0) {
-            split = tile / tiles;
-            tile -= split * tiles;
-        }
-    }
-    if (tiles == 0 || (EPI == XE_STATS || EPI == XE_DLOGITS ? tile >= tiles : split >= splits)) return;
-    int tm, tn;
-    xt_tile_of(tile, a.tilesM, tilesN, tm, tn);
     const int steps = a.segments * ksteps;
+    int splits = 1;
+    if constexpr (EPI == XE_DX || EPI == XE_DW) splits = xt_splits(tiles, a.segments * (EPI == XE_DW ? ksteps : a.split_k / XT_BK), a.max_blocks);
+    if ((int)blockIdx.x >= tiles * splits) return;
+    const int split = (int)blockIdx.x / tiles;
+    int tm, tn;
+    xt_tile_of(blockIdx.x - split * tiles, a.tilesM, tilesN, tm, tn);
     const int s0 = (int)((long long)steps * split / splits), n_steps = (int)((long long)steps * (split + 1) / splits) - s0;
 
     // loader
     const bool loads_a = wave * LOADS < TM / 8;
     const unsigned ld = loads_a ? a.lda : a.ldb;
     const bool tr = loads_a ? A_TR : B_TR;
-    const long long at0 = loads_a ? (long long)tm * TM : (long long)tn * TN;
     const int dma0 = wave * LOADS - (loads_a ? 0 : TM / 8);     // this wavefront's first instruction of its operand
+    const unsigned k_bytes = tr ? XT_BK * ld : XT_BK * 2;
+    const unsigned lds_wave = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem + wave * LOADS * 1024);
     // memory rows behind an operand's end repeat its last one: their results are dropped, or the other operand has zeros there
     const int rows = tr ? (EPI == XE_DW ? 0x7fffffff : (int)a.K) : loads_a ? a.rowsA : rowsB;
+
+    const int at0 = loads_a ? tm * TM : tn * TN;
     auto offset = [&](int q, int first, int limit) -> unsigned {
         if (tr) {
             const int per = loads_a ? SA::PIECES : SB::PIECES, row = (dma0 + q) * (64 / per) + lane / per;
             const int f = loads_a ? XSide<TM, true, false>::f(row) : XSide<TN, true, false>::f(row);
-            const int col = min((int)at0 + ((lane % per) ^ f) * 8, (loads_a ? a.colsA : (int)(a.ldb / 2)) - 8);
+            const int col = min(at0 + ((lane % per) ^ f) * 8, (loads_a ? a.colsA : (int)(a.ldb / 2)) - 8);
             return (unsigned)min(row, limit - 1 - first) * ld + (unsigned)col * 2;
         }
         const int row = (dma0 + q) * 8 + (lane >> 3);
@@ -352,13 +358,11 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     };
     unsigned voff[LOADS];
 #pragma unroll
-    for (int q = 0; q < LOADS; ++q) voff[q] = offset(q, tr ? 0 : (int)at0, tr ? XT_BK : rows);
-    const unsigned lds_wave = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem + wave * LOADS * 1024);
+    for (int q = 0; q < LOADS; ++q) voff[q] = offset(q, tr ? 0 : at0, tr ? XT_BK : rows);
     // the step that is loaded next
-    const unsigned k_bytes = tr ? XT_BK * ld : XT_BK * 2;
     int seg = __builtin_amdgcn_readfirstlane(s0 / (ksteps > 0 ? ksteps : 1)), kst = __builtin_amdgcn_readfirstlane(s0 - seg * ksteps);
     auto plane = [&]() { return uniform((loads_a ? a.A[seg] : a.B[seg]) + (tr ? 0 : (size_t)at0 * ld) + (size_t)kst * k_bytes); };
-    const char *base = plane();
+    const char *base = n_steps > 0 ? plane() : nullptr;
     auto issue = [&](int buf) {
         if (A_TR && EPI != XE_DW && tr && (kst + 1) * XT_BK > rows) {           // the last rows of k
             unsigned last[LOADS];
@@ -374,6 +378,34 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
             if (++seg < a.segments) base = plane();
         }
     };
+    // What the epilogue of the logits needs, {target, logsumexp, g / max g} of the tile's rows and the bias of its columns: loaded by a
+    // thread each in front of the first steps (loads return in order), kept in LDS behind the buffers.
+    constexpr bool LOGITS = EPI == XE_STATS || EPI == XE_DLOGITS;
+    typedef std::conditional_t<WIDE, float, T> TB;              // the inputs' type
+    struct Row {
+        int hit;
+        float lse, rel;
+    };
+    static_assert(!LOGITS || NW * 64 == TM + TN, "a thread for each row and column of the tile");
+    Row *const row_meta = reinterpret_cast<Row *>(smem + 2 * BUF + WM * TN * sizeof(float2));             // [TN]
+    float *const bias_meta = reinterpret_cast<float *>(row_meta + TN);                                    // [TM]
+    Row my_row{-1, 0.f, 0.f};
+    float my_bias = 0.f;
+    if constexpr (LOGITS) {
+        if ((int)threadIdx.x < TN) {
+            const int n = tn * TN + threadIdx.x;
+            if (n < count) my_row = Row{a.target[n] - a.first_v, EPI == XE_DLOGITS ? a.lse[n] : 0.f, EPI == XE_DLOGITS && a.rel ? a.rel[n] : 1.f};
+        } else {
+            const int m = tm * TM + threadIdx.x - TN;
+            my_bias = m >= a.rowsA ? -INFINITY : a.bias ? to_f32(static_cast<const TB *>(a.bias)[m]) : 0.f;     // (columns behind the vocabulary: exp 0)
+        }
+    }
+    if (n_steps > 0) issue(0);
+    if (n_steps > 1) issue(1);
+    if constexpr (LOGITS) {
+        if ((int)threadIdx.x < TN) row_meta[threadIdx.x] = my_row;
+        else bias_meta[threadIdx.x - TN] = my_bias;
+    }
 
     f32x4_t acc[FM][FN];
 #pragma unroll
@@ -399,10 +431,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     lds_char *lds = (lds_char *)smem;
     if (n_steps > 0) {
         frag fa[2][FM], fb[2][FN];
-        issue(0);
         xt_wait_all();
         __builtin_amdgcn_s_barrier();
-        if (n_steps > 1) issue(1);
 #pragma unroll
         for (int j = 0; j < FN; ++j) fb[0][j] = SB::template read<frag>(lds + TM * 128, nb, j, 0, lane);
 #pragma unroll
@@ -424,34 +454,32 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     const int fr = lane & 15, fg = lane >> 4;
     const int m_base = tm * TM + ma, n0 = tn * TN + nb + fr;
     auto m_of = [&](int i) { return m_base + SA::index(i, fg * 4); };
-    if constexpr (EPI == XE_STATS || EPI == XE_DLOGITS) {
-        typedef std::conditional_t<WIDE, float, T> TB;
-        float bias[FM][4];
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int m = m_of(i) + r;
-                float b = 0.f;
-                if (a.bias && m < a.rowsA) b = to_f32(static_cast<const TB *>(a.bias)[m]);
-                bias[i][r] = m < a.rowsA ? b : -INFINITY;       // columns behind the vocabulary: exp 0
-            }
+    if constexpr (LOGITS) {
+        const Row *row_of = row_meta + nb + fr;
+        auto bias = [&](int i, int r) { return bias_meta[ma + SA::index(i, fg * 4) + r]; };
         if constexpr (EPI == XE_STATS) {
             float mx[FN], sum[FN];
+            int hit[FN];
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
-                const int n = n0 + j * 16;
-                const int hit = n < rowsB ? a.target[n] - a.first_v : -1;
+                hit[j] = row_of[j * 16].hit;
                 mx[j] = -INFINITY;
+            }
 #pragma unroll
-                for (int i = 0; i < FM; ++i)
+            for (int i = 0; i < FM; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float l = acc[i][j][r] + bias[i][r];
+                for (int r = 0; r < 4; ++r) {
+                    const float b = bias(i, r);
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) {
+                        const float l = acc[i][j][r] + b;
                         acc[i][j][r] = l;
                         mx[j] = fmaxf(mx[j], l);
-                        if (hit == m_of(i) + r) a.target_logit[n] = l;
+                        if (hit[j] == m_of(i) + r) a.target_logit[n0 + j * 16] = l;
                     }
+                }
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
                 mx[j] = fmaxf(mx[j], __shfl_xor(mx[j], 16));
                 mx[j] = fmaxf(mx[j], __shfl_xor(mx[j], 32));
                 const float shift = mx[j] == -INFINITY ? 0.f : mx[j];       // nothing but -inf: every exponential is 0
@@ -463,13 +491,13 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
                 sum[j] += __shfl_xor(sum[j], 16);
                 sum[j] += __shfl_xor(sum[j], 32);
             }
-            // the wavefronts along m, through LDS
-            __syncthreads();
-            float2 *meet = reinterpret_cast<float2 *>(smem);                // [WM][TN]
+            // the wavefronts along m, through LDS behind the buffers (a barrier that orders LDS alone)
+            float2 *meet = reinterpret_cast<float2 *>(smem + 2 * BUF);      // [WM][TN]
             if (fg == 0)
 #pragma unroll
                 for (int j = 0; j < FN; ++j) meet[wm * TN + nb + j * 16 + fr] = make_float2(mx[j], sum[j]);
-            __syncthreads();
+            xt_wait_lds();
+            __builtin_amdgcn_s_barrier();
             for (int c = threadIdx.x; c < TN; c += NW * 64) {
                 const int n = tn * TN + c;
                 if (n >= rowsB) continue;
@@ -484,44 +512,43 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
             }
         } else {
             const int n_end = (count + XT_BK - 1) / XT_BK * XT_BK;          // zero rows up to a whole step of the weight gradient's k
-            float dbs[FM][4] = {};
+            Row row[FN];
 #pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                const int n = n0 + j * 16;
-                const bool in = n < count;
-                const int hit = in ? a.target[n] - a.first_v : -1;
-                const float lse = in ? a.lse[n] : 0.f, rel = in ? a.rel[n] : 0.f;
+            for (int j = 0; j < FN; ++j) row[j] = row_of[j * 16];
 #pragma unroll
-                for (int i = 0; i < FM; i += 2) {
+            for (int i = 0; i < FM; i += 2) {
+                float b[8], db[8] = {};
+#pragma unroll
+                for (int e = 0; e < 8; ++e) b[e] = bias(i + e / 4, e % 4);
+                const int m0 = m_of(i);                                      // 8 consecutive columns of two fragments
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    const int n = n0 + j * 16;
                     TB d[8];
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const int ii = i + e / 4, r = e % 4, m = m_of(ii) + r;
-                        const float l = acc[ii][j][r] + bias[ii][r];
-                        const float p = WIDE ? expf(l - lse) : __expf(l - lse);
-                        const float v = in && m < a.rowsA ? (p - (hit == m ? 1.f : 0.f)) * rel : 0.f;
-                        dbs[ii][r] += v;
+                        const float l = acc[i + e / 4][j][e % 4] + b[e];
+                        const float p = WIDE ? expf(l - row[j].lse) : __expf(l - row[j].lse);
+                        const float v = n < count && m0 + e < a.rowsA ? (p - (row[j].hit == m0 + e ? 1.f : 0.f)) * row[j].rel : 0.f;
+                        db[e] += v;
                         d[e] = (TB)(v * a.d_scale);
                     }
-                    if (n < n_end && m_of(i) < a.ldd) put_planes<TB, 8>(a.d, (size_t)n * a.ldd + m_of(i), d);
+                    if (n < n_end && m0 < a.ldd) put_planes<TB, 8>(a.d, (size_t)n * a.ldd + m0, d);
                 }
-            }
-            if (a.db_part) {
+                if (a.db_part)
 #pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        float v = dbs[i][r];
+                    for (int e = 0; e < 8; ++e) {
+                        float v = db[e];
 #pragma unroll
                         for (int x = 1; x < 16; x <<= 1) v += __shfl_xor(v, x);
-                        const int m = m_of(i) + r;
-                        if (fr == 0 && m < a.rowsA) a.db_part[(size_t)(tn * WN + wn) * a.rowsA + m] = v;
+                        if (fr == 0 && m0 + e < a.rowsA) a.db_part[(size_t)(tn * WN + wn) * a.rowsA + m0 + e] = v;
                     }
+                __builtin_amdgcn_sched_barrier(0);                           // (registers: one pair of fragments at a time)
             }
         }
     } else {
         typedef std::conditional_t<WIDE, float, T> TO;
-        const float s = a.out_scale * *a.scale;
+        const float s = a.out_scale * xt_scale(a.top, a.dloss, a.mean, count);
         const bool final = splits == 1 && (EPI == XE_DW || a.pieces == 1);
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
@@ -742,7 +769,7 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
                                                         const int *__restrict__ count, const float *__restrict__ target_logit,
                                                         const int *__restrict__ from, float *__restrict__ lse, float *__restrict__ row_loss,
                                                         float *__restrict__ loss) {
-    __shared__ float sm[64][16], ss[64][16];
+    __shared__ float sm[16][16], ss[16][16];
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int n = blockIdx.x * 16 + c, kept = *count;
     if (blockIdx.x * 16 >= kept) return;
@@ -750,11 +777,20 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
     float mx = -INFINITY, sum = 0.f;
     if (n < kept)
         for (int p = group; p < parts; p += 64) xt_join(mx, sum, part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
-    sm[group][c] = mx;
-    ss[group][c] = sum;
+    // lane groups of a wavefront, then the wavefronts
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) xt_join(mx, sum, __shfl_xor(mx, d), __shfl_xor(sum, d));
+    if ((threadIdx.x & 63) < 16) {
+        sm[threadIdx.x >> 6][c] = mx;
+        ss[threadIdx.x >> 6][c] = sum;
+    }
     __syncthreads();
+    if (threadIdx.x >= 64) return;
+    mx = -INFINITY, sum = 0.f;
+    for (int w = group; w < 16; w += 4) xt_join(mx, sum, sm[w][c], ss[w][c]);
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) xt_join(mx, sum, __shfl_xor(mx, d), __shfl_xor(sum, d));
     if (group == 0 && n < kept) {
-        for (int w = 1; w < 64; ++w) xt_join(mx, sum, sm[w][c], ss[w][c]);
         const float l = mx + logf(sum);
         lse[n] = l;
         row_loss[n] = l - target_logit[n];
@@ -784,14 +820,13 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float *__restri
     }
 }
 
-// g_i of every packed row: top = max |g_i|, rel = g_i / top (what the rows of d carry; top goes to the products' outputs)
-__global__ __launch_bounds__(1024) void xent_scales_kernel(const float *__restrict__ dloss, int per_row, int mean, const int *__restrict__ count,
+// A g_i of its own for every packed row: top = max |g_i|, rel = g_i / top (what the rows of d carry; top goes to the products' outputs)
+__global__ __launch_bounds__(1024) void xent_scales_kernel(const float *__restrict__ dloss, const int *__restrict__ count,
                                                           const int *__restrict__ from, float *__restrict__ rel, float *__restrict__ top) {
     __shared__ float red[16];
     const int kept = *count;
-    auto g_of = [&](int i) { return per_row ? dloss[from[i]] : mean ? dloss[0] / (float)kept : dloss[0]; };
     float m = 0.f;
-    for (int i = threadIdx.x; i < kept; i += 1024) m = fmaxf(m, fabsf(g_of(i)));
+    for (int i = threadIdx.x; i < kept; i += 1024) m = fmaxf(m, fabsf(dloss[from[i]]));
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
@@ -799,7 +834,7 @@ __global__ __launch_bounds__(1024) void xent_scales_kernel(const float *__restri
     for (int w = 0; w < 16; ++w) m = fmaxf(m, red[w]);
     if (threadIdx.x == 0) *top = m;
     for (int i = threadIdx.x; i < kept; i += 1024) {
-        const float g = g_of(i);
+        const float g = dloss[from[i]];
         rel[i] = g == 0.f ? 0.f : g / m;
     }
 }
@@ -813,19 +848,36 @@ __global__ __launch_bounds__(256) void xent_sum_slabs_kernel(const float *__rest
     const int steps = segments * (row_of ? split_steps : (*count + XT_BK - 1) / XT_BK);
     const int n = xt_splits(tilesM * ((rows + TN - 1) / TN), steps, max_blocks);
     if (n == 1 && (!row_of || pieces == 1)) return;
-    const long long total = (long long)rows * D;
-    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < total; e += (long long)gridDim.x * 256) {
-        float v = slabs[e];
-        for (int s = 1; s < n; ++s) v += slabs[(size_t)s * total + e];
-        const long long r = e / D;
-        out[row_of ? (long long)row_of[r] * D + (e - r * D) : e] = from_f32<T>(v);
+    const size_t total = (size_t)rows * D;
+    const int per = (D + 3) / 4;                                  // 4 elements a thread
+    for (long long e = (long long)blockIdx.x * 256 + threadIdx.x; e < (long long)rows * per; e += (long long)gridDim.x * 256) {
+        const int r = (int)(e / per), c = (int)(e - (long long)r * per) * 4;
+        const float *src = slabs + (size_t)r * D + c;
+        T *dst = out + (size_t)(row_of ? row_of[r] : r) * D + c;
+        if (c + 4 <= D) {
+            float v[4];
+            load_loose<float, 4>(src, v);
+            for (int s = 1; s < n; ++s) {
+                float o[4];
+                load_loose<float, 4>(src + s * total, o);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] += o[k];
+            }
+            store_loose<T, 4>(dst, v);
+        } else {
+            for (int k = 0; c + k < D; ++k) {
+                float v = src[k];
+                for (int s = 1; s < n; ++s) v += src[s * total + k];
+                dst[k] = from_f32<T>(v);
+            }
+        }
     }
 }
 
 // db[v] = top sum over the row tiles' partial sums, in order: 16 columns a workgroup, 16 lane groups share the parts
 template <typename T>
 __global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ part, const int *__restrict__ count, int nv,
-                                                     const float *__restrict__ top, T *__restrict__ db) {
+                                                     const float *__restrict__ top, const float *__restrict__ dloss, int mean, T *__restrict__ db) {
     __shared__ float meet[16][16];
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4, v = blockIdx.x * 16 + c;
     const int n = xt_big(nv, *count) ? (*count + 255) / 256 * 4 : (*count + 127) / 128 * 2;
@@ -836,7 +888,7 @@ __global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ 
     __syncthreads();
     if (group == 0 && v < nv) {
         for (int w = 1; w < 16; ++w) s += meet[w][c];
-        db[v] = from_f32<T>(s * *top);
+        db[v] = from_f32<T>(n > 0 ? s * xt_scale(top, dloss, mean, *count) : 0.f);
     }
 }
 
@@ -956,9 +1008,8 @@ static unsigned flat_grid(long long n) {
 
 template <typename T>
 static void pack_as(const void *src, long long ld, long long R, long long C, long long Cp, const XRows *rows, void *zero, const XPlanes &out, hipStream_t s) {
-    const int vec = aligned_to(src, 16) && (ld * sizeof(T)) % 16 == 0;
     PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_pack_kernel<T>), dim3(flat_grid((R + (rows ? XT_BK : 0)) * (Cp / 8))), dim3(256), 0, s, static_cast<const T *>(src), ld,
-                  R, (int)C, (int)Cp, vec, rows ? (const int *)rows->to : (const int *)nullptr, rows ? (const int *)rows->count : (const int *)nullptr,
+                  R, (int)C, (int)Cp, rows ? (const int *)rows->to : (const int *)nullptr, rows ? (const int *)rows->count : (const int *)nullptr,
                   static_cast<T *>(zero), out);
 }
 static void pack(int dtype, const void *src, long long ld, long long R, long long C, long long Cp, const XRows *rows, void *zero, const XPlanes &out,
@@ -979,12 +1030,13 @@ static void set_planes(const XPlan &p, const XPlanes &A, const XPlanes &B, XGemm
 
 template <typename T, int EPI, bool WIDE, typename TILE>
 static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
-    constexpr int LDS = 4 * TILE::SIZE * 128;
+    constexpr int LDS = 4 * TILE::SIZE * 128 + TILE::SIZE * (TILE::WM * (int)sizeof(float2) + 12 + 4);      // buffers, the wavefronts' meeting place, rows and columns
     g.tilesM = (int)ceil_div(g.rowsA, TILE::SIZE);
     g.tilesN = (int)ceil_div(g.rowsB, TILE::SIZE);
     g.max_blocks = TILE::BLOCKS;
     auto kernel = xent_gemm_kernel<T, EPI, WIDE, TILE::WM, TILE::WN, TILE::FM, TILE::FN>;
     if (!ensure_dynamic_lds(kernel, LDS)) return false;
+    // a workgroup for each tile; dx, dW: or for each split of them
     long long blocks = (long long)g.tilesM * g.tilesN;
     if ((EPI == XE_DX || EPI == XE_DW) && blocks < TILE::BLOCKS) blocks = TILE::BLOCKS;
     PHC_LAUNCH_AS(kid, kernel, dim3((unsigned)blocks), dim3(TILE::WM * TILE::WN * 64), LDS, s, g);
@@ -1008,7 +1060,7 @@ static int gemm(const phc_linear_xent_desc *d, int kid, bool big, XGemm &g, hipS
 
 template <typename T>
 static void sum_slabs_as(int kid, const float *slabs, const XGemm &g, int tile, int pieces, void *out, hipStream_t s) {
-    PHC_LAUNCH_AS(kid, (xent_sum_slabs_kernel<T>), dim3(flat_grid((long long)g.rowsB * g.ldo)), dim3(256), 0, s, slabs, g.count, g.rowsB, g.tilesM, tile,
+    PHC_LAUNCH_AS(kid, (xent_sum_slabs_kernel<T>), dim3(flat_grid((long long)g.rowsB * ceil_div(g.ldo, 4))), dim3(256), 0, s, slabs, g.count, g.rowsB, g.tilesM, tile,
                   g.split_k / XT_BK, g.segments, g.max_blocks, g.ldo, pieces, g.row_of, static_cast<T *>(out));
 }
 static void sum_slabs(int dtype, int kid, const float *slabs, const XGemm &g, int tile, int pieces, void *out, hipStream_t s) {
@@ -1018,8 +1070,8 @@ static void sum_slabs(int dtype, int kid, const float *slabs, const XGemm &g, in
 }
 
 template <typename T>
-static void db_as(const float *part, const XRows &r, int nv, const float *top, void *db, hipStream_t s) {
-    PHC_LAUNCH_AS(K_XENT_DW, (xent_db_kernel<T>), dim3((unsigned)ceil_div(nv, 16)), dim3(256), 0, s, part, (const int *)r.count, nv, top,
+static void db_as(const float *part, const XRows &r, int nv, const float *top, const float *dloss, int mean, void *db, hipStream_t s) {
+    PHC_LAUNCH_AS(K_XENT_DW, (xent_db_kernel<T>), dim3((unsigned)ceil_div(nv, 16)), dim3(256), 0, s, part, (const int *)r.count, nv, top, dloss, mean,
                   static_cast<T *>(db));
 }
 
@@ -1127,8 +1179,11 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
     XWs w(d, p, true, d->ws);
     const XState st(d->N, d->state);
     const int es = dtype_bytes(d->dtype), N = (int)d->N;
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_scales_kernel, dim3(1), dim3(1024), 0, s, d->dloss, d->reduction == PHC_REDUCE_NONE ? 1 : 0,
-                  d->reduction == PHC_REDUCE_MEAN ? 1 : 0, (const int *)st.rows.count, (const int *)st.rows.from, w.rel, w.top);
+    const bool per_row = d->reduction == PHC_REDUCE_NONE;
+    const float *rel = per_row ? w.rel : nullptr, *top = per_row ? w.top : nullptr;
+    const int mean = d->reduction == PHC_REDUCE_MEAN ? 1 : 0;
+    if (per_row)
+        PHC_LAUNCH_AS(K_XENT_ROWS, xent_scales_kernel, dim3(1), dim3(1024), 0, s, d->dloss, (const int *)st.rows.count, (const int *)st.rows.from, w.rel, w.top);
     pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &st.rows, d->dx, w.x, s);
     // fp16 has no normal values below 6e-5, where most probabilities of a large vocabulary lie: its d are stored times 2^14
     const float d_scale = d->dtype == PHC_DTYPE_F16 ? 16384.f : 1.f;
@@ -1154,7 +1209,7 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         g.target = st.rows.target;
         g.first_v = (int)v0;
         g.lse = st.lse;
-        g.rel = w.rel;
+        g.rel = rel;
         g.d = w.dl;
         g.ldd = nvp;
         g.d_scale = d_scale;
@@ -1162,9 +1217,9 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         if (int rc = gemm<XE_DLOGITS>(d, K_XENT_DLOGITS, p.big_d, g, s)) return rc;
         if (d->db) {
             char *db = static_cast<char *>(d->db) + (size_t)v0 * es;
-            if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, st.rows, nv, w.top, db, s);
-            else if (d->dtype == PHC_DTYPE_BF16) db_as<bf16_t>(w.db_part, st.rows, nv, w.top, db, s);
-            else db_as<f16_t>(w.db_part, st.rows, nv, w.top, db, s);
+            if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, st.rows, nv, top, d->dloss, mean, db, s);
+            else if (d->dtype == PHC_DTYPE_BF16) db_as<bf16_t>(w.db_part, st.rows, nv, top, d->dloss, mean, db, s);
+            else db_as<f16_t>(w.db_part, st.rows, nv, top, d->dloss, mean, db, s);
         }
         if (d->dx) {
             o = XGemm{};
@@ -1177,7 +1232,9 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             o.colsA = (int)p.wcols;
             o.rowsB = N;
             o.count = st.rows.count;
-            o.scale = w.top;
+            o.top = top;
+            o.dloss = d->dloss;
+            o.mean = mean;
             o.out_scale = 1.f / d_scale;
             o.row_of = st.rows.from;
             o.out = d->dx;
@@ -1196,7 +1253,9 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             q.colsA = (int)p.Kp;
             q.rowsB = nv;
             q.count = st.rows.count;
-            q.scale = w.top;
+            q.top = top;
+            q.dloss = d->dloss;
+            q.mean = mean;
             q.out_scale = 1.f / d_scale;
             q.out = static_cast<char *>(d->dW) + (size_t)v0 * d->D * es;
             q.ldo = (int)d->D;

@@ -58,7 +58,7 @@ def _formula(x, w, b, t, reduction, up, ignore=-100):
         g = (up.double() / count).expand(n)
     g = torch.where(kept, g, torch.zeros_like(g))
     D = p.clone()
-    D[torch.arange(n), at] -= 1.0
+    D[torch.arange(n, device=D.device), at] -= 1.0
     D[~kept] = 0
     half = torch.finfo(x.dtype).eps / 2 if not wide else 2.0 ** -25
     tiny = 2.0 ** -39 if x.dtype == torch.float16 else 2.0 ** -130
@@ -118,6 +118,19 @@ def test_vocabulary_in_pieces(piece, reduction, dtype):
 @pytest.mark.parametrize("n,v,d", [(1100, 2500, 320), (640, 3001, 576), (2000, 700, 136)])
 def test_more_tiles_and_splits(n, v, d, dtype):
     _check(n, v, d, dtype, reduction="mean", ignored=0.05, seed=7)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(40, 66003, 64), (150, 33100, 300), (33100, 150, 300), (2700, 7000, 130)])
+def test_more_tiles_than_the_card_holds(n, v, d, dtype):
+    """More output tiles than workgroups fit at once, in each of the products (256 of the large tiles, 512 of the small ones).  The formula
+    and its bounds on the GPU, in 64 bits."""
+    x, w, b, t = (q.to(DEV) for q in _case(n, v, d, dtype, seed=9))
+    up = torch.tensor(1.0, device=DEV)
+    exact, bound = _formula(x, w, b, t, "mean", up)
+    for what, a, e, m in zip(("loss", "dx", "dW", "db"), _run(x, w, b, t, "mean", up), exact, bound):
+        err = (a.double() - e).abs()
+        assert bool((err <= m).all()), (what, float(err.max()), float((err / m).max()))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
