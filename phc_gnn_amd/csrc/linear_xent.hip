@@ -20,7 +20,8 @@
 
 namespace phc {
 
-constexpr int XT_BK = 64;                      // k per step: 128 bytes of a k-contiguous row = one line of LDS
+constexpr int XT_ROW = 128;                    // bytes of a k-contiguous operand row per step = one line of LDS: 64 k of 16 bits, 32 of fp32
+constexpr int XT_BK = 64;                      // what rows and columns of operands are padded to
 
 // ---- rows that count --------------------------------------------------------------------------------------------------------------------
 // Rows whose target is ignored cost nothing: the others are numbered in order ("packed" rows), and every product runs over those.
@@ -85,10 +86,10 @@ __device__ __forceinline__ void split3(float a, bf16_t &h, bf16_t &m, bf16_t &l)
     l = (bf16_t)(r - (float)m);
 }
 
-// W consecutive values -> the operand planes (one for 16-bit types, three for fp32)
-template <typename TIN, int W>
+// W consecutive values -> the operand: as they are, or (SPLIT) in three planes
+template <bool SPLIT, typename TIN, int W>
 __device__ __forceinline__ void put_planes(const XPlanes &o, size_t at, const TIN (&v)[W]) {
-    if constexpr (sizeof(TIN) == 4) {
+    if constexpr (SPLIT) {
         Pack<bf16_t, W> h, m, l;
 #pragma unroll
         for (int i = 0; i < W; ++i) split3(v[i], h.v[i], m.v[i], l.v[i]);
@@ -96,16 +97,20 @@ __device__ __forceinline__ void put_planes(const XPlanes &o, size_t at, const TI
         *reinterpret_cast<Pack<bf16_t, W> *>(static_cast<bf16_t *>(o.p[1]) + at) = m;
         *reinterpret_cast<Pack<bf16_t, W> *>(static_cast<bf16_t *>(o.p[2]) + at) = l;
     } else {
-        Pack<TIN, W> q;
+        constexpr int H = 16 / sizeof(TIN);
 #pragma unroll
-        for (int i = 0; i < W; ++i) q.v[i] = v[i];
-        *reinterpret_cast<Pack<TIN, W> *>(static_cast<TIN *>(o.p[0]) + at) = q;
+        for (int k = 0; k < W; k += H) {
+            Pack<TIN, H> q;
+#pragma unroll
+            for (int i = 0; i < H; ++i) q.v[i] = v[k + i];
+            *reinterpret_cast<Pack<TIN, H> *>(static_cast<TIN *>(o.p[0]) + at + k) = q;
+        }
     }
 }
 
 // Rows [R, C] -> operand rows [., Cp] (8 columns a thread), columns behind C zero.  `to`: row i goes to packed row to[i]; an ignored one
 // has its row of `zero` (dense [R, C], may be null) cleared instead; the packed rows behind `count` up to a whole step are zero.
-template <typename TIN>
+template <typename TIN, bool SPLIT>
 __global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ src, long long ld, long long R, int C, int Cp,
                                                        const int *__restrict__ to, const int *__restrict__ count, TIN *__restrict__ zero, XPlanes out) {
     const int per = Cp / 8;
@@ -142,7 +147,7 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ 
 #pragma unroll
             for (int k = 0; k < 8; ++k) v[k] = !fill && c + k < C ? src[r * ld + c + k] : (TIN)0.f;
         }
-        put_planes<TIN, 8>(out, (size_t)at * Cp + c, v);
+        put_planes<SPLIT, TIN, 8>(out, (size_t)at * Cp + c, v);
     }
 }
 
@@ -150,10 +155,10 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ 
 __device__ __forceinline__ void xt_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void xt_wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
-// Eight LDS-DMA instructions: every lane's 16 bytes at base + voff[q] land at LDS byte address lds + 1024 q + 16 lane.  In asm because hipcc
+// Eight (four) LDS-DMA instructions: every lane's 16 bytes at base + voff[q] land at LDS byte address lds + 1024 q + 16 lane.  In asm because hipcc
 // orders its builtin against every later LDS read with s_waitcnt vmcnt(0), which would drain the prefetch; the loop's own waits order
 // them.  M0 is the DMA's LDS base, saved and restored inside the statement.
-__device__ __forceinline__ void xt_dma8(unsigned lds, const unsigned (&voff)[8], const void *base) {
+__device__ __forceinline__ void xt_dma(unsigned lds, const unsigned (&voff)[8], const void *base) {
     unsigned keep;
     asm volatile(
         "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %10\n\t"
@@ -167,6 +172,19 @@ __device__ __forceinline__ void xt_dma8(unsigned lds, const unsigned (&voff)[8],
         "s_mov_b32 m0, %0"
         : "=&s"(keep)
         : "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "v"(voff[4]), "v"(voff[5]), "v"(voff[6]), "v"(voff[7]), "s"(base)
+        : "memory", "scc");
+}
+
+__device__ __forceinline__ void xt_dma(unsigned lds, const unsigned (&voff)[4], const void *base) {
+    unsigned keep;
+    asm volatile(
+        "s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %6\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %3, %6\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %4, %6\n\t"
+        "s_add_u32 m0, m0, 0x400\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %5, %6\n\t"
+        "s_mov_b32 m0, %0"
+        : "=&s"(keep)
+        : "s"(lds), "v"(voff[0]), "v"(voff[1]), "v"(voff[2]), "v"(voff[3]), "s"(base)
         : "memory", "scc");
 }
 
@@ -188,6 +206,17 @@ template <>
 struct Mfma16<f16_t> {
     typedef f16x8_t frag;
     static __device__ __forceinline__ f32x4_t mul(frag a, frag b, f32x4_t c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// fp32: 16 bytes are 4 k of each of 4 lane groups, product q takes the q-th of each (any order of k will do that both operands share)
+template <>
+struct Mfma16<float> {
+    typedef f32x4_t frag;
+    static __device__ __forceinline__ f32x4_t mul(frag a, frag b, f32x4_t c) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], b[q], c, 0, 0, 0);
+        return c;
+    }
 };
 
 typedef __attribute__((ext_vector_type(4))) short s16x4_t;
@@ -272,15 +301,15 @@ __device__ __forceinline__ void xt_tile_of(unsigned b, int tilesM, int tilesN, i
     tn = (int)(in / height);
 }
 
-// One operand's side of the tile: T rows (m or n) by XT_BK of k, in LDS either as it is read k-contiguous, [T][64], or, where memory holds
-// it as [k][m], as [64][T] with the transposing LDS read.  16-byte pieces of an LDS row are stored at piece ^ f(row), which spreads the
-// banks of the 8 (16) rows that a quarter wavefront reads together.
-template <int T, bool TR, bool PAIR>
+// One operand's side of the tile: S rows (m or n) by a step's k, in LDS either as it is read k-contiguous, [S][128 bytes], or, where memory
+// holds it as [k][m], as [k][S] (16 bits: with the transposing LDS read; fp32: a word for each k).  16-byte pieces of an LDS row are stored at
+// piece ^ f(row), which spreads the banks of the rows that are read together.
+template <typename T, int S, bool TR, bool PAIR>
 struct XSide {
-    static constexpr int PIECES = TR ? T / 8 : 8;                       // per LDS row
-    static constexpr int ROWS_PER_DMA = 64 / PIECES;
+    static constexpr int BK = XT_ROW / sizeof(T);
+    static constexpr int PIECES = TR ? S * (int)sizeof(T) / 16 : 8;     // per LDS row
     static __device__ __forceinline__ int f(int row) {
-        if constexpr (TR) return ((row & 3) << 1) ^ (((row >> 3) & 1) << 3);
+        if constexpr (TR) return sizeof(T) == 4 ? ((row >> 2) & 3) << 2 : ((row & 3) << 1) ^ (((row >> 3) & 1) << 3);
         else return PAIR ? (row & 3) | ((row >> 1) & 4) : row & 7;
     }
     // m (n) of row rho of fragment i.  PAIR: two fragments give a lane 8 consecutive m (it holds rows 4 g .. 4 g + 3 of each).
@@ -291,15 +320,22 @@ struct XSide {
     template <typename frag>
     static __device__ __forceinline__ frag read(lds_char *tile, int first, int i, int kk, int lane) {
         const int rho = lane & 15, g = lane >> 4;
-        if constexpr (TR) {
+        if constexpr (TR && sizeof(T) == 4) {
+            const int k = kk * 16 + g * 4, piece = ((first + i * 16) >> 2) + (rho >> 2);
+            lds_char *at = tile + k * (S * 4) + ((piece ^ f(k)) << 4) + (rho & 3) * 4;          // f(k) .. f(k + 3) are the same
+            frag r;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) r[q] = *(__attribute__((address_space(3))) const float *)(at + q * (S * 4));
+            return r;
+        } else if constexpr (TR) {
             const int k = kk * 32 + g * 8 + (rho >> 2), piece = ((first + i * 16) >> 3) + ((rho >> 1) & 1);
-            lds_char *at = tile + k * (T * 2) + ((piece ^ f(k)) << 4) + (rho & 1) * 8;          // f(k + 4) = f(k)
+            lds_char *at = tile + k * (S * 2) + ((piece ^ f(k)) << 4) + (rho & 1) * 8;          // f(k + 4) = f(k)
             const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)at);
-            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 4 * (T * 2)));
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(at + 4 * (S * 2)));
             return __builtin_bit_cast(frag, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             const int row = first + index(i, rho);
-            return __builtin_bit_cast(frag, *(lds_s16x8 *)(tile + row * 128 + (((kk * 4 + g) ^ f(row)) << 4)));
+            return __builtin_bit_cast(frag, *(lds_s16x8 *)(tile + row * XT_ROW + (((kk * 4 + g) ^ f(row)) << 4)));
         }
     }
 };
@@ -309,12 +345,13 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     typedef typename Mfma16<T>::frag frag;
     constexpr int NW = WM * WN, TM = WM * FM * 16, TN = WN * FN * 16;
     constexpr bool A_TR = EPI == XE_DX || EPI == XE_DW, B_TR = EPI == XE_DW, PAIR = EPI == XE_DLOGITS;
-    typedef XSide<TM, A_TR, PAIR> SA;
-    typedef XSide<TN, B_TR, false> SB;
+    typedef XSide<T, TM, A_TR, PAIR> SA;
+    typedef XSide<T, TN, B_TR, false> SB;
+    constexpr int BK = SA::BK, PER = 16 / sizeof(T);            // k of a step, elements of a 16-byte piece
     constexpr int LOADS = (TM + TN) / 8 / NW;                   // LDS-DMA instructions per wavefront and step (1 KiB each)
     static_assert(FN <= FM, "a group of products for each n fragment's read");
-    static_assert(LOADS == 8 && (TM / 8) % LOADS == 0, "a wavefront loads 8 KiB of one operand");
-    constexpr unsigned BUF = (TM + TN) * 128;
+    static_assert((TM / 8) % LOADS == 0, "a wavefront loads one operand");
+    constexpr unsigned BUF = (TM + TN) * XT_ROW;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave / WN, wn = wave % WN;
@@ -324,10 +361,10 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     if ((EPI == XE_STATS || EPI == XE_DLOGITS) && a.pick && xt_big(a.rowsA, count) != (TM == 256)) return;
     const int rowsB = EPI == XE_DW ? a.rowsB : count;
     const int tilesN = (rowsB + TN - 1) / TN, tiles = a.tilesM * tilesN;
-    const int ksteps = EPI == XE_DW ? (count + XT_BK - 1) / XT_BK : (int)((a.K + XT_BK - 1) / XT_BK);
+    const int ksteps = EPI == XE_DW ? (count + BK - 1) / BK : (int)((a.K + BK - 1) / BK);
     const int steps = a.segments * ksteps;
     int splits = 1;
-    if constexpr (EPI == XE_DX || EPI == XE_DW) splits = xt_splits(tiles, a.segments * (EPI == XE_DW ? ksteps : a.split_k / XT_BK), a.max_blocks);
+    if constexpr (EPI == XE_DX || EPI == XE_DW) splits = xt_splits(tiles, a.segments * (EPI == XE_DW ? ksteps : a.split_k / BK), a.max_blocks);
     if ((int)blockIdx.x >= tiles * splits) return;
     const int split = (int)blockIdx.x / tiles;
     int tm, tn;
@@ -339,7 +376,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     const unsigned ld = loads_a ? a.lda : a.ldb;
     const bool tr = loads_a ? A_TR : B_TR;
     const int dma0 = wave * LOADS - (loads_a ? 0 : TM / 8);     // this wavefront's first instruction of its operand
-    const unsigned k_bytes = tr ? XT_BK * ld : XT_BK * 2;
+    const unsigned k_bytes = tr ? BK * ld : XT_ROW;
     const unsigned lds_wave = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)smem + wave * LOADS * 1024);
     // memory rows behind an operand's end repeat its last one: their results are dropped, or the other operand has zeros there
     const int rows = tr ? (EPI == XE_DW ? 0x7fffffff : (int)a.K) : loads_a ? a.rowsA : rowsB;
@@ -348,29 +385,29 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     auto offset = [&](int q, int first, int limit) -> unsigned {
         if (tr) {
             const int per = loads_a ? SA::PIECES : SB::PIECES, row = (dma0 + q) * (64 / per) + lane / per;
-            const int f = loads_a ? XSide<TM, true, false>::f(row) : XSide<TN, true, false>::f(row);
-            const int col = min(at0 + ((lane % per) ^ f) * 8, (loads_a ? a.colsA : (int)(a.ldb / 2)) - 8);
-            return (unsigned)min(row, limit - 1 - first) * ld + (unsigned)col * 2;
+            const int f = XSide<T, TM, true, false>::f(row);
+            const int col = min(at0 + ((lane % per) ^ f) * PER, (loads_a ? a.colsA : (int)(a.ldb / sizeof(T))) - PER);
+            return (unsigned)min(row, limit - 1 - first) * ld + (unsigned)col * (unsigned)sizeof(T);
         }
         const int row = (dma0 + q) * 8 + (lane >> 3);
-        const int f = loads_a ? XSide<TM, false, PAIR>::f(row) : XSide<TN, false, false>::f(row);
+        const int f = loads_a ? XSide<T, TM, false, PAIR>::f(row) : XSide<T, TN, false, false>::f(row);
         return (unsigned)min(row, limit - 1 - first) * ld + ((lane & 7) ^ f) * 16;
     };
     unsigned voff[LOADS];
 #pragma unroll
-    for (int q = 0; q < LOADS; ++q) voff[q] = offset(q, tr ? 0 : at0, tr ? XT_BK : rows);
+    for (int q = 0; q < LOADS; ++q) voff[q] = offset(q, tr ? 0 : at0, tr ? BK : rows);
     // the step that is loaded next
     int seg = __builtin_amdgcn_readfirstlane(s0 / (ksteps > 0 ? ksteps : 1)), kst = __builtin_amdgcn_readfirstlane(s0 - seg * ksteps);
     auto plane = [&]() { return uniform((loads_a ? a.A[seg] : a.B[seg]) + (tr ? 0 : (size_t)at0 * ld) + (size_t)kst * k_bytes); };
     const char *base = n_steps > 0 ? plane() : nullptr;
     auto issue = [&](int buf) {
-        if (A_TR && EPI != XE_DW && tr && (kst + 1) * XT_BK > rows) {           // the last rows of k
+        if (A_TR && EPI != XE_DW && tr && (kst + 1) * BK > rows) {           // the last rows of k
             unsigned last[LOADS];
 #pragma unroll
-            for (int q = 0; q < LOADS; ++q) last[q] = offset(q, kst * XT_BK, rows);
-            xt_dma8(lds_wave + buf * BUF, last, base);
+            for (int q = 0; q < LOADS; ++q) last[q] = offset(q, kst * BK, rows);
+            xt_dma(lds_wave + buf * BUF, last, base);
         } else {
-            xt_dma8(lds_wave + buf * BUF, voff, base);
+            xt_dma(lds_wave + buf * BUF, voff, base);
         }
         base += k_bytes;
         if (++kst == ksteps) {
@@ -386,7 +423,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
         int hit;
         float lse, rel;
     };
-    static_assert(!LOGITS || NW * 64 == TM + TN, "a thread for each row and column of the tile");
+    static_assert(!LOGITS || NW * 64 >= TM + TN, "a thread for each row and column of the tile");
     Row *const row_meta = reinterpret_cast<Row *>(smem + 2 * BUF + WM * TN * sizeof(float2));             // [TN]
     float *const bias_meta = reinterpret_cast<float *>(row_meta + TN);                                    // [TM]
     Row my_row{-1, 0.f, 0.f};
@@ -395,7 +432,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
         if ((int)threadIdx.x < TN) {
             const int n = tn * TN + threadIdx.x;
             if (n < count) my_row = Row{a.target[n] - a.first_v, EPI == XE_DLOGITS ? a.lse[n] : 0.f, EPI == XE_DLOGITS && a.rel ? a.rel[n] : 1.f};
-        } else {
+        } else if ((int)threadIdx.x < TN + TM) {
             const int m = tm * TM + threadIdx.x - TN;
             my_bias = m >= a.rowsA ? -INFINITY : a.bias ? to_f32(static_cast<const TB *>(a.bias)[m]) : 0.f;     // (columns behind the vocabulary: exp 0)
         }
@@ -404,7 +441,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     if (n_steps > 1) issue(1);
     if constexpr (LOGITS) {
         if ((int)threadIdx.x < TN) row_meta[threadIdx.x] = my_row;
-        else bias_meta[threadIdx.x - TN] = my_bias;
+        else if ((int)threadIdx.x < TN + TM) bias_meta[threadIdx.x - TN] = my_bias;
     }
 
     f32x4_t acc[FM][FN];
@@ -418,7 +455,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
         if (load) issue(buf);
 #pragma unroll
         for (int i = 0; i < FM; ++i) {
-            if (i < FN) b1[i] = SB::template read<frag>(tile + TM * 128, nb, i, kk, lane);
+            if (i < FN) b1[i] = SB::template read<frag>(tile + TM * XT_ROW, nb, i, kk, lane);
             a1[i] = SA::template read<frag>(tile, ma, i, kk, lane);
 #pragma unroll
             for (int j = 0; j < FN; ++j) acc[i][j] = Mfma16<T>::mul(a0[i], b0[j], acc[i][j]);
@@ -434,7 +471,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
         xt_wait_all();
         __builtin_amdgcn_s_barrier();
 #pragma unroll
-        for (int j = 0; j < FN; ++j) fb[0][j] = SB::template read<frag>(lds + TM * 128, nb, j, 0, lane);
+        for (int j = 0; j < FN; ++j) fb[0][j] = SB::template read<frag>(lds + TM * XT_ROW, nb, j, 0, lane);
 #pragma unroll
         for (int i = 0; i < FM; ++i) fa[0][i] = SA::template read<frag>(lds, ma, i, 0, lane);
         for (int t = 0; t < n_steps; ++t) {
@@ -487,7 +524,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) sum[j] += WIDE ? expf(acc[i][j][r] - shift) : __expf(acc[i][j][r] - shift);
+                    for (int r = 0; r < 4; ++r) sum[j] += sizeof(TB) == 4 ? expf(acc[i][j][r] - shift) : __expf(acc[i][j][r] - shift);
                 sum[j] += __shfl_xor(sum[j], 16);
                 sum[j] += __shfl_xor(sum[j], 32);
             }
@@ -528,12 +565,12 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
                         const float l = acc[i + e / 4][j][e % 4] + b[e];
-                        const float p = WIDE ? expf(l - row[j].lse) : __expf(l - row[j].lse);
+                        const float p = sizeof(TB) == 4 ? expf(l - row[j].lse) : __expf(l - row[j].lse);
                         const float v = n < count && m0 + e < a.rowsA ? (p - (row[j].hit == m0 + e ? 1.f : 0.f)) * row[j].rel : 0.f;
                         db[e] += v;
                         d[e] = (TB)(v * a.d_scale);
                     }
-                    if (n < n_end && m0 < a.ldd) put_planes<TB, 8>(a.d, (size_t)n * a.ldd + m0, d);
+                    if (n < n_end && m0 < a.ldd) put_planes<WIDE, TB, 8>(a.d, (size_t)n * a.ldd + m0, d);
                 }
                 if (a.db_part)
 #pragma unroll
@@ -606,20 +643,8 @@ struct XFew {
 };
 
 template <typename T>
-struct XFewStep {                  // 16-bit: 8 k of each of 4 lane groups
-    static constexpr int PER = 8, K = 32;
-    typedef typename Mfma16<T>::frag frag;
-    static __device__ __forceinline__ f32x4_t mul(frag a, frag b, f32x4_t c) { return Mfma16<T>::mul(a, b, c); }
-};
-template <>
-struct XFewStep<float> {
-    static constexpr int PER = 4, K = 16;
-    typedef f32x4_t frag;
-    static __device__ __forceinline__ f32x4_t mul(frag a, frag b, f32x4_t c) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], b[q], c, 0, 0, 0);
-        return c;
-    }
+struct XFewStep : Mfma16<T> {
+    static constexpr int PER = 16 / sizeof(T), K = 4 * PER;      // k of a lane group, of an operand
 };
 
 // 16 bytes at an element-aligned address, zeros behind the row's end
@@ -765,7 +790,7 @@ __global__ __launch_bounds__(1024) void xent_few_finish_kernel(XFew a, int parts
 
 // ---- rows -------------------------------------------------------------------------------------------------------------------------------
 // A workgroup joins the parts of 16 rows: 64 lane groups share the parts, then one adds them up.
-__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int V, int N,
+__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int V, int big, int small, int N,
                                                         const int *__restrict__ count, const float *__restrict__ target_logit,
                                                         const int *__restrict__ from, float *__restrict__ lse, float *__restrict__ row_loss,
                                                         float *__restrict__ loss) {
@@ -773,7 +798,7 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int n = blockIdx.x * 16 + c, kept = *count;
     if (blockIdx.x * 16 >= kept) return;
-    const int parts = xt_big(V, kept) ? (V + 255) / 256 : (V + 127) / 128;
+    const int parts = big && xt_big(V, kept) ? (V + 255) / 256 : (V + small - 1) / small;
     float mx = -INFINITY, sum = 0.f;
     if (n < kept)
         for (int p = group; p < parts; p += 64) xt_join(mx, sum, part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
@@ -842,10 +867,10 @@ __global__ __launch_bounds__(1024) void xent_scales_kernel(const float *__restri
 // The splits' partial outputs in order.  dx: rows go back to their places; dW: nothing to do where one split wrote the result.
 template <typename T>
 __global__ __launch_bounds__(256) void xent_sum_slabs_kernel(const float *__restrict__ slabs, const int *__restrict__ count, int rows_static, int tilesM,
-                                                            int TN, int split_steps, int segments, int max_blocks, int D, int pieces,
+                                                            int TN, int split_steps, int bk, int segments, int max_blocks, int D, int pieces,
                                                             const int *__restrict__ row_of, T *__restrict__ out) {
     const int rows = row_of ? *count : rows_static;
-    const int steps = segments * (row_of ? split_steps : (*count + XT_BK - 1) / XT_BK);
+    const int steps = segments * (row_of ? split_steps : (*count + bk - 1) / bk);
     const int n = xt_splits(tilesM * ((rows + TN - 1) / TN), steps, max_blocks);
     if (n == 1 && (!row_of || pieces == 1)) return;
     const size_t total = (size_t)rows * D;
@@ -876,11 +901,11 @@ __global__ __launch_bounds__(256) void xent_sum_slabs_kernel(const float *__rest
 
 // db[v] = top sum over the row tiles' partial sums, in order: 16 columns a workgroup, 16 lane groups share the parts
 template <typename T>
-__global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ part, const int *__restrict__ count, int nv,
+__global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ part, const int *__restrict__ count, int nv, int big, int small,
                                                      const float *__restrict__ top, const float *__restrict__ dloss, int mean, T *__restrict__ db) {
     __shared__ float meet[16][16];
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4, v = blockIdx.x * 16 + c;
-    const int n = xt_big(nv, *count) ? (*count + 255) / 256 * 4 : (*count + 127) / 128 * 2;
+    const int n = big && xt_big(nv, *count) ? (*count + 255) / 256 * 4 : (*count + small - 1) / small * 2;
     float s = 0.f;
     if (v < nv)
         for (int i = group; i < n; i += 16) s += part[(size_t)i * nv + v];
@@ -908,12 +933,18 @@ struct Tile128 {
     static constexpr int WM = 2, WN = 2, FM = 4, FN = 4, SIZE = 128, BLOCKS = 512;
 };
 
+// small problems: four times the workgroups of Tile128 for the logits, which do not split their k loop
+struct Tile64 {
+    static constexpr int WM = 2, WN = 2, FM = 2, FN = 2, SIZE = 64, BLOCKS = 512;
+};
+
 struct XPlan {
-    bool wide;                 // fp32 inputs
-    int planes, segments;
+    bool wide;                 // fp32 inputs in three planes
+    int planes, segments, bytes, bk;       // bytes of an operand's element, k of a step
     long long Kp, Np, piece, pieces;
     bool pack_w;
     bool big_fwd, big_d;       // 256 x 256 tiles, if enough rows count (known on the device alone)
+    int small_fwd, small_d;    // the other tile size
     bool big_dx, big_dw;       // 256 x 256 tiles
     long long wcols;           // readable columns of W's operand rows
 };
@@ -923,27 +954,38 @@ static bool big_split(long long m, long long n) {
     return m > 128 && n > 128 && ceil_div(m, 256) * ceil_div(n, 256) >= 32;
 }
 
+static int small_tile(long long m, long long n) { return ceil_div(m, 128) * ceil_div(n, 128) < 192 ? 64 : 128; }
+
+// Where the planes' cost (20 bytes of traffic for each element of W, over both directions) equals what they save (8 N products at 130 instead
+// of 200 TFLOP/s): N = 205.
+constexpr long long XT_NATIVE = 256;
+
 static XPlan make_plan(const phc_linear_xent_desc *d) {
     XPlan p;
-    p.wide = d->dtype == PHC_DTYPE_F32;
+    // fp32: three planes from XT_NATIVE rows on; below, laying W out costs more than the fp32 matrix instructions lose
+    p.wide = d->dtype == PHC_DTYPE_F32 && d->N > XT_NATIVE;
     p.planes = p.wide ? 3 : 1;
     p.segments = p.wide ? 6 : 1;
-    p.Kp = round_up(d->D, XT_BK);
+    p.bytes = p.wide ? 2 : dtype_bytes(d->dtype);
+    p.bk = XT_ROW / p.bytes;
+    p.Kp = round_up(d->D, p.bk);
     p.Np = round_up(d->N, XT_BK);
     // W is read where it lies when its rows are whole steps and 16-byte aligned
-    p.pack_w = p.wide || d->D % XT_BK || d->ldw % 8 || !aligned_to(d->W, 16);
+    p.pack_w = p.wide || d->D % p.bk || d->ldw * p.bytes % 16 || !aligned_to(d->W, 16);
     p.wcols = p.Kp;
-    long long piece = XT_PIECE_BYTES / (2 * p.planes * (d->N > 0 ? d->N : 1)) / 256 * 256;
+    long long piece = XT_PIECE_BYTES / (p.bytes * p.planes * d->N) / 256 * 256;
     if (piece < 2048) piece = 2048;
     if (d->piece > 0) piece = round_up(d->piece, 64);
     if (piece >= d->V) piece = round_up(d->V, 64);
     p.pieces = ceil_div(d->V, piece);
     p.piece = d->piece > 0 ? piece : round_up(ceil_div(d->V, p.pieces), 64);
     p.pieces = ceil_div(d->V, p.piece);
-    p.big_fwd = xt_big((int)d->V, (int)d->N);
-    p.big_d = xt_big((int)p.piece, (int)d->N);
-    p.big_dx = big_split(d->D, d->N);
-    p.big_dw = big_split(d->D, p.piece);
+    p.big_fwd = p.bytes == 2 && xt_big((int)d->V, (int)d->N);
+    p.big_d = p.bytes == 2 && xt_big((int)p.piece, (int)d->N);
+    p.small_fwd = small_tile(d->V, d->N);
+    p.small_d = small_tile(p.piece, d->N);
+    p.big_dx = p.bytes == 2 && big_split(d->D, d->N);
+    p.big_dw = p.bytes == 2 && big_split(d->D, p.piece);
     return p;
 }
 
@@ -979,12 +1021,12 @@ struct XWs {
     XWs(const phc_linear_xent_desc *d, const XPlan &p, bool backward, void *ws) {
         Carve c(ws);
         auto planes = [&](XPlanes &o, size_t count) {
-            for (int i = 0; i < p.planes; ++i) o.p[i] = c.take<unsigned short>(count);
+            for (int i = 0; i < p.planes; ++i) o.p[i] = c.take<char>(count * p.bytes);
         };
         planes(x, (size_t)p.Np * p.Kp);
         if (p.pack_w) planes(w, (size_t)(backward ? p.piece : d->V) * p.Kp);
         if (!backward) {
-            const size_t parts = ceil_div(d->V, 128);
+            const size_t parts = ceil_div(d->V, p.small_fwd);
             part_max = c.take<float>(parts * d->N);
             part_sum = c.take<float>(parts * d->N);
             target_logit = c.take<float>(d->N);
@@ -995,7 +1037,7 @@ struct XWs {
             planes(dl, (size_t)p.Np * p.piece);
             if (d->dx) dx_slabs = c.take<float>(slab_floats(d->N, d->D, p.big_dx, p.pieces > 1));
             if (d->dW) dw_slabs = c.take<float>(slab_floats(p.piece, d->D, p.big_dw, false));
-            if (d->db) db_part = c.take<float>((size_t)(ceil_div(d->N, 256) * Tile256::WN) * p.piece);          // (4 parts of each 256 rows, either size)
+            if (d->db) db_part = c.take<float>((size_t)(ceil_div(d->N, 64) * 2 + 2) * p.piece);          // (large tiles: 4 parts of 256 rows, small ones 2 of 128 or 64)
         }
         bytes = c.used;
     }
@@ -1006,17 +1048,18 @@ static unsigned flat_grid(long long n) {
     return (unsigned)(b < 1 ? 1 : b > 8192 ? 8192 : b);
 }
 
-template <typename T>
+template <typename T, bool SPLIT>
 static void pack_as(const void *src, long long ld, long long R, long long C, long long Cp, const XRows *rows, void *zero, const XPlanes &out, hipStream_t s) {
-    PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_pack_kernel<T>), dim3(flat_grid((R + (rows ? XT_BK : 0)) * (Cp / 8))), dim3(256), 0, s, static_cast<const T *>(src), ld,
-                  R, (int)C, (int)Cp, rows ? (const int *)rows->to : (const int *)nullptr, rows ? (const int *)rows->count : (const int *)nullptr,
+    PHC_LAUNCH_AS(K_XENT_LAYOUT, (xent_pack_kernel<T, SPLIT>), dim3(flat_grid((R + (rows ? XT_BK : 0)) * (Cp / 8))), dim3(256), 0, s, static_cast<const T *>(src),
+                  ld, R, (int)C, (int)Cp, rows ? (const int *)rows->to : (const int *)nullptr, rows ? (const int *)rows->count : (const int *)nullptr,
                   static_cast<T *>(zero), out);
 }
-static void pack(int dtype, const void *src, long long ld, long long R, long long C, long long Cp, const XRows *rows, void *zero, const XPlanes &out,
+static void pack(const XPlan &p, int dtype, const void *src, long long ld, long long R, long long C, const XRows *rows, void *zero, const XPlanes &out,
                  hipStream_t s) {
-    if (dtype == PHC_DTYPE_F32) pack_as<float>(src, ld, R, C, Cp, rows, zero, out, s);
-    else if (dtype == PHC_DTYPE_BF16) pack_as<bf16_t>(src, ld, R, C, Cp, rows, zero, out, s);
-    else pack_as<f16_t>(src, ld, R, C, Cp, rows, zero, out, s);
+    if (p.wide) pack_as<float, true>(src, ld, R, C, p.Kp, rows, zero, out, s);
+    else if (dtype == PHC_DTYPE_F32) pack_as<float, false>(src, ld, R, C, p.Kp, rows, zero, out, s);
+    else if (dtype == PHC_DTYPE_BF16) pack_as<bf16_t, false>(src, ld, R, C, p.Kp, rows, zero, out, s);
+    else pack_as<f16_t, false>(src, ld, R, C, p.Kp, rows, zero, out, s);
 }
 
 static void set_planes(const XPlan &p, const XPlanes &A, const XPlanes &B, XGemm *g) {
@@ -1030,7 +1073,7 @@ static void set_planes(const XPlan &p, const XPlanes &A, const XPlanes &B, XGemm
 
 template <typename T, int EPI, bool WIDE, typename TILE>
 static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
-    constexpr int LDS = 4 * TILE::SIZE * 128 + TILE::SIZE * (TILE::WM * (int)sizeof(float2) + 12 + 4);      // buffers, the wavefronts' meeting place, rows and columns
+    constexpr int LDS = 4 * TILE::SIZE * XT_ROW + TILE::SIZE * (TILE::WM * (int)sizeof(float2) + 12 + 4);      // buffers, the wavefronts' meeting place, rows and columns
     g.tilesM = (int)ceil_div(g.rowsA, TILE::SIZE);
     g.tilesN = (int)ceil_div(g.rowsB, TILE::SIZE);
     g.max_blocks = TILE::BLOCKS;
@@ -1042,36 +1085,44 @@ static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
     PHC_LAUNCH_AS(kid, kernel, dim3((unsigned)blocks), dim3(TILE::WM * TILE::WN * 64), LDS, s, g);
     return true;
 }
+template <typename T, int EPI, bool WIDE>
+static bool launch_tile(int kid, int tile, XGemm &g, hipStream_t s) {
+    if constexpr (!(sizeof(T) == 4))
+        if (tile == 256) return launch_gemm<T, EPI, WIDE, Tile256>(kid, g, s);
+    if constexpr (EPI == XE_STATS || EPI == XE_DLOGITS)
+        if (tile == 64) return launch_gemm<T, EPI, WIDE, Tile64>(kid, g, s);
+    return launch_gemm<T, EPI, WIDE, Tile128>(kid, g, s);
+}
+// big: 256 x 256 tiles; for the logits only if the rows that count fill the card with them, otherwise tiles of `small`
 template <int EPI>
-static int gemm(const phc_linear_xent_desc *d, int kid, bool big, XGemm &g, hipStream_t s) {
-    bool ok;
+static int gemm(const XPlan &p, int dtype, int kid, bool big, int small, XGemm &g, hipStream_t s) {
     if ((EPI == XE_STATS || EPI == XE_DLOGITS) && big && !g.pick) {
         // Enough rows for large tiles, if they count, which the device alone knows: both sizes are launched, one of them ends at once
         // (4 us; 13 568 rows of which 15 % count against 5000 columns would fill 160 of the 256 CUs with large tiles).
         g.pick = 1;
-        if (int rc = gemm<EPI>(d, kid, false, g, s)) return rc;
+        if (int rc = gemm<EPI>(p, dtype, kid, false, small, g, s)) return rc;
     }
-    if (d->dtype == PHC_DTYPE_F32) ok = big ? launch_gemm<bf16_t, EPI, true, Tile256>(kid, g, s) : launch_gemm<bf16_t, EPI, true, Tile128>(kid, g, s);
-    else if (d->dtype == PHC_DTYPE_BF16) ok = big ? launch_gemm<bf16_t, EPI, false, Tile256>(kid, g, s) : launch_gemm<bf16_t, EPI, false, Tile128>(kid, g, s);
-    else ok = big ? launch_gemm<f16_t, EPI, false, Tile256>(kid, g, s) : launch_gemm<f16_t, EPI, false, Tile128>(kid, g, s);
+    const int tile = big ? 256 : small;
+    const bool ok = p.wide ? launch_tile<bf16_t, EPI, true>(kid, tile, g, s) : dtype == PHC_DTYPE_F32 ? launch_tile<float, EPI, false>(kid, tile, g, s)
+                    : dtype == PHC_DTYPE_BF16 ? launch_tile<bf16_t, EPI, false>(kid, tile, g, s) : launch_tile<f16_t, EPI, false>(kid, tile, g, s);
     PHC_REQUIRE(ok, PHC_ERR_LAUNCH, "phc_linear_xent: the runtime refused the kernel's LDS size");
     return PHC_OK;
 }
 
 template <typename T>
-static void sum_slabs_as(int kid, const float *slabs, const XGemm &g, int tile, int pieces, void *out, hipStream_t s) {
+static void sum_slabs_as(int kid, const float *slabs, const XGemm &g, int tile, int bk, int pieces, void *out, hipStream_t s) {
     PHC_LAUNCH_AS(kid, (xent_sum_slabs_kernel<T>), dim3(flat_grid((long long)g.rowsB * ceil_div(g.ldo, 4))), dim3(256), 0, s, slabs, g.count, g.rowsB, g.tilesM, tile,
-                  g.split_k / XT_BK, g.segments, g.max_blocks, g.ldo, pieces, g.row_of, static_cast<T *>(out));
+                  g.split_k / bk, bk, g.segments, g.max_blocks, g.ldo, pieces, g.row_of, static_cast<T *>(out));
 }
-static void sum_slabs(int dtype, int kid, const float *slabs, const XGemm &g, int tile, int pieces, void *out, hipStream_t s) {
-    if (dtype == PHC_DTYPE_F32) sum_slabs_as<float>(kid, slabs, g, tile, pieces, out, s);
-    else if (dtype == PHC_DTYPE_BF16) sum_slabs_as<bf16_t>(kid, slabs, g, tile, pieces, out, s);
-    else sum_slabs_as<f16_t>(kid, slabs, g, tile, pieces, out, s);
+static void sum_slabs(int dtype, int kid, const float *slabs, const XGemm &g, int tile, int bk, int pieces, void *out, hipStream_t s) {
+    if (dtype == PHC_DTYPE_F32) sum_slabs_as<float>(kid, slabs, g, tile, bk, pieces, out, s);
+    else if (dtype == PHC_DTYPE_BF16) sum_slabs_as<bf16_t>(kid, slabs, g, tile, bk, pieces, out, s);
+    else sum_slabs_as<f16_t>(kid, slabs, g, tile, bk, pieces, out, s);
 }
 
 template <typename T>
-static void db_as(const float *part, const XRows &r, int nv, const float *top, const float *dloss, int mean, void *db, hipStream_t s) {
-    PHC_LAUNCH_AS(K_XENT_DW, (xent_db_kernel<T>), dim3((unsigned)ceil_div(nv, 16)), dim3(256), 0, s, part, (const int *)r.count, nv, top, dloss, mean,
+static void db_as(const float *part, const XRows &r, int nv, int big, int small, const float *top, const float *dloss, int mean, void *db, hipStream_t s) {
+    PHC_LAUNCH_AS(K_XENT_DW, (xent_db_kernel<T>), dim3((unsigned)ceil_div(nv, 16)), dim3(256), 0, s, part, (const int *)r.count, nv, big, small, top, dloss, mean,
                   static_cast<T *>(db));
 }
 
@@ -1140,17 +1191,17 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     const int es = dtype_bytes(d->dtype), N = (int)d->N;
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_that_count_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const long long *>(d->target),
                   (long long)d->ignore_index, N, (long long)d->V, err_word(), st.rows);
-    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &st.rows, nullptr, w.x, s);
+    pack(p, d->dtype, d->x, d->ldx, d->N, d->D, &st.rows, nullptr, w.x, s);
     XPlanes W{{const_cast<void *>(d->W)}};
     if (p.pack_w) {
-        pack(d->dtype, d->W, d->ldw, d->V, d->D, p.Kp, nullptr, nullptr, w.w, s);
+        pack(p, d->dtype, d->W, d->ldw, d->V, d->D, nullptr, nullptr, w.w, s);
         W = w.w;
     }
     XGemm g{};
     set_planes(p, W, w.x, &g);
     g.K = p.Kp;
-    g.lda = (unsigned)(p.pack_w ? p.Kp * 2 : d->ldw * es);
-    g.ldb = (unsigned)(p.Kp * 2);
+    g.lda = (unsigned)(p.pack_w ? p.Kp * p.bytes : d->ldw * es);
+    g.ldb = (unsigned)(p.Kp * p.bytes);
     g.rowsA = (int)d->V;
     g.rowsB = g.N = N;
     g.count = st.rows.count;
@@ -1159,10 +1210,10 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     g.part_max = w.part_max;
     g.part_sum = w.part_sum;
     g.target_logit = w.target_logit;
-    if (int rc = gemm<XE_STATS>(d, K_XENT_LOGITS, p.big_fwd, g, s)) return rc;
+    if (int rc = gemm<XE_STATS>(p, d->dtype, K_XENT_LOGITS, p.big_fwd, p.small_fwd, g, s)) return rc;
     float *loss = d->reduction == PHC_REDUCE_NONE ? d->loss : nullptr;
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_kernel, dim3((unsigned)ceil_div(N, 16)), dim3(1024), 0, s, (const float *)w.part_max, (const float *)w.part_sum,
-                  (int)d->V, N, g.count, (const float *)w.target_logit, (const int *)st.rows.from, st.lse, w.row_loss, loss);
+                  (int)d->V, p.big_fwd ? 1 : 0, p.small_fwd, N, g.count, (const float *)w.target_logit, (const int *)st.rows.from, st.lse, w.row_loss, loss);
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_reduce_kernel, dim3(1), dim3(1024), 0, s, (const float *)w.row_loss, g.count, (const int *)st.rows.to, N,
                   d->reduction == PHC_REDUCE_MEAN ? 1 : 0, loss ? (float *)nullptr : d->loss, loss);
     return launch_status("phc_linear_xent_fwd");
@@ -1184,7 +1235,7 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
     const int mean = d->reduction == PHC_REDUCE_MEAN ? 1 : 0;
     if (per_row)
         PHC_LAUNCH_AS(K_XENT_ROWS, xent_scales_kernel, dim3(1), dim3(1024), 0, s, d->dloss, (const int *)st.rows.count, (const int *)st.rows.from, w.rel, w.top);
-    pack(d->dtype, d->x, d->ldx, d->N, d->D, p.Kp, &st.rows, d->dx, w.x, s);
+    pack(p, d->dtype, d->x, d->ldx, d->N, d->D, &st.rows, d->dx, w.x, s);
     // fp16 has no normal values below 6e-5, where most probabilities of a large vocabulary lie: its d are stored times 2^14
     const float d_scale = d->dtype == PHC_DTYPE_F16 ? 16384.f : 1.f;
     XGemm o{};                                                   // (the last piece's dx product: its splits are joined at the end)
@@ -1193,15 +1244,15 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         const char *Wv = static_cast<const char *>(d->W) + (size_t)v0 * d->ldw * es;
         XPlanes W{{const_cast<char *>(Wv)}};
         if (p.pack_w) {
-            pack(d->dtype, Wv, d->ldw, nv, d->D, p.Kp, nullptr, nullptr, w.w, s);
+            pack(p, d->dtype, Wv, d->ldw, nv, d->D, nullptr, nullptr, w.w, s);
             W = w.w;
         }
-        const unsigned ldw = (unsigned)(p.pack_w ? p.Kp * 2 : d->ldw * es);
+        const unsigned ldw = (unsigned)(p.pack_w ? p.Kp * p.bytes : d->ldw * es);
         XGemm g{};
         set_planes(p, W, w.x, &g);
         g.K = p.Kp;
         g.lda = ldw;
-        g.ldb = (unsigned)(p.Kp * 2);
+        g.ldb = (unsigned)(p.Kp * p.bytes);
         g.rowsA = nv;
         g.rowsB = g.N = N;
         g.count = st.rows.count;
@@ -1214,12 +1265,12 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         g.ldd = nvp;
         g.d_scale = d_scale;
         g.db_part = d->db ? w.db_part : nullptr;
-        if (int rc = gemm<XE_DLOGITS>(d, K_XENT_DLOGITS, p.big_d, g, s)) return rc;
+        if (int rc = gemm<XE_DLOGITS>(p, d->dtype, K_XENT_DLOGITS, p.big_d, p.small_d, g, s)) return rc;
         if (d->db) {
             char *db = static_cast<char *>(d->db) + (size_t)v0 * es;
-            if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, st.rows, nv, top, d->dloss, mean, db, s);
-            else if (d->dtype == PHC_DTYPE_BF16) db_as<bf16_t>(w.db_part, st.rows, nv, top, d->dloss, mean, db, s);
-            else db_as<f16_t>(w.db_part, st.rows, nv, top, d->dloss, mean, db, s);
+            if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, st.rows, nv, p.big_d, p.small_d, top, d->dloss, mean, db, s);
+            else if (d->dtype == PHC_DTYPE_BF16) db_as<bf16_t>(w.db_part, st.rows, nv, p.big_d, p.small_d, top, d->dloss, mean, db, s);
+            else db_as<f16_t>(w.db_part, st.rows, nv, p.big_d, p.small_d, top, d->dloss, mean, db, s);
         }
         if (d->dx) {
             o = XGemm{};
@@ -1227,7 +1278,7 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             o.K = nv;
             o.split_k = (int)p.piece;
             o.lda = ldw;
-            o.ldb = (unsigned)(nvp * 2);
+            o.ldb = (unsigned)(nvp * p.bytes);
             o.rowsA = (int)d->D;
             o.colsA = (int)p.wcols;
             o.rowsB = N;
@@ -1242,13 +1293,13 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             o.slabs = w.dx_slabs;
             o.accumulate = v0 > 0;
             o.pieces = (int)p.pieces;
-            if (int rc = gemm<XE_DX>(d, K_XENT_DX, p.big_dx, o, s)) return rc;
+            if (int rc = gemm<XE_DX>(p, d->dtype, K_XENT_DX, p.big_dx, 128, o, s)) return rc;
         }
         if (d->dW) {
             XGemm q{};
             set_planes(p, w.x, w.dl, &q);
-            q.lda = (unsigned)(p.Kp * 2);
-            q.ldb = (unsigned)(nvp * 2);
+            q.lda = (unsigned)(p.Kp * p.bytes);
+            q.ldb = (unsigned)(nvp * p.bytes);
             q.rowsA = (int)d->D;
             q.colsA = (int)p.Kp;
             q.rowsB = nv;
@@ -1261,12 +1312,12 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             q.ldo = (int)d->D;
             q.slabs = w.dw_slabs;
             q.pieces = 1;
-            if (int rc = gemm<XE_DW>(d, K_XENT_DW, p.big_dw, q, s)) return rc;
+            if (int rc = gemm<XE_DW>(p, d->dtype, K_XENT_DW, p.big_dw, 128, q, s)) return rc;
             if ((long long)q.tilesM * q.tilesN * 2 <= q.max_blocks)
-                sum_slabs(d->dtype, K_XENT_DW, w.dw_slabs, q, p.big_dw ? 256 : 128, 1, q.out, s);
+                sum_slabs(d->dtype, K_XENT_DW, w.dw_slabs, q, p.big_dw ? 256 : 128, p.bk, 1, q.out, s);
         }
     }
-    if (d->dx) sum_slabs(d->dtype, K_XENT_DX, w.dx_slabs, o, p.big_dx ? 256 : 128, (int)p.pieces, d->dx, s);
+    if (d->dx) sum_slabs(d->dtype, K_XENT_DX, w.dx_slabs, o, p.big_dx ? 256 : 128, p.bk, (int)p.pieces, d->dx, s);
     return launch_status("phc_linear_xent_bwd");
 }
 

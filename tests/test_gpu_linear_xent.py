@@ -121,7 +121,7 @@ def test_more_tiles_and_splits(n, v, d, dtype):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("n,v,d", [(40, 66003, 64), (150, 33100, 300), (33100, 150, 300), (2700, 7000, 130)])
+@pytest.mark.parametrize("n,v,d", [(40, 66003, 64), (150, 33100, 300), (256, 50000, 70), (33100, 150, 300), (2700, 7000, 130)])
 def test_more_tiles_than_the_card_holds(n, v, d, dtype):
     """More output tiles than workgroups fit at once, in each of the products (256 of the large tiles, 512 of the small ones).  The formula
     and its bounds on the GPU, in 64 bits."""
