@@ -261,6 +261,7 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
         if o.shape != g.shape or not o.is_contiguous():
             raise L.PhcError(f"clip_grads: result {i} has to be a contiguous tensor of shape {tuple(g.shape)}")
     norm = _norm_clip("clip_grads", gs, max_norm, norm_type, out)[0]
+    torch.autograd.graph.increment_version(out)
     if error_if_nonfinite:
         _finite_or_raise("clip_grads", norm)
     return norm, out
@@ -282,6 +283,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     if error_if_nonfinite:
         _finite_or_raise("clip_grad_norm_", _norm_clip("clip_grad_norm_", dense, 0.0, norm_type, None)[0])
     norm = _norm_clip("clip_grad_norm_", dense, max_norm, norm_type, dense)[0]
+    torch.autograd.graph.increment_version(dense)
     for g, d in zip(grads, dense):
         if d is not g:
             g.copy_(d)

@@ -89,25 +89,29 @@ class _EmbeddingFn(torch.autograd.Function):
                                           raw_stream(dev)), "phc_embedding_fwd")
         L.maybe_check_indices(dev)
         ctx.save_for_backward(tokens)
-        ctx.meta = (V, D, w.dtype, scale, pad)
+        # (autograd runs the backward on a thread of its own, where every Python step costs several times what it does here)
+        ctx.meta = (N, V, D, w.dtype, L.DTYPE_IDS[w.dtype], scale, pad, dev, lib.phc_embedding_bwd_ws_bytes(N, V, D))
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        lib = L.load()
-        (tokens,) = ctx.saved_tensors
-        V, D, dtype, scale, pad = ctx.meta
-        dev = tokens.device
-        N = tokens.numel()
-        dy = _rows(dout.to(dtype).reshape(N, D))
-        dw = torch.empty((V, D), dtype=dtype, device=dev)
-        ws_bytes = lib.phc_embedding_bwd_ws_bytes(N, V, D)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        with on_device(dev):
-            L.check(lib.phc_embedding_bwd(L.ptr(tokens), L.ptr(dy), N, V, D, _row_stride(dy), L.DTYPE_IDS[dtype], scale, pad, L.ptr(dw),
-                                          L.ptr(ws), ws_bytes, raw_stream(dev)), "phc_embedding_bwd")
-        return None, dw, None, None
+        return _embedding_backward_once(ctx, dout) if torch.is_grad_enabled() else _embedding_backward(ctx, dout)
+
+
+def _embedding_backward(ctx, dout):
+    (tokens,) = ctx.saved_tensors
+    N, V, D, dtype, dtype_id, scale, pad, dev, ws_bytes = ctx.meta
+    if dout.dtype != dtype:
+        dout = dout.to(dtype)
+    dy = _rows(dout.reshape(N, D))
+    dw = torch.empty((V, D), dtype=dtype, device=dev)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    L.check(L.load().phc_embedding_bwd(L.ptr(tokens), L.ptr(dy), N, V, D, _row_stride(dy), dtype_id, scale, pad, L.ptr(dw), ws.data_ptr(),
+                                       ws_bytes, raw_stream(dev)), "phc_embedding_bwd")       # (autograd has made dev the current device)
+    return None, dw, None, None
+
+
+_embedding_backward_once = once_differentiable(_embedding_backward)
 
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
@@ -179,28 +183,33 @@ class _LinearCrossEntropyFn(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dloss):
-        lib = L.load()
-        ignore_index, reduction, piece = ctx.meta
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        if len(ctx.saved_tensors) == 3:                          # no rows
-            x, w, b = ctx.saved_tensors
-            return (torch.zeros_like(x) if need_x else None, torch.zeros_like(w) if need_w else None,
-                    torch.zeros_like(b) if need_b else None, None, None, None, None)
-        x, w, b, target, state = ctx.saved_tensors
-        dev = x.device
-        g = dloss.to(torch.float32).contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
-        db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need_b else None
-        d = _xent_desc(x, w, b, target, ignore_index, reduction, state, piece)
-        d.dloss, d.dx, d.dW, d.db = L.ptr(g), L.ptr(dx), L.ptr(dw), L.ptr(db)
-        ws = _xent_workspace(lib, d, 1, dev)
-        with on_device(dev):
-            L.check(lib.phc_linear_xent_bwd(C.byref(d), raw_stream(dev)), "phc_linear_xent_bwd")
-        del ws
-        return dx, dw, db, None, None, None, None
+        return _xent_backward_once(ctx, dloss) if torch.is_grad_enabled() else _xent_backward(ctx, dloss)
+
+
+def _xent_backward(ctx, dloss):
+    lib = L.load()
+    ignore_index, reduction, piece = ctx.meta
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
+    if len(ctx.saved_tensors) == 3:                          # no rows
+        x, w, b = ctx.saved_tensors
+        return (torch.zeros_like(x) if need_x else None, torch.zeros_like(w) if need_w else None,
+                torch.zeros_like(b) if need_b else None, None, None, None, None)
+    x, w, b, target, state = ctx.saved_tensors
+    dev = x.device
+    g = dloss.to(torch.float32).contiguous()
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
+    db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need_b else None
+    d = _xent_desc(x, w, b, target, ignore_index, reduction, state, piece)
+    d.dloss, d.dx, d.dW, d.db = L.ptr(g), L.ptr(dx), L.ptr(dw), L.ptr(db)
+    ws = _xent_workspace(lib, d, 1, dev)
+    L.check(lib.phc_linear_xent_bwd(C.byref(d), raw_stream(dev)), "phc_linear_xent_bwd")       # (autograd has made dev the current device)
+    del ws
+    return dx, dw, db, None, None, None, None
+
+
+_xent_backward_once = once_differentiable(_xent_backward)
 
 
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None,

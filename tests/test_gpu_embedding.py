@@ -52,7 +52,7 @@ def _check(n, v, d, dtype, kind="falling", scale=1.0, pad=None, seed=0):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,v,d", [(0, 7, 8), (1, 1, 1), (1, 5000, 64), (31, 9, 5), (32, 9, 8), (33, 300, 130), (64, 1, 16), (2047, 119, 32),
-                                   (2049, 257, 24), (5000, 70000, 36), (300, 65536, 8), (4100, 1000, 257), (513, 40, 2056)])
+                                   (2049, 257, 24), (5000, 70000, 36), (300, 65536, 8), (100, 300000, 8), (17000, 600001, 4), (4100, 1000, 257), (513, 40, 2056)])
 def test_lookup_and_gradient(n, v, d, dtype):
     _check(n, v, d, dtype, scale=0.75, pad=0 if v > 1 else None)
 
@@ -225,3 +225,18 @@ def test_capture_beside_a_live_eager_graph_is_refused():
     g2.replay()
     torch.cuda.synchronize()
     assert torch.equal(dw[:, 0].cpu(), torch.bincount(t.cpu(), minlength=40).float())
+
+
+def test_second_derivatives_are_refused():
+    from phc_gnn_amd import ops
+    w = torch.randn(10, 4, device=DEV, requires_grad=True)
+    t = torch.tensor([1, 2, 2], device=DEV)
+    dy = torch.ones(3, 4, device=DEV, requires_grad=True)
+    (dw,) = torch.autograd.grad(ops.embedding(t, w), [w], dy, create_graph=True)
+    assert torch.equal(dw.detach().cpu()[:, 0], torch.tensor([0.0, 1, 2, 0, 0, 0, 0, 0, 0, 0]))
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dw.sum().backward()
+    x = torch.randn(3, 4, device=DEV, requires_grad=True)
+    (dx,) = torch.autograd.grad(ops.linear_cross_entropy(x, w.detach(), t), [x], create_graph=True)
+    with pytest.raises(RuntimeError, match="does not require grad"):
+        dx.sum().backward()

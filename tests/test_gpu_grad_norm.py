@@ -197,3 +197,16 @@ def test_graph_replay():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(norm, want_norm) and all(torch.equal(a, b) for a, b in zip(out, want)), k
+
+
+def test_scaled_tensors_count_as_changed():
+    """Autograd has to notice that a tensor it saved was scaled."""
+    from phc_gnn_amd import optim
+    a = torch.ones(5, device=DEV)
+    x = torch.ones(5, device=DEV, requires_grad=True)
+    y = (x * a).sum()
+    p = torch.nn.Parameter(torch.zeros(5, device=DEV))
+    p.grad = a
+    optim.clip_grad_norm_([p], 0.5)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
