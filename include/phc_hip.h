@@ -1221,7 +1221,7 @@ int phc_phm_weight_reg(const float *const *W, float *const *dW, const int32_t *n
 #define PHC_DTYPE_F16 2
 
 /* out[i, :] = scale * weight[tokens[i], :]   (out dense [N, D]; weight rows ldw elements apart).  A token outside [0, V) reads row 0
- * and sets PHC_IDX_ERR_TOKEN.  N <= 2^28, V <= 2^30, D <= 2^20. */
+ * and sets PHC_IDX_ERR_TOKEN.  N <= 2^28, V <= 2^29, D <= 2^20. */
 int phc_embedding_fwd(const int64_t *tokens, const void *weight, int64_t N, int64_t V, int64_t D, int64_t ldw, int dtype, float scale,
                       void *out, void *stream);
 /* dW[v, :] = scale * sum over i with tokens[i] = v of dy[i, :], for every v (dense [V, D], rows without a token zero); row padding_idx

@@ -445,21 +445,39 @@ static int pack_width(int esize, long long D, long long ld, const void *a, const
     return 1;
 }
 
+// threads of one launch (the hardware counts them in 32 bits)
+constexpr long long EB_MAX_THREADS = 1ll << 31;
+
 template <typename T, int W>
 static void launch_fwd(const int64_t *tokens, const void *weight, int64_t N, int64_t V, int64_t ldw, int D, float scale, void *out,
                        hipStream_t s) {
     const int lg = lane_group(D, W);
-    const long long blocks = ((N << lg) + EB_THREADS - 1) / EB_THREADS;
-    PHC_LAUNCH_AS(K_EMBEDDING_FWD, (embedding_fwd_kernel<T, W>), dim3((unsigned)blocks), dim3(EB_THREADS), 0, s, reinterpret_cast<const long long *>(tokens),
-               static_cast<const T *>(weight), (long long)N, (long long)V, (long long)ldw, D, scale, lg, static_cast<T *>(out), err_word());
+    const long long most = EB_MAX_THREADS >> lg;
+    for (long long i = 0; i < N; i += most) {
+        const long long n = N - i < most ? N - i : most;
+        PHC_LAUNCH_AS(K_EMBEDDING_FWD, (embedding_fwd_kernel<T, W>), dim3((unsigned)(((n << lg) + EB_THREADS - 1) / EB_THREADS)), dim3(EB_THREADS), 0, s,
+                      reinterpret_cast<const long long *>(tokens) + i, static_cast<const T *>(weight), n, (long long)V, (long long)ldw, D, scale, lg,
+                      static_cast<T *>(out) + i * D, err_word());
+    }
+}
+
+// Sums: a lane for each W columns of a chunk.
+static int bwd_lanes(int D, int W) {
+    const int lg = lane_group(D, W);
+    return lg < 3 ? 3 : lg;                                       // (8 lanes at least: a group stages 66 words)
+}
+static long long bwd_chunk_blocks(long long N, int D, int W) {
+    const int lg = bwd_lanes(D, W);
+    const long long slabs = (D + (W << lg) - 1) / (W << lg), chunks = (N + EB_CHUNK - 1) / EB_CHUNK;
+    return (((chunks * slabs) << lg) + EB_THREADS - 1) / EB_THREADS;
 }
 
 template <typename T, int W>
 static void launch_bwd(const EmbeddingWs &w, int side, const void *dy, int64_t N, int64_t V, int64_t ldy, int D, float scale, int pad,
                        void *dW, hipStream_t s) {
-    const int lg = lane_group(D, W) < 3 ? 3 : lane_group(D, W);          // (8 lanes at least: a group stages 66 words)
+    const int lg = bwd_lanes(D, W);
     const long long slabs = (D + (W << lg) - 1) / (W << lg), chunks = (N + EB_CHUNK - 1) / EB_CHUNK;
-    const long long cb = (((chunks * slabs) << lg) + EB_THREADS - 1) / EB_THREADS, zb = (V + 63) / 64;
+    const long long cb = bwd_chunk_blocks(N, D, W), zb = (V + 63) / 64;
     PHC_LAUNCH_AS(K_EMBEDDING_BWD, (embedding_bwd_kernel<T, W>), dim3((unsigned)(cb + zb)), dim3(EB_THREADS),
                   (EB_THREADS >> lg) * (2 * EB_CHUNK + 2) * sizeof(int), s, (const int *)w.keys[side],
                (const int *)w.pos[side], static_cast<const T *>(dy), (long long)ldy, (int)N, (int)V, D, scale, pad, lg, (int)cb,
@@ -495,7 +513,7 @@ using namespace phc;
 static int embedding_check(const char *who, int64_t N, int64_t V, int64_t D, int64_t ld, int dtype) {
     PHC_REQUIRE(dtype_bytes(dtype) != 0, PHC_ERR_INVALID_ARG, "%s: unknown dtype %d", who, dtype);
     PHC_REQUIRE(N >= 0 && V >= 1 && D >= 1, PHC_ERR_INVALID_ARG, "%s: N=%lld V=%lld D=%lld", who, (long long)N, (long long)V, (long long)D);
-    PHC_REQUIRE(N <= (1ll << 28) && V <= (1ll << 30) && D <= (1ll << 20), PHC_ERR_UNSUPPORTED, "%s: N=%lld V=%lld D=%lld is beyond 2^28, 2^30, 2^20",
+    PHC_REQUIRE(N <= (1ll << 28) && V <= (1ll << 29) && D <= (1ll << 20), PHC_ERR_UNSUPPORTED, "%s: N=%lld V=%lld D=%lld is beyond 2^28, 2^29, 2^20",
                 who, (long long)N, (long long)V, (long long)D);
     PHC_REQUIRE(ld >= D || N <= 1 || V <= 1, PHC_ERR_INVALID_ARG, "%s: row stride %lld below the row length %lld", who, (long long)ld, (long long)D);
     return PHC_OK;
@@ -515,7 +533,7 @@ int phc_embedding_fwd(const int64_t *tokens, const void *weight, int64_t N, int6
 }
 
 size_t phc_embedding_bwd_ws_bytes(int64_t N, int64_t V, int64_t D) {
-    if (N < 0 || N > (1ll << 28) || V < 1 || V > (1ll << 30) || D < 1 || D > (1ll << 20)) return 0;
+    if (N < 0 || N > (1ll << 28) || V < 1 || V > (1ll << 29) || D < 1 || D > (1ll << 20)) return 0;
     return EmbeddingWs(nullptr, N, (int)D).bytes + 256;
 }
 
@@ -526,6 +544,9 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
     PHC_REQUIRE(ws && aligned_to(ws, 16) && ws_bytes >= phc_embedding_bwd_ws_bytes(N, V, D), PHC_ERR_WORKSPACE,
                 "phc_embedding_bwd: workspace of %zu bytes, %zu needed", ws_bytes, phc_embedding_bwd_ws_bytes(N, V, D));
     hipStream_t s = static_cast<hipStream_t>(stream);
+    const int width = pack_width(dtype_bytes(dtype), D, ldy, dy ? dy : dW, dW);
+    PHC_REQUIRE(bwd_chunk_blocks(N, (int)D, width) <= EB_MAX_THREADS / EB_THREADS - (V + 63) / 64, PHC_ERR_UNSUPPORTED,
+                "phc_embedding_bwd: N=%lld rows of %lld are beyond one launch", (long long)N, (long long)D);
     EmbeddingWs w(ws, N, (int)D);
     const int pad = padding_idx >= 0 && padding_idx < V ? (int)padding_idx : -1;
     int side = 0;
@@ -533,7 +554,6 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
         side = sort_tokens(tokens, (int)N, V, w, s);
         PHC_REQUIRE(side >= 0, PHC_ERR_LAUNCH, "phc_embedding_bwd: the runtime refused the sort's LDS size");
     }
-    const int width = pack_width(dtype_bytes(dtype), D, ldy, dy ? dy : dW, dW);
     EB_DISPATCH(launch_bwd, dtype, width, w, side, dy, N, V, ldy, (int)D, scale, pad, dW, s);
     return launch_status("phc_embedding_bwd");
 }

@@ -277,8 +277,9 @@ __host__ __device__ inline bool xt_big(int m, int n) {
 
 // what the products of d are multiplied by: the largest |g_i| where the rows of d carry g_i / that, else the one g
 __device__ __forceinline__ float xt_scale(const float *top, const float *dloss, int mean, int count) {
+    if (count <= 0) return 0.f;                                 // (a sum over nothing, whatever its factor)
     if (top) return *top;
-    return mean ? (count > 0 ? *dloss / (float)count : 0.f) : *dloss;
+    return mean ? *dloss / (float)count : *dloss;
 }
 
 // Work of a product over `tiles` output tiles: the k loop is split where the tiles alone do not fill the card, never below 4 steps.
@@ -365,10 +366,11 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     const int steps = a.segments * ksteps;
     int splits = 1;
     if constexpr (EPI == XE_DX || EPI == XE_DW) splits = xt_splits(tiles, a.segments * (EPI == XE_DW ? ksteps : a.split_k / BK), a.max_blocks);
-    if ((int)blockIdx.x >= tiles * splits) return;
-    const int split = (int)blockIdx.x / tiles;
+    const int block = (int)(blockIdx.y * gridDim.x + blockIdx.x);
+    if (block >= tiles * splits) return;
+    const int split = block / tiles;
     int tm, tn;
-    xt_tile_of(blockIdx.x - split * tiles, a.tilesM, tilesN, tm, tn);
+    xt_tile_of(block - split * tiles, a.tilesM, tilesN, tm, tn);
     const int s0 = (int)((long long)steps * split / splits), n_steps = (int)((long long)steps * (split + 1) / splits) - s0;
 
     // loader
@@ -1071,6 +1073,8 @@ static void set_planes(const XPlan &p, const XPlanes &A, const XPlanes &B, XGemm
     }
 }
 
+constexpr long long XT_LINE = 1 << 21;         // workgroups in x: a dimension of a launch holds less than 2^32 threads
+
 template <typename T, int EPI, bool WIDE, typename TILE>
 static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
     constexpr int LDS = 4 * TILE::SIZE * XT_ROW + TILE::SIZE * (TILE::WM * (int)sizeof(float2) + 12 + 4);      // buffers, the wavefronts' meeting place, rows and columns
@@ -1082,7 +1086,8 @@ static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
     // a workgroup for each tile; dx, dW: or for each split of them
     long long blocks = (long long)g.tilesM * g.tilesN;
     if ((EPI == XE_DX || EPI == XE_DW) && blocks < TILE::BLOCKS) blocks = TILE::BLOCKS;
-    PHC_LAUNCH_AS(kid, kernel, dim3((unsigned)blocks), dim3(TILE::WM * TILE::WN * 64), LDS, s, g);
+    const long long line = blocks < XT_LINE ? blocks : XT_LINE;
+    PHC_LAUNCH_AS(kid, kernel, dim3((unsigned)line, (unsigned)ceil_div(blocks, line)), dim3(TILE::WM * TILE::WN * 64), LDS, s, g);
     return true;
 }
 template <typename T, int EPI, bool WIDE>

@@ -280,6 +280,9 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     if not grads:
         return torch.zeros(())
     dense = [g if _dense(g) else g.contiguous() for g in grads]
+    for g, d in zip(grads, dense):
+        if d is not g and torch._debug_has_internal_overlap(g) == 1:
+            raise L.PhcError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} cannot be scaled in place")
     if error_if_nonfinite:
         _finite_or_raise("clip_grad_norm_", _norm_clip("clip_grad_norm_", dense, 0.0, norm_type, None)[0])
     norm = _norm_clip("clip_grad_norm_", dense, max_norm, norm_type, dense)[0]

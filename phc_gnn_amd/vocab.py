@@ -66,10 +66,14 @@ def _check_capture(who: str, dev: torch.device, *tensors: Optional[torch.Tensor]
 
 
 def _tag(out: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    """Marks the leaves' gradient nodes behind ``out`` with their stream (the nodes live as long as the graph)."""
+    """Marks the leaves' gradient nodes behind ``out`` with their stream (the nodes live as long as the graph), through the views that
+    the operators make of their arguments."""
     if out.grad_fn is not None:
+        leaf = torch._C._functions.AccumulateGrad
         for fn, _ in out.grad_fn.next_functions:
-            if isinstance(fn, torch._C._functions.AccumulateGrad):
+            if fn is not None and not isinstance(fn, leaf) and len(fn.next_functions) == 1:
+                fn = fn.next_functions[0][0]
+            if isinstance(fn, leaf):
                 fn.metadata.setdefault("phc_stream", raw_stream(dev))
     return out
 

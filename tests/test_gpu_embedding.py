@@ -240,3 +240,19 @@ def test_second_derivatives_are_refused():
     (dx,) = torch.autograd.grad(ops.linear_cross_entropy(x, w.detach(), t), [x], create_graph=True)
     with pytest.raises(RuntimeError, match="does not require grad"):
         dx.sum().backward()
+
+
+def test_more_rows_than_one_launch_takes():
+    """2^25 rows of an odd length need 2^31 threads; the lookup goes on in a second launch.  All sums are of ones and exact: no partial sum
+    passes 2^24."""
+    from phc_gnn_amd import ops
+    n, v, d = (1 << 25) + 37, 9, 33
+    w = torch.randn(v, d, device=DEV, requires_grad=True)
+    t = torch.randint(0, v, (n,), device=DEV)
+    out = ops.embedding(t, w, scale=0.5)
+    for at in (0, (1 << 25) - 100, n - 1000):
+        s = slice(at, at + 1000)
+        assert torch.equal(out[s], 0.5 * w.detach()[t[s]])
+    dy = torch.ones(n, d, device=DEV)
+    (dw,) = torch.autograd.grad(out, [w], dy)
+    assert torch.equal(dw, 0.5 * torch.bincount(t, minlength=v).float()[:, None].expand(v, d))

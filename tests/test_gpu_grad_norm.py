@@ -210,3 +210,24 @@ def test_scaled_tensors_count_as_changed():
     optim.clip_grad_norm_([p], 0.5)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def test_expanded_gradients_are_refused_before_anything_is_scaled():
+    from phc_gnn_amd import optim
+    from phc_gnn_amd.lib import PhcError
+    p = [torch.nn.Parameter(torch.zeros(4, device=DEV)), torch.nn.Parameter(torch.zeros(6, device=DEV))]
+    p[0].grad = torch.full((4,), 3.0, device=DEV)
+    p[1].grad = torch.full((1,), 2.0, device=DEV).expand(6)
+    with pytest.raises(PhcError, match="in place"):
+        optim.clip_grad_norm_(p, 1.0)
+    assert torch.equal(p[0].grad.cpu(), torch.full((4,), 3.0)) and torch.equal(p[1].grad.cpu(), torch.full((6,), 2.0))
+    assert float(optim.grad_norm([q.grad for q in p])) == pytest.approx((4 * 9 + 6 * 4) ** 0.5, rel=2.0 ** -23)
+
+
+def test_inference_mode():
+    from phc_gnn_amd import optim
+    g = [torch.full((5,), 2.0, device=DEV), torch.full((3,), 4.0, device=DEV, dtype=torch.bfloat16)]
+    with torch.inference_mode():
+        norm, out = optim.clip_grads(g, 1.0)
+        again, _ = optim.clip_grads(out, 10.0, out=out)
+    assert float(norm) == pytest.approx(68 ** 0.5, rel=2.0 ** -23) and 0.99 < float(again) < 1.01

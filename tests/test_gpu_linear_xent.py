@@ -418,3 +418,55 @@ def test_embedding_loss_and_clipping_together():
         opt.step()
     from phc_gnn_amd import check_indices
     check_indices(DEV)
+
+
+def test_more_tiles_than_a_line_of_the_launch():
+    """2^21 tiles of 256 x 256 and more: the launch is laid out in two dimensions.  |x . w| <= 8 * 3 * 3 (clipped), accumulated in fp32 over
+    8 terms: an error of at most 8 * 72 * 2^-24 = 3.5e-5 in a logit, in the target's and, weighted, in the logarithm's.  Three more
+    roundings at that size (l - max, max + log, the loss: 3 * 72 * 2^-24 = 1.3e-5) and the sum (below 100 additions to a term, an
+    exponential of 2^-20: 0.7e-5) stay below 2^-15."""
+    from phc_gnn_amd import ops
+    n, v, d = (1 << 19) + 300, (1 << 18) + 77, 8
+    x = torch.randn(n, d, device=DEV).clamp_(-3, 3).bfloat16()
+    w = torch.randn(v, d, device=DEV).clamp_(-3, 3).bfloat16()
+    t = torch.randint(0, v, (n,), device=DEV)
+    loss = ops.linear_cross_entropy(x, w, t, reduction="none")
+    for rows in (torch.arange(0, 40), torch.arange(n // 2, n // 2 + 40), torch.arange(n - 40, n)):
+        rows = rows.to(DEV)
+        logits = x[rows].double() @ w.double().T
+        want = torch.logsumexp(logits, 1) - logits.gather(1, t[rows][:, None])[:, 0]
+        assert float((loss[rows].double() - want).abs().max()) <= 2 * 3.5e-5 + 2.0 ** -15
+
+
+def test_no_row_counts_whatever_the_upstream_gradient():
+    from phc_gnn_amd import ops
+    for n in (3, 100):
+        x = torch.randn(n, 16, device=DEV, requires_grad=True)
+        w = torch.randn(50, 16, device=DEV, requires_grad=True)
+        b = torch.zeros(50, device=DEV, requires_grad=True)
+        t = torch.full((n,), -100, device=DEV)
+        for reduction in ("mean", "sum"):
+            loss = ops.linear_cross_entropy(x, w, t, b, reduction=reduction)
+            for g in torch.autograd.grad(loss, [x, w, b], torch.tensor(float("inf"), device=DEV)):
+                assert float(g.abs().max()) == 0.0
+
+
+def test_capture_beside_a_live_eager_graph_of_x_is_refused():
+    """x is flattened on the way: its gradient node stands behind a view."""
+    from phc_gnn_amd import ops
+    from phc_gnn_amd.lib import PhcError
+    x = torch.randn(2, 70, 8, device=DEV, requires_grad=True)
+    w = torch.randn(40, 8, device=DEV)
+    t = torch.randint(0, 40, (2, 70), device=DEV)
+    alive = ops.linear_cross_entropy(x, w, t)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            with pytest.raises(PhcError, match="captured into a graph"):
+                ops.linear_cross_entropy(x, w, t)
+            out = ops.linear_cross_entropy(x.detach(), w, t)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, alive.detach())
