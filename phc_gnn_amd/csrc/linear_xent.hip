@@ -630,9 +630,11 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 
 // ---- a few rows -------------------------------------------------------------------------------------------------------------------------
 // Up to 64 rows (scoring a few tokens): W is read once and everything else is small, so the launch is W's bytes at the memory's rate and
-// latency.  A workgroup takes 64 columns; its four wavefronts share the k (their loads are all in flight at once) and meet in LDS.  W and x go
-// from memory straight into matrix operands: lane (rho, g) loads 16 bytes of row rho at k = g * 16 bytes, the same for both operands, so any
-// order of k inside a step will do.  fp32 on the fp32 matrix instructions (4 k each): their rate is enough beside W's bytes.
+// latency.  A workgroup takes 64 columns at a time; its four wavefronts share the k and meet in LDS.  W and x go from memory straight into
+// matrix operands: lane (rho, g) loads 16 bytes of row rho at k = g * 16 bytes, the same for both operands, so any order of k inside a step
+// will do.  Two sets of registers: a step is loaded while the one before is multiplied.  fp32 on the fp32 matrix instructions (4 k each).
+// bf16, V = 131072, D = 2048 (537 MB): 1 / 16 / 32 / 64 rows 110 / 119 / 133 / 170 us = 4.9 .. 3.2 TB/s (x comes from L2 for every group, as
+// many bytes as W at 64 rows); fp32: 214 / 231 / 266 / 405 us (at 64 rows half of it matrix instructions).
 struct XFew {
     const void *W, *x, *bias;
     long long ldw, ldx;            // elements
@@ -640,7 +642,7 @@ struct XFew {
     const long long *target;
     long long ignore;
     int *err;
-    float *part_max, *part_sum;    // [64-column group][16 NF]
+    float *part_max, *part_sum;    // [workgroup][16 NF]
     float *target_logit;           // [row]
 };
 
@@ -649,117 +651,195 @@ struct XFewStep : Mfma16<T> {
     static constexpr int PER = 16 / sizeof(T), K = 4 * PER;      // k of a lane group, of an operand
 };
 
-// 16 bytes at an element-aligned address, zeros behind the row's end
-template <typename T, typename frag>
-__device__ __forceinline__ frag few_load(const T *p, int left) {
-    constexpr int PER = 16 / sizeof(T);
-    LoosePack<T, PER> q = {};
-    if (left >= PER) q = *reinterpret_cast<const LoosePack<T, PER> *>(p);
-    else if (left > 0)
+// 16 bytes at an element-aligned address.  ODD: 16-bit rows that may begin at odd elements are loaded as the words that hold them (each of which
+// holds an element of the row) and shifted: accesses that are not word-aligned take several times as long.
+template <typename T, bool ODD, typename frag>
+__device__ __forceinline__ frag few_load(const T *p) {
+    if constexpr (ODD) {
+        const bool odd = reinterpret_cast<uintptr_t>(p) & 2;
+        const unsigned *at = reinterpret_cast<const unsigned *>(reinterpret_cast<uintptr_t>(p) & ~(uintptr_t)2);
+        const LoosePack<unsigned, 4> w = *reinterpret_cast<const LoosePack<unsigned, 4> *>(at);
+        const unsigned last = at[odd ? 4 : 3], shift = odd ? 16 : 0;
+        LoosePack<unsigned, 4> o;
 #pragma unroll
-        for (int e = 0; e < PER; ++e)
-            if (e < left) q.v[e] = p[e];
+        for (int e = 0; e < 4; ++e) o.v[e] = __builtin_amdgcn_alignbit(e < 3 ? w.v[e + 1] : last, w.v[e], shift);
+        return __builtin_bit_cast(frag, o);
+    } else {
+        return __builtin_bit_cast(frag, *reinterpret_cast<const LoosePack<T, 16 / sizeof(T)> *>(p));
+    }
+}
+// the first `left` elements of it, zeros behind
+template <typename T, typename frag>
+__device__ __forceinline__ frag few_load_part(const T *p, int left) {
+    LoosePack<T, 16 / sizeof(T)> q = {};
+#pragma unroll
+    for (int e = 0; e < 16 / (int)sizeof(T); ++e)
+        if (e < left) q.v[e] = p[e];
     return __builtin_bit_cast(frag, q);
 }
 
-template <typename T, int NF>
+template <typename T, int NF, bool ODD>
 __global__ __launch_bounds__(256) void xent_few_kernel(XFew a) {
     typedef XFewStep<T> S;
     typedef typename S::frag frag;
-    constexpr int UNROLL = NF > 2 ? 2 : 4;
-    __shared__ f32x4_t meet[4][4][NF][64];
+    constexpr int AHEAD = NF > 1 ? 1 : 2;                       // steps of a set of registers
+    __shared__ f32x4_t meet[4][4][64];
     __shared__ float2 top[4][NF * 16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
-    const int v0 = blockIdx.x * 64;
+    int v0 = blockIdx.x * 64;
     const T *w[4], *x[NF];
+    auto columns = [&]() {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = static_cast<const T *>(a.W) + (long long)min(v0 + i * 16 + fr, a.V - 1) * a.ldw + fg * S::PER;
+        for (int i = 0; i < 4; ++i) w[i] = static_cast<const T *>(a.W) + (long long)min(v0 + i * 16 + fr, a.V - 1) * a.ldw + fg * S::PER;
+    };
+    columns();
 #pragma unroll
     for (int j = 0; j < NF; ++j) x[j] = static_cast<const T *>(a.x) + (long long)min(j * 16 + fr, a.N - 1) * a.ldx + fg * S::PER;
     f32x4_t acc[4][NF];
+    // a wavefront takes every fourth step; two sets of registers: one is loaded while the other is multiplied
+    const int full = a.D / S::K;
+    auto load = [&](frag (&fw)[AHEAD][4], frag (&fx)[AHEAD][NF], int step) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+        for (int u = 0; u < AHEAD; ++u) {
+            if (step + 4 * u >= full) break;
+            const long long k = (long long)(step + 4 * u) * S::K;
 #pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    for (int k0 = wave * S::K; k0 < a.D; k0 += 4 * UNROLL * S::K) {
-        frag fw[UNROLL][4], fx[UNROLL][NF];
+            for (int i = 0; i < 4; ++i) fw[u][i] = few_load<T, ODD, frag>(w[i] + k);
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u) {
-            const int k = k0 + u * 4 * S::K;
-            const int left = a.D - k - fg * S::PER;              // elements of the rows from this lane's on
-#pragma unroll
-            for (int i = 0; i < 4; ++i) fw[u][i] = few_load<T, frag>(w[i] + k, left);
-#pragma unroll
-            for (int j = 0; j < NF; ++j) fx[u][j] = few_load<T, frag>(x[j] + k, left);
+            for (int j = 0; j < NF; ++j) fx[u][j] = few_load<T, ODD, frag>(x[j] + k);
         }
+    };
+    auto multiply = [&](const frag (&fw)[4], const frag (&fx)[NF]) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < NF; ++j) acc[i][j] = S::mul(fw[i], fx[j], acc[i][j]);
+    };
+    auto multiply_all = [&](const frag (&fw)[AHEAD][4], const frag (&fx)[AHEAD][NF], int step) {
 #pragma unroll
-                for (int j = 0; j < NF; ++j) acc[i][j] = S::mul(fw[u][i], fx[u][j], acc[i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) meet[wave][i][j][lane] = acc[i][j];
-    __syncthreads();
-    // wavefront w: columns v0 + 16 w ..; a lane holds columns 4 fg .. 4 fg + 3 of row fr
+        for (int u = 0; u < AHEAD; ++u)
+            if (step + 4 * u < full) multiply(fw[u], fx[u]);
+    };
+    frag fw0[AHEAD][4], fx0[AHEAD][NF], fw1[AHEAD][4], fx1[AHEAD][NF];
+    int hit[NF];
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
-        f32x4_t l = meet[0][wave][j][lane];
-#pragma unroll
-        for (int q = 1; q < 4; ++q) l += meet[q][wave][j][lane];
-        const int n = j * 16 + fr;
-        const long long t = n < a.N ? a.target[n] : a.ignore;
-        const int hit = t == a.ignore ? -1 : (int)checked_index(t, a.V, blockIdx.x == 0 ? a.err : nullptr, PHC_IDX_ERR_TARGET);
-        float mx = -INFINITY, sum = 0.f;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int v = v0 + wave * 16 + fg * 4 + r;
-            if (v >= a.V) {
-                l[r] = -INFINITY;
-                continue;
-            }
-            if (a.bias) l[r] += to_f32(static_cast<const T *>(a.bias)[v]);
-            mx = fmaxf(mx, l[r]);
-            if (hit == v) a.target_logit[n] = l[r];
-        }
-        mx = fmaxf(mx, __shfl_xor(mx, 16));
-        mx = fmaxf(mx, __shfl_xor(mx, 32));
-        const float shift = mx == -INFINITY ? 0.f : mx;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) sum += sizeof(T) == 4 ? expf(l[r] - shift) : __expf(l[r] - shift);
-        sum += __shfl_xor(sum, 16);
-        sum += __shfl_xor(sum, 32);
-        if (fg == 0) top[wave][n] = make_float2(mx, sum);
+        const long long t = j * 16 + fr < a.N ? a.target[j * 16 + fr] : a.ignore;
+        hit[j] = t == a.ignore ? -1 : (int)checked_index(t, a.V, blockIdx.x == 0 ? a.err : nullptr, PHC_IDX_ERR_TARGET);
     }
-    __syncthreads();
-    if (threadIdx.x < NF * 16) {
-        float m = top[0][threadIdx.x].x, s = top[0][threadIdx.x].y;
+    float row_max = -INFINITY, row_sum = 0.f;                   // of row threadIdx.x, over this workgroup's columns
+    load(fw0, fx0, wave);
+    while (v0 < a.V) {
 #pragma unroll
-        for (int q = 1; q < 4; ++q) xt_join(m, s, top[q][threadIdx.x].x, top[q][threadIdx.x].y);
-        a.part_max[(size_t)blockIdx.x * NF * 16 + threadIdx.x] = m;
-        a.part_sum[(size_t)blockIdx.x * NF * 16 + threadIdx.x] = s;
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < NF; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int step = wave; step < full; step += 8 * AHEAD) {
+            load(fw1, fx1, step + 4 * AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply_all(fw0, fx0, step);
+            load(fw0, fx0, step + 8 * AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply_all(fw1, fx1, step + 4 * AHEAD);
+        }
+        if (full * S::K < a.D && wave == full % 4) {            // the rest of the rows
+            const int left = min(max(a.D - full * S::K - fg * S::PER, 0), S::PER);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fw0[0][i] = few_load_part<T, frag>(w[i] + full * S::K, left);
+#pragma unroll
+            for (int j = 0; j < NF; ++j) fx0[0][j] = few_load_part<T, frag>(x[j] + full * S::K, left);
+            multiply(fw0[0], fx0[0]);
+        }
+        const int first = v0 + wave * 16 + fg * 4;              // this lane's columns of the 64
+        v0 += (int)gridDim.x * 64;
+        if (v0 < a.V) {                                         // the next ones are under way while these end
+            columns();
+            load(fw0, fx0, wave);
+        }
+        // wavefront w: columns 16 w .. of the 64; a lane holds 4 columns of row fr.  16 rows at a time: LDS for all of them would halve the
+        // wavefronts on a CU
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) meet[wave][i][lane] = acc[i][j];
+            __syncthreads();
+            f32x4_t l = meet[0][wave][lane];
+#pragma unroll
+            for (int q = 1; q < 4; ++q) l += meet[q][wave][lane];
+            const int n = j * 16 + fr;
+            float mx = -INFINITY, sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int v = first + r;
+                if (v >= a.V) {
+                    l[r] = -INFINITY;
+                    continue;
+                }
+                if (a.bias) l[r] += to_f32(static_cast<const T *>(a.bias)[v]);
+                mx = fmaxf(mx, l[r]);
+                if (hit[j] == v) a.target_logit[n] = l[r];
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float shift = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum += sizeof(T) == 4 ? expf(l[r] - shift) : __expf(l[r] - shift);
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (fg == 0) top[wave][n] = make_float2(mx, sum);
+        }
+        __syncthreads();
+        if (threadIdx.x < NF * 16) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) xt_join(row_max, row_sum, top[q][threadIdx.x].x, top[q][threadIdx.x].y);
+        }
+    }
+    if (threadIdx.x < NF * 16) {
+        a.part_max[(size_t)blockIdx.x * NF * 16 + threadIdx.x] = row_max;
+        a.part_sum[(size_t)blockIdx.x * NF * 16 + threadIdx.x] = row_sum;
     }
 }
 
-// joins the column groups' parts; losses, their reduction and the state for the backward: one workgroup, rows in the lanes of a wavefront
+// joins the workgroups' parts; losses, their reduction and the state for the backward: one workgroup, rows in the lanes of a wavefront
 __global__ __launch_bounds__(1024) void xent_few_finish_kernel(XFew a, int parts, int cols, int reduction, XRows rows, float *__restrict__ lse,
                                                               float *__restrict__ loss) {
+    // the maximum first, then the sums against it: one exponential for each part.  (The fast one: an error of |x| 2^-24 in exp x, weighted with
+    // exp x, moves the logarithm by less than log(parts) 2^-24.)
     __shared__ float sm[1024], ss[1024];
     const int c = threadIdx.x % cols, group = threadIdx.x / cols, groups = 1024 / cols;
+    constexpr int AHEAD = 8;                                         // parts in flight
     float mx = -INFINITY, sum = 0.f;
-    for (int p = group; p < parts; p += groups) xt_join(mx, sum, a.part_max[(size_t)p * cols + c], a.part_sum[(size_t)p * cols + c]);
+    for (int p = group; p < parts; p += groups * AHEAD) {
+        float m[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) m[q] = p + q * groups < parts ? a.part_max[(size_t)(p + q * groups) * cols + c] : -INFINITY;
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) mx = fmaxf(mx, m[q]);
+    }
     sm[threadIdx.x] = mx;
-    ss[threadIdx.x] = sum;
     for (int half = groups / 2; half >= 1; half /= 2) {              // (groups is a power of two)
         __syncthreads();
-        if (group < half) {
-            xt_join(mx, sum, sm[threadIdx.x + half * cols], ss[threadIdx.x + half * cols]);
-            sm[threadIdx.x] = mx;
-            ss[threadIdx.x] = sum;
+        if (group < half) sm[threadIdx.x] = mx = fmaxf(mx, sm[threadIdx.x + half * cols]);
+    }
+    __syncthreads();
+    mx = sm[c];
+    const float shift = mx == -INFINITY ? 0.f : mx;
+    for (int p = group; p < parts; p += groups * AHEAD) {
+        float m[AHEAD], t[AHEAD];
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {
+            const bool in = p + q * groups < parts;
+            m[q] = in ? a.part_max[(size_t)(p + q * groups) * cols + c] : -INFINITY;
+            t[q] = in ? a.part_sum[(size_t)(p + q * groups) * cols + c] : 0.f;
         }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) sum += t[q] * __expf(m[q] - shift);
+    }
+    ss[threadIdx.x] = sum;
+    for (int half = groups / 2; half >= 1; half /= 2) {
+        __syncthreads();
+        if (group < half) ss[threadIdx.x] = sum += ss[threadIdx.x + half * cols];
     }
     __syncthreads();
     if (threadIdx.x >= 64) return;
@@ -1134,16 +1214,27 @@ static void db_as(const float *part, const XRows &r, int nv, int big, int small,
 constexpr int XT_FEW = 64;
 static bool few_rows(const phc_linear_xent_desc *d) { return d->N <= XT_FEW; }
 
+// Workgroups: two on a CU, each with every 512th group of 64 columns (64 rows, V = 100000, D = 1024, bf16: 512, 768, 1024 and one workgroup for
+// each group took 68, 79, 75 and 81 us; fewer parts to join, and the next group's loads run beside a group's end).
+constexpr long long XT_FEW_BLOCKS = 512;
+static long long few_parts(long long V) { return ceil_div(V, 64) < XT_FEW_BLOCKS ? ceil_div(V, 64) : XT_FEW_BLOCKS; }
+
+template <typename T, bool ODD>
+static void launch_few_as(const XFew &f, hipStream_t s) {
+    const dim3 grid((unsigned)few_parts(f.V));
+    if (f.N <= 16) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 1, ODD>), grid, dim3(256), 0, s, f);
+    else if (f.N <= 32) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 2, ODD>), grid, dim3(256), 0, s, f);
+    else PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 4, ODD>), grid, dim3(256), 0, s, f);
+}
 template <typename T>
 static void launch_few(const XFew &f, hipStream_t s) {
-    const dim3 grid((unsigned)ceil_div(f.V, 64));
-    if (f.N <= 16) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 1>), grid, dim3(256), 0, s, f);
-    else if (f.N <= 32) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 2>), grid, dim3(256), 0, s, f);
-    else PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 4>), grid, dim3(256), 0, s, f);
+    if constexpr (sizeof(T) == 2)
+        if ((f.ldw | f.ldx) & 1 || !aligned_to(f.W, 4) || !aligned_to(f.x, 4)) return launch_few_as<T, true>(f, s);
+    launch_few_as<T, false>(f, s);
 }
 
 static int forward_few(const phc_linear_xent_desc *d, const XState &st, hipStream_t s) {
-    const int cols = d->N <= 16 ? 16 : d->N <= 32 ? 32 : 64, parts = (int)ceil_div(d->V, 64);
+    const int cols = d->N <= 16 ? 16 : d->N <= 32 ? 32 : 64, parts = (int)few_parts(d->V);
     Carve c(d->ws);
     XFew f{d->W, d->x, d->bias, d->ldw, d->ldx, (int)d->N, (int)d->V, (int)d->D, reinterpret_cast<const long long *>(d->target), d->ignore_index, err_word()};
     f.part_max = c.take<float>((size_t)parts * cols);
@@ -1179,7 +1270,7 @@ size_t phc_linear_xent_state_bytes(int64_t N) { return N < 0 || N > (1 << 22) ? 
 
 size_t phc_linear_xent_ws_bytes(const phc_linear_xent_desc *d, int backward) {
     if (xent_check("phc_linear_xent_ws_bytes", d)) return 0;
-    if (!backward && few_rows(d)) return (size_t)ceil_div(d->V, 64) * 64 * 2 * sizeof(float) + 2048;
+    if (!backward && few_rows(d)) return (size_t)few_parts(d->V) * 64 * 2 * sizeof(float) + 2048;
     return XWs(d, make_plan(d), backward != 0, nullptr).bytes + 256;
 }
 

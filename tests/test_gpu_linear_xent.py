@@ -470,3 +470,41 @@ def test_capture_beside_a_live_eager_graph_of_x_is_refused():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, alive.detach())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(1, 33001, 129), (3, 32769, 1), (20, 40007, 67), (50, 35000, 33), (64, 70001, 31), (16, 5000, 255), (64, 3000, 513)])
+def test_few_rows_of_odd_lengths(n, v, d, dtype):
+    """Rows that begin at odd elements, alone and inside wider buffers (the last element of a buffer is the last of a row), and more columns than
+    one round of the workgroups takes."""
+    from phc_gnn_amd import ops
+    x, w, b, t = (q.to(DEV) for q in _case(n, v, d, dtype, seed=11))
+    for bias in (None, b):
+        exact, bound = _formula(x, w, bias, t, "none", torch.ones(n, device=DEV))
+        runs = []
+        for pad in (0, 1, 2):
+            xs = torch.zeros(n * (d + pad), device=DEV, dtype=dtype).view(n, d + pad)[:, pad:].copy_(x)
+            ws = torch.zeros(v * (d + pad), device=DEV, dtype=dtype).view(v, d + pad)[:, pad:].copy_(w)
+            runs.append(ops.linear_cross_entropy(xs, ws, t, bias, reduction="none"))
+        assert all(torch.equal(r, runs[0]) for r in runs)
+        err = (runs[0].double() - exact[0]).abs()
+        assert bool((err <= bound[0]).all()), float((err / bound[0]).max())
+
+
+def test_few_rows_with_groups_of_columns_taken_out():
+    """Whole groups of columns at -inf, at the beginning, for one workgroup's every round, and for all but the last column."""
+    from phc_gnn_amd import ops
+    n, v, d = 30, 70000, 16
+    g = torch.Generator().manual_seed(5)
+    x, w = torch.randn(n, d, generator=g).to(DEV), torch.randn(v, d, generator=g).to(DEV)
+    for kept in (torch.arange(64, v), torch.arange(v)[(torch.arange(v) // 64) % 512 != 3], torch.tensor([v - 1])):
+        b = torch.full((v,), float("-inf"))
+        b[kept] = 0.0
+        b, k = b.to(DEV), kept.to(DEV)
+        t = k[torch.arange(n, device=DEV) * 7 % len(kept)]
+        got = ops.linear_cross_entropy(x, w, t, b, reduction="none")
+        logits = x.double() @ w[k].double().T
+        want = torch.logsumexp(logits, 1) - (x.double() * w[t].double()).sum(1)
+        # 16 products in fp32 (4 steps of 4): 16 * 2^-24 of sum |x w| <= 40 here; 8 roundings at the logits' size in what follows
+        bound = (16 + 8) * 2.0 ** -24 * (2 * (x.abs() @ w[k].abs().T).max().double() + 20)
+        assert float((got.double() - want).abs().max()) <= float(bound)
