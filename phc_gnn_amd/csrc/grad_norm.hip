@@ -7,6 +7,7 @@
 // square overflows for |g| > 1.8e19, and the conversion + fma per element hide behind the loads.  Every workgroup sums a fixed set of
 // chunks into its own partial, partials are added in a fixed order: the result does not depend on timing.
 //
+// 536 M fp32 into other fp32 tensors: 371 us for the norm (5.8 TB/s), 831 for the scaling (5.2 TB/s read and written).
 // Tensors come by kernel argument, GN_MAX_TENSORS per launch: no table in memory that a captured graph would have to keep alive.
 #include <algorithm>
 #include <new>

@@ -3,19 +3,24 @@
 //   l_iv = x_i . w_v + b_v      lse_i = log sum_v exp l_iv      loss_i = lse_i - l_{i, t_i}      (0 where t_i = ignore_index)
 //   d_iv = exp(l_iv - lse_i) - [v = t_i]       dx_i = g_i sum_v d_iv w_v       dw_v = sum_i g_i d_iv x_i       db_v = sum_i g_i d_iv
 //
-// Forward: ONE product whose tiles never leave the registers — every tile leaves the maximum and the sum of exponentials of its part
+// Forward: ONE product whose tiles never leave the registers: every tile leaves the maximum and the sum of exponentials of its part
 // of a row and, where the target lies in it, the target's logit; a small kernel joins the parts.  Backward keeps only lse: the
-// vocabulary is walked in pieces, a piece's logits are computed again, become d in the tile's registers, are written in 16 bits in
-// both orders (N x piece and piece x N) and feed the two gradient products while they lie in the caches.
+// vocabulary is walked in pieces, a piece's logits are computed again, become d in the tile's registers, and are written once,
+// [row][column], 16 bits (three times 16 for fp32), for the two gradient products.  Four products instead of three, and no N x V tensor.
 //
-// All products run through one kernel, C[m, n] = sum_k A[m, k] B[n, k] with k contiguous in both operands, on 16-bit matrix
-// instructions with fp32 accumulators.  The vocabulary (or the output's contiguous dimension) is always the m side: a lane then holds four
-// consecutive m of one n, so row statistics are mostly in-lane and outputs are stored in 16-byte pieces.
+// All products run through one kernel, C[m, n] = sum_k A[m, k] B[n, k], on 16-bit matrix instructions with fp32 accumulators.  An
+// operand lies in memory with k contiguous, or with m (n) contiguous (W in dx; x and d in dW) and is transposed by its LDS reads.  The
+// vocabulary (or the output's contiguous dimension) is always the m side: a lane then holds four consecutive m of one n, so row statistics
+// are mostly in-lane and outputs are stored in 16-byte pieces.
 //
 // fp32 inputs: every value is split into three bf16 terms, a = h + m + l (8 bits each, |a - h - m - l| <= 2^-26 |a|), and the product
 // is the sum of the six term products l h, h l, m m, m h, h m, h h (smallest first; the three left out are below 2^-25 |a b|): the same
 // kernel walks six (plane of A, plane of B) pairs.  Six 16-bit products cost less than one product on the fp32 matrix instructions,
-// whose rate is a sixteenth of the 16-bit one.
+// whose rate is a sixteenth of the 16-bit one; with few rows (XT_NATIVE) it is the other way round.
+//
+// What bounds it: large products run at 1.25 - 1.33 PFLOP/s (8192 x 131072 x 2048 bf16: 3.5 ms forward, 0.86 - 0.96 ms each for d, dx and dW of
+// a piece of 32768 columns), which is the rate of a library product of those sizes and the card's power: on zeros the same launch
+// runs 20 % faster.  4096 x 32000 x 1024 bf16: 0.97 - 1.05 ms for a step.  Smaller ones: the beginning and end of each tile's k loop.
 #include "dtype_io.h"
 
 namespace phc {
@@ -341,6 +346,9 @@ struct XSide {
     }
 };
 
+// One workgroup a tile (or a split of its k).  Loads go straight to LDS two steps ahead; 16-byte LDS reads without bank conflicts; the matrix pipes
+// are busy 0.52 - 0.63 of the cycles.  256 x 256 by 8 wavefronts reads half the operand bytes of 128 x 128 by 4 (14.5 against 17.1 ms for
+// 8192 x 131072 x 2048).  Tried without gain: raised wave priority, all of a step's reads first, workgroups that stay for more tiles.
 template <typename T, int EPI, bool WIDE, int WM, int WN, int FM, int FN>
 __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     typedef typename Mfma16<T>::frag frag;
