@@ -1,4 +1,4 @@
-"""Build libphc_hip.so (gfx950 only) in-tree with hipcc.
+"""Build libphc_hip.so (gfx950 only) in-tree with hipcc, and libphc_torch.so (operators of torch over it) with the host compiler.
 
     python -m phc_gnn_amd.build [--force]
 
@@ -20,6 +20,7 @@ CSRC = os.path.join(PKG_DIR, "csrc")
 INCLUDE = os.path.join(REPO, "include")
 OBJ_DIR = os.path.join(PKG_DIR, "build")
 LIB_PATH = os.path.join(PKG_DIR, "libphc_hip.so")
+TORCH_LIB_PATH = os.path.join(PKG_DIR, "libphc_torch.so")
 ARCH = "gfx950"
 
 SOURCES = ["api.hip", "phm_linear.hip", "gemm_agw.hip", "aggregate.hip", "csr.hip", "encoder.hip", "norm.hip", "softmax_agg.hip", "readout.hip", "optim.hip", "downstream.hip", "head_chain.hip", "mlp_fused.hip",
@@ -38,6 +39,23 @@ def _hipcc() -> str:
         if cand and os.path.exists(cand):
             return cand
     raise RuntimeError("hipcc not found: libphc_hip.so cannot be built")
+
+
+def build_torch_ops(force: bool = False, verbose: bool = True) -> str:
+    """libphc_torch.so: operators of torch with native gradient nodes (host code, linked to torch, not to the engine)."""
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    src = os.path.join(CSRC, "torch_embedding.cpp")
+    if force or _stale(TORCH_LIB_PATH, [src, os.path.join(INCLUDE, "phc_hip.h"), torch.__file__]):
+        rocm = os.path.dirname(os.path.dirname(os.path.realpath(_hipcc())))
+        cmd = ([shutil.which("g++") or _hipcc(), "-shared", "-fPIC", "-O2", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",
+                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}"]
+               + [f"-I{d}" for d in include_paths()] + [f"-I{os.path.join(rocm, 'include')}", src, "-o", TORCH_LIB_PATH]
+               + [f"-L{d}" for d in library_paths()] + ["-ltorch_cpu", "-lc10", "-lc10_hip"])
+        if verbose:
+            print("[phc build]", " ".join(cmd), flush=True)
+        subprocess.run(cmd, check=True)
+    return TORCH_LIB_PATH
 
 
 def _stale(target: str, deps) -> bool:
@@ -94,12 +112,15 @@ def build(force: bool = False, verbose: bool = True, defines=(), lib_path: str =
 
     with ThreadPoolExecutor(max_workers=4) as ex:
         audit_future = ex.submit(audit_hs) if need_audit else None
+        torch_future = ex.submit(build_torch_ops, force, verbose) if lib_path == LIB_PATH else None
         objs = list(ex.map(compile_one, sources))
         if audit_future is not None:
             msg = audit_future.result()
             open(stamp, "w").write(msg + "\n")
             if verbose:
                 print("[phc build] asm audit:", msg, flush=True)
+        if torch_future is not None:
+            torch_future.result()
     if force or _stale(lib_path, objs):
         cmd = [hipcc, "-shared", "-fPIC", f"--offload-arch={ARCH}", "-o", lib_path] + objs
         if verbose:

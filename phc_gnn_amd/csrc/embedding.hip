@@ -385,6 +385,56 @@ __global__ __launch_bounds__(EB_THREADS) void embedding_join_kernel(const int *_
     }
 }
 
+// ---- up to 64 positions -----------------------------------------------------------------------------------------------------------------
+// A wavefront holds all tokens, one a lane: no sort, one launch.  Workgroups [0, sum_blocks): a wavefront for each (position, column slab); the
+// first position of a token adds the token's rows in order.  The others: 64 rows of the table each, zero where no token is.
+template <typename T, int W>
+__global__ __launch_bounds__(EB_THREADS) void embedding_bwd_few_kernel(const long long *__restrict__ tokens, const T *__restrict__ dy, long long ldy, int N,
+                                                                      int V, int D, float scale, int pad, int sum_blocks, T *__restrict__ dW) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int key = lane < N ? (int)safe_index(tokens[lane], V) : -1;
+    if ((int)blockIdx.x >= sum_blocks) {
+        const int row0 = ((int)blockIdx.x - sum_blocks) * 64, rows = min(64, V - row0);
+        unsigned long long used = key >= row0 && key < row0 + 64 && key != pad ? 1ull << (key - row0) : 0;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) used |= __shfl_xor(used, d);
+        for (int r = wave; r < rows; r += EB_THREADS / 64) {
+            if ((used >> r) & 1) continue;
+            T *dst = dW + (size_t)(row0 + r) * D;
+            for (int c = lane * W; c < D; c += 64 * W) store_zeros<T, W>(dst + c);
+        }
+        return;
+    }
+    const int slabs = (D + 64 * W - 1) / (64 * W), unit = (int)blockIdx.x * (EB_THREADS / 64) + wave, i = unit / slabs;
+    if (i >= N) return;
+    const int mine = __shfl(key, i);
+    unsigned long long todo = __ballot(key == mine);
+    const int col = (unit % slabs) * 64 * W + lane * W;
+    if (__builtin_ctzll(todo) != i || mine == pad || col >= D) return;
+    float acc[W] = {};
+    constexpr int AHEAD = 8;                                       // rows in flight
+    while (todo) {
+        Pack<T, W> row[AHEAD];
+        bool in[AHEAD];
+        int at = 0;
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q) {                          // (behind the token's last row: that one again, not used)
+            in[q] = todo != 0;
+            if (in[q]) at = __builtin_ctzll(todo);
+            todo &= todo - 1;
+            row[q] = *reinterpret_cast<const Pack<T, W> *>(dy + at * ldy + col);
+        }
+#pragma unroll
+        for (int q = 0; q < AHEAD; ++q)
+            if (in[q])
+#pragma unroll
+                for (int c = 0; c < W; ++c) acc[c] += to_f32(row[q].v[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < W; ++c) acc[c] *= scale;
+    store_pack<T, W>(dW + (size_t)mine * D + col, acc);
+}
+
 // ---- host ---------------------------------------------------------------------------------------------------------------------------
 constexpr int EB_LDS_SORT = 16384;
 template <int PER>
@@ -493,6 +543,16 @@ static void launch_bwd(const EmbeddingWs &w, int side, const void *dy, int64_t N
                       (int)N, D, scale, pad, lg, (int)chunks, (int)slabs, (const float *)w.partial, static_cast<T *>(dW));
 }
 
+constexpr int EB_FEW = 64;
+
+template <typename T, int W>
+static void launch_bwd_few(const int64_t *tokens, const void *dy, int64_t N, int64_t V, int64_t ldy, int D, float scale, int pad, void *dW, hipStream_t s) {
+    const long long units = N * ((D + 64 * W - 1) / (64 * W)), sb = (units + EB_THREADS / 64 - 1) / (EB_THREADS / 64);
+    PHC_LAUNCH_AS(K_EMBEDDING_BWD, (embedding_bwd_few_kernel<T, W>), dim3((unsigned)(sb + (V + 63) / 64)), dim3(EB_THREADS), 0, s,
+                  reinterpret_cast<const long long *>(tokens), static_cast<const T *>(dy), (long long)ldy, (int)N, (int)V, D, scale, pad, (int)sb,
+                  static_cast<T *>(dW));
+}
+
 }  // namespace phc
 
 using namespace phc;
@@ -553,13 +613,14 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
     const int width = pack_width(dtype_bytes(dtype), D, ldy, dy ? dy : dW, dW);
     PHC_REQUIRE(bwd_chunk_blocks(N, (int)D, width) <= EB_MAX_THREADS / EB_THREADS - (V + 63) / 64, PHC_ERR_UNSUPPORTED,
                 "phc_embedding_bwd: N=%lld rows of %lld are beyond one launch", (long long)N, (long long)D);
-    EmbeddingWs w(ws, N, (int)D);
     const int pad = padding_idx >= 0 && padding_idx < V ? (int)padding_idx : -1;
-    int side = 0;
-    if (N > 0) {
-        side = sort_tokens(tokens, (int)N, V, w, s);
-        PHC_REQUIRE(side >= 0, PHC_ERR_LAUNCH, "phc_embedding_bwd: the runtime refused the sort's LDS size");
+    if (N <= EB_FEW) {
+        EB_DISPATCH(launch_bwd_few, dtype, width, tokens, dy, N, V, ldy, (int)D, scale, pad, dW, s);
+        return launch_status("phc_embedding_bwd");
     }
+    EmbeddingWs w(ws, N, (int)D);
+    const int side = sort_tokens(tokens, (int)N, V, w, s);
+    PHC_REQUIRE(side >= 0, PHC_ERR_LAUNCH, "phc_embedding_bwd: the runtime refused the sort's LDS size");
     EB_DISPATCH(launch_bwd, dtype, width, w, side, dy, N, V, ldy, (int)D, scale, pad, dW, s);
     return launch_status("phc_embedding_bwd");
 }

@@ -7,6 +7,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+import os
 from typing import Optional
 
 import torch
@@ -51,73 +52,42 @@ def raw_stream(dev: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
-def _check_capture(who: str, dev: torch.device, *tensors: Optional[torch.Tensor]) -> None:
+def _check_capture(who: str, *tensors: Optional[torch.Tensor]) -> None:
     """A leaf has ONE gradient node while any graph that ends in it lives, and autograd runs that node on the stream it was made on.  A
     backward captured on another stream would pull that stream into the capture, which ends the process when the capture ends: refused
-    here, before anything is recorded, for graphs these operators made (``_tag``)."""
+    here, before anything is recorded."""
     leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
     if not leaves or not torch.is_grad_enabled() or not torch.cuda.is_current_stream_capturing():
         return
     for t in leaves:
-        node = torch.autograd.graph.get_gradient_edge(t).node
-        if node.metadata.get("phc_stream", raw_stream(dev)) != raw_stream(dev):
+        if _torch_ops().gradient_on_another_stream(t):
             raise L.PhcError(f"{who}: captured into a graph while an eager result of the same parameter, made on another stream, still holds its "
                              "autograd graph; detach or delete that result (or make it on the capture's stream) first")
 
 
-def _tag(out: torch.Tensor, dev: torch.device) -> torch.Tensor:
-    """Marks the leaves' gradient nodes behind ``out`` with their stream (the nodes live as long as the graph), through the views that
-    the operators make of their arguments."""
-    if out.grad_fn is not None:
-        leaf = torch._C._functions.AccumulateGrad
-        for fn, _ in out.grad_fn.next_functions:
-            if fn is not None and not isinstance(fn, leaf) and len(fn.next_functions) == 1:
-                fn = fn.next_functions[0][0]
-            if isinstance(fn, leaf):
-                fn.metadata.setdefault("phc_stream", raw_stream(dev))
-    return out
+_ops = None
+
+
+def _torch_ops():
+    """The operators of torch in ``phc_gnn_amd`` (csrc/torch_embedding.cpp), bound to the loaded engine."""
+    global _ops
+    if _ops is None:
+        path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libphc_torch.so")
+        if not os.path.exists(path):
+            raise L.PhcError(f"{path} not found: the operators of torch are not built (run `python -m phc_gnn_amd.build`)")
+        lib = L.load()
+        try:
+            torch.ops.load_library(path)
+            bind = C.CDLL(path).phc_torch_bind
+        except (OSError, AttributeError) as exc:
+            raise L.PhcError(f"cannot load {path}: {exc}; rebuild it") from exc
+        bind.restype, bind.argtypes = None, [C.c_void_p] * 4
+        bind(*(C.cast(f, C.c_void_p) for f in (lib.phc_embedding_fwd, lib.phc_embedding_bwd, lib.phc_embedding_bwd_ws_bytes, lib.phc_last_error)))
+        _ops = torch.ops.phc_gnn_amd
+    return _ops
 
 
 # ---- embedding ------------------------------------------------------------------------------------------------------------------
-class _EmbeddingFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, tokens, weight, scale: float, pad: int):
-        lib = L.load()
-        dev = weight.device
-        w = _rows(weight)
-        V, D = w.shape
-        N = tokens.numel()
-        out = torch.empty((*tokens.shape, D), dtype=w.dtype, device=dev)
-        with on_device(dev):
-            L.check(lib.phc_embedding_fwd(L.ptr(tokens), L.ptr(w), N, V, D, _row_stride(w), L.DTYPE_IDS[w.dtype], scale, L.ptr(out),
-                                          raw_stream(dev)), "phc_embedding_fwd")
-        L.maybe_check_indices(dev)
-        ctx.save_for_backward(tokens)
-        # (autograd runs the backward on a thread of its own, where every Python step costs several times what it does here)
-        ctx.meta = (N, V, D, w.dtype, L.DTYPE_IDS[w.dtype], scale, pad, dev, lib.phc_embedding_bwd_ws_bytes(N, V, D))
-        return out
-
-    @staticmethod
-    def backward(ctx, dout):
-        return _embedding_backward_once(ctx, dout) if torch.is_grad_enabled() else _embedding_backward(ctx, dout)
-
-
-def _embedding_backward(ctx, dout):
-    (tokens,) = ctx.saved_tensors
-    N, V, D, dtype, dtype_id, scale, pad, dev, ws_bytes = ctx.meta
-    if dout.dtype != dtype:
-        dout = dout.to(dtype)
-    dy = _rows(dout.reshape(N, D))
-    dw = torch.empty((V, D), dtype=dtype, device=dev)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    L.check(L.load().phc_embedding_bwd(L.ptr(tokens), L.ptr(dy), N, V, D, _row_stride(dy), dtype_id, scale, pad, L.ptr(dw), ws.data_ptr(),
-                                       ws_bytes, raw_stream(dev)), "phc_embedding_bwd")       # (autograd has made dev the current device)
-    return None, dw, None, None
-
-
-_embedding_backward_once = once_differentiable(_embedding_backward)
-
-
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * weight[tokens]``: ``weight`` [V, D], ``tokens`` int64 / int32 of any shape -> [*tokens.shape, D] in the weight's type.
 
@@ -128,14 +98,21 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
     _dtype_id("embedding: weight", weight)
     if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
         raise L.PhcError(f"embedding: weight [V, D] expected, got {tuple(weight.shape)}")
-    _check_capture("embedding", dev, weight)
+    _check_capture("embedding", weight)
     V = weight.shape[0]
     pad = -1
     if padding_idx is not None:
         if not -V <= padding_idx < V:
             raise L.PhcError(f"embedding: padding_idx {padding_idx} outside the {V} rows")
         pad = int(padding_idx) % V
-    return _tag(_EmbeddingFn.apply(_int64("embedding: tokens", tokens), weight, float(scale), pad), dev)
+    try:
+        out = (_ops or _torch_ops()).embedding.default(_int64("embedding: tokens", tokens), weight, float(scale), pad)
+    except RuntimeError as exc:
+        if str(exc).startswith("phc_embedding_fwd"):
+            raise L.PhcError(str(exc).splitlines()[0]) from None
+        raise
+    L.maybe_check_indices(dev)
+    return out
 
 
 # ---- softmax cross entropy of a linear map ----------------------------------------------------------------------------------------
@@ -242,8 +219,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
         raise L.PhcError(f"linear_cross_entropy: unknown reduction '{reduction}' (known: {sorted(_REDUCTIONS)})")
     if piece < 0:
         raise L.PhcError(f"linear_cross_entropy: piece {piece}")
-    _check_capture("linear_cross_entropy", dev, x, weight, bias)
+    _check_capture("linear_cross_entropy", x, weight, bias)
     t = _int64("linear_cross_entropy: target", target).reshape(-1)
     loss = _LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, bias, t, int(ignore_index), _REDUCTIONS[reduction], int(piece))
-    _tag(loss, dev)
     return loss.reshape(target.shape) if reduction == "none" else loss

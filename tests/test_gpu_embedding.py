@@ -256,3 +256,61 @@ def test_more_rows_than_one_launch_takes():
     dy = torch.ones(n, d, device=DEV)
     (dw,) = torch.autograd.grad(out, [w], dy)
     assert torch.equal(dw, 0.5 * torch.bincount(t, minlength=v).float()[:, None].expand(v, d))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [1, 2, 9, 63, 64, 65])
+def test_few_positions(n, dtype):
+    """Up to 64 positions are not sorted: every token's first position adds its rows, in order.  One token for all, two in turn, all
+    different ones, the padding row among them, out-of-range ones; several column slabs and an odd length."""
+    from phc_gnn_amd import check_indices, ops
+    g = torch.Generator().manual_seed(n)
+    for v, d in ((130, 1032), (65, 129), (64, 4)):
+        w = torch.randn(v, d, generator=g).to(dtype).to(DEV).requires_grad_()
+        dy = torch.randn(n, d, generator=g).to(dtype).to(DEV)
+        for t in (torch.full((n,), v - 1), torch.arange(n) % 2, torch.randperm(v, generator=g).repeat(2)[:n], torch.full((n,), 5)):
+            (dw,) = torch.autograd.grad(ops.embedding(t.to(DEV), w, scale=0.5, padding_idx=5), [w], dy)
+            want = torch.zeros(v, d, dtype=torch.float64).index_add_(0, t, dy.cpu().double()) * 0.5
+            mag = torch.zeros(v, d, dtype=torch.float64).index_add_(0, t, dy.cpu().double().abs()) * 0.5
+            want[5], mag[5] = 0, 0
+            # n roundings of 2^-24 of the sum of magnitudes, and the rounding to the type
+            bound = mag * n * 2.0 ** -24 + want.abs() * (torch.finfo(dtype).eps / 2) * (1 + 2.0 ** -10) + 2.0 ** -24 * (dtype == torch.float16)
+            assert bool(((dw.cpu().double() - want).abs() <= bound).all())
+    t = torch.randint(0, 30, (n,), generator=g)
+    t[0] = 64
+    w = torch.randn(64, 8, device=DEV, requires_grad=True)
+    (dw,) = torch.autograd.grad(ops.embedding(t.to(DEV), w), [w], torch.ones(n, 8, device=DEV))
+    with pytest.raises(IndexError):
+        check_indices()
+    t[0] = 0
+    assert torch.equal(dw.cpu()[:, 0], torch.bincount(t, minlength=64).float())
+
+
+def test_capture_beside_a_live_graph_of_other_operators_is_refused():
+    """The eager graph may be anybody's; one made on the capture's own stream is no obstacle."""
+    from phc_gnn_amd import ops
+    from phc_gnn_amd.lib import PhcError
+    w = torch.randn(40, 8, device=DEV, requires_grad=True)
+    t = torch.randint(0, 40, (30,), device=DEV)
+    alive = w * 2.0
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = ops.embedding(t, w.detach())
+            with pytest.raises(PhcError, match="captured into a graph"):
+                ops.embedding(t, w)
+            with pytest.raises(PhcError, match="captured into a graph"):
+                ops.linear_cross_entropy(torch.ones(2, 8, device=DEV), w, t[:2])
+    del alive
+    with torch.cuda.stream(s):
+        here = ops.embedding(t, w)                              # its node is this stream's
+        g2 = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g2, stream=s):
+            (dw,) = torch.autograd.grad(ops.embedding(t, w), [w], torch.ones(30, 8, device=DEV))
+    g.replay()
+    g2.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, here.detach())
+    assert torch.equal(dw[:, 0].cpu(), torch.bincount(t.cpu(), minlength=40).float())

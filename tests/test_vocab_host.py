@@ -152,28 +152,6 @@ def test_shape_checks_of_the_python_layer(monkeypatch):
             ops.embedding(*args, **kw)
 
 
-def test_gradient_nodes_are_marked_through_views(monkeypatch):
-    """linear_cross_entropy flattens x: the gradient node of a leaf x stands behind that view and has to carry its stream all the same."""
-    from phc_gnn_amd import vocab
-    monkeypatch.setattr(vocab, "raw_stream", lambda dev: 7)
-
-    class F(torch.autograd.Function):
-        @staticmethod
-        def forward(ctx, x, w):
-            return x.sum() + w.sum()
-
-        @staticmethod
-        def backward(ctx, g):
-            return None, None
-    for shape in ((3, 4), (2, 3, 4)):
-        x, w = torch.randn(shape, requires_grad=True), torch.randn(5, 4, requires_grad=True)
-        out = vocab._tag(F.apply(x.reshape(-1, 4), w), torch.device("cpu"))
-        for leaf in (x, w):
-            assert torch.autograd.graph.get_gradient_edge(leaf).node.metadata.get("phc_stream") == 7
-        del out
-        assert "phc_stream" not in torch.autograd.graph.get_gradient_edge(x).node.metadata      # (gone with the graph)
-
-
 def test_sizes_beyond_one_launch_are_refused():
     """The hardware counts a launch's threads in 32 bits: sizes that would need more are refused before anything is launched."""
     lib, h = _lib()
