@@ -45,7 +45,7 @@ def build_torch_ops(force: bool = False, verbose: bool = True) -> str:
     """libphc_torch.so: operators of torch with native gradient nodes (host code, linked to torch, not to the engine)."""
     import torch
     from torch.utils.cpp_extension import include_paths, library_paths
-    src = os.path.join(CSRC, "torch_embedding.cpp")
+    src = os.path.join(CSRC, "torch_vocab.cpp")
     if force or _stale(TORCH_LIB_PATH, [src, os.path.join(INCLUDE, "phc_hip.h"), torch.__file__]):
         rocm = os.path.dirname(os.path.dirname(os.path.realpath(_hipcc())))
         cmd = ([shutil.which("g++") or _hipcc(), "-shared", "-fPIC", "-O2", "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-DUSE_ROCM",

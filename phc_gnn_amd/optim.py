@@ -9,13 +9,12 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from array import array
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import lib as L
-from .vocab import on_device, raw_stream
+from .vocab import torch_ops
 
 
 # clip + Adam as ONE launch whose workgroups exchange the sums of squares inside it (csrc/optim.hip, round 6); 0 = the two launches
@@ -184,48 +183,36 @@ def _dense(t: torch.Tensor) -> bool:
     return t.is_contiguous() or torch._prims_common.is_non_overlapping_and_dense(t)
 
 
-def _one_device(who: str, tensors: Sequence[torch.Tensor]) -> torch.device:
-    dev = L.require_device(tensors[0])
-    index = dev.index
-    for t in tensors:
-        if t.get_device() != index or not t.is_cuda:
-            L.require_device(tensors[0], t)                       # (raises)
-    return dev
+_NORM, _IN_PLACE, _INTO = 0, 1, 2
 
 
-def _dtype_array(who: str, tensors: Sequence[torch.Tensor]) -> array:
-    ids = L.DTYPE_IDS
-    try:
-        return array("i", [ids[t.dtype] for t in tensors])
-    except KeyError as exc:
-        raise L.PhcError(f"{who}: float32, bfloat16 or float16 expected, got {exc.args[0]}") from None
-
-
-def _norm_clip(who: str, grads: Sequence[torch.Tensor], max_norm: float, norm_type: float, out: Optional[Sequence[torch.Tensor]]):
-    """{norm, coefficient} of ``grads`` as a device tensor; the scaled gradients in ``out``."""
-    lib = L.load()
+def _norm_clip(who: str, grads: List[torch.Tensor], mode: int, max_norm: float, norm_type: float, out: Sequence[torch.Tensor] = ()):
+    """{norm, coefficient, ..} of ``grads`` as a device tensor, the scaled gradients written; None where a layout stands in the way."""
     kind = _NORM_KINDS.get(float(norm_type))
     if kind is None:
         raise L.PhcError(f"{who}: norm_type {norm_type} (known: 1, 2, inf)")
     if not max_norm >= 0.0:
         raise L.PhcError(f"{who}: max_norm {max_norm}")
-    dev = _one_device(who, grads) if out is None or out is grads else _one_device(who, (*grads, *out))
-    n = len(grads)
-    dtypes = _dtype_array(who, grads)
-    numel, src = array("q", [g.numel() for g in grads]), array("Q", [g.data_ptr() for g in grads])
-    if out is None:
-        dst = out_dtypes = None
-    elif out is grads:
-        dst, out_dtypes = src, dtypes
-    else:
-        dst, out_dtypes = array("Q", [o.data_ptr() for o in out]), _dtype_array(who, out)
-    host = lambda a: None if a is None else a.buffer_info()[0]
-    ws_bytes = lib.phc_grad_norm_ws_bytes(n, host(numel))
-    res = torch.empty(2 + ws_bytes // 4, dtype=torch.float32, device=dev)          # {norm, coefficient} | workspace
-    at = res.data_ptr()
-    with on_device(dev):
-        L.check(lib.phc_grad_norm_clip(n, host(src), host(numel), host(dtypes), kind, float(max_norm), host(dst), host(out_dtypes), at, at + 8,
-                                       ws_bytes, raw_stream(dev)), who)
+    try:
+        return torch_ops().norm_clip.default(grads, out, mode, float(max_norm), kind)
+    except RuntimeError as exc:
+        text = str(exc)
+        if text.startswith("phc_layout"):
+            return None
+        if text.startswith("phc_"):
+            raise L.PhcError(f"{who}: " + text.splitlines()[0]) from None
+        raise
+
+
+def _clip_or_raise(who: str, grads: List[torch.Tensor], mode: int, max_norm: float, norm_type: float, out: Sequence[torch.Tensor] = ()):
+    """As ``_norm_clip`` for tensors in layouts the kernels take: what still stands in the way is named."""
+    res = _norm_clip(who, grads, mode, max_norm, norm_type, out)
+    if res is None:
+        L.require_device(*grads, *out)
+        for t in (*grads, *out):
+            if t.dtype not in L.DTYPE_IDS:
+                raise L.PhcError(f"{who}: float32, bfloat16 or float16 expected, got {t.dtype}")
+        raise L.PhcError(f"{who}: dense tensors expected")
     return res
 
 
@@ -237,10 +224,13 @@ def _finite_or_raise(who: str, norm: torch.Tensor) -> None:
 @torch.no_grad()
 def grad_norm(tensors: Iterable[torch.Tensor], norm_type: float = 2.0) -> torch.Tensor:
     """The norm (2, 1 or inf) over all ``tensors`` together (fp32 / bf16 / fp16, mixed) as an fp32 device scalar; 0 for none."""
-    ts = [t if _dense(t) else t.contiguous() for t in tensors]
+    ts = list(tensors)
     if not ts:
         return torch.zeros(())
-    return _norm_clip("grad_norm", ts, 0.0, norm_type, None)[0]
+    res = _norm_clip("grad_norm", ts, _NORM, 0.0, norm_type)
+    if res is None:
+        res = _clip_or_raise("grad_norm", [t if _dense(t) else t.contiguous() for t in ts], _NORM, 0.0, norm_type)
+    return res[0]
 
 
 @torch.no_grad()
@@ -249,22 +239,21 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
     """``(norm, results)``: the norm over ``grads`` together, and ``grads`` times ``min(1, max_norm / (norm + 1e-6))`` in new tensors or in
     ``out`` (same shapes, contiguous, fp32 / bf16 / fp16 — e.g. an optimizer's fp32 copies of 16-bit gradients).  ``out`` may be ``grads``
     themselves; results must share memory neither with each other nor with another gradient."""
-    gs = [g.contiguous() for g in grads]
-    if out is None:
-        out = [torch.empty_like(g) for g in gs]
-    out = list(out)
+    gs = list(grads)
+    out = [torch.empty_like(g, memory_format=torch.contiguous_format) for g in gs] if out is None else list(out)
     if len(out) != len(gs):
         raise L.PhcError(f"clip_grads: {len(gs)} gradients, {len(out)} results")
     if not gs:
         return torch.zeros(()), out
-    for i, (g, o) in enumerate(zip(gs, out)):
-        if o.shape != g.shape or not o.is_contiguous():
-            raise L.PhcError(f"clip_grads: result {i} has to be a contiguous tensor of shape {tuple(g.shape)}")
-    norm = _norm_clip("clip_grads", gs, max_norm, norm_type, out)[0]
-    torch.autograd.graph.increment_version(out)
+    res = _norm_clip("clip_grads", gs, _INTO, max_norm, norm_type, out)
+    if res is None:
+        for i, (g, o) in enumerate(zip(gs, out)):
+            if o.shape != g.shape or not o.is_contiguous():
+                raise L.PhcError(f"clip_grads: result {i} has to be a contiguous tensor of shape {tuple(g.shape)}")
+        res = _clip_or_raise("clip_grads", [g.contiguous() for g in gs], _INTO, max_norm, norm_type, out)
     if error_if_nonfinite:
-        _finite_or_raise("clip_grads", norm)
-    return norm, out
+        _finite_or_raise("clip_grads", res[0])
+    return res[0], out
 
 
 @torch.no_grad()
@@ -276,18 +265,19 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     device; two of them may not share memory."""
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
-    grads = [p.grad for p in parameters if p.grad is not None]
+    grads = [g for p in parameters if (g := p.grad) is not None]
     if not grads:
         return torch.zeros(())
-    dense = [g if _dense(g) else g.contiguous() for g in grads]
-    for g, d in zip(grads, dense):
-        if d is not g and torch._debug_has_internal_overlap(g) == 1:
-            raise L.PhcError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} cannot be scaled in place")
     if error_if_nonfinite:
-        _finite_or_raise("clip_grad_norm_", _norm_clip("clip_grad_norm_", dense, 0.0, norm_type, None)[0])
-    norm = _norm_clip("clip_grad_norm_", dense, max_norm, norm_type, dense)[0]
-    torch.autograd.graph.increment_version(dense)
-    for g, d in zip(grads, dense):
-        if d is not g:
-            g.copy_(d)
-    return norm
+        _finite_or_raise("clip_grad_norm_", grad_norm(grads, norm_type))
+    res = _norm_clip("clip_grad_norm_", grads, _IN_PLACE, max_norm, norm_type)
+    if res is None:
+        dense = [g if _dense(g) else g.contiguous() for g in grads]
+        for g, d in zip(grads, dense):
+            if d is not g and torch._debug_has_internal_overlap(g) == 1:
+                raise L.PhcError(f"clip_grad_norm_: a gradient of shape {tuple(g.shape)} and strides {g.stride()} cannot be scaled in place")
+        res = _clip_or_raise("clip_grad_norm_", dense, _IN_PLACE, max_norm, norm_type)
+        for g, d in zip(grads, dense):
+            if d is not g:
+                g.copy_(d)
+    return res[0]

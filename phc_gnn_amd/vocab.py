@@ -5,22 +5,15 @@ Unlike the message-passing operators they take fp32, bf16 and fp16 tensors.  Sum
 every case; gradients come in the type of their input, rounded once.  There is no CPU path."""
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 import os
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import lib as L
 
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-
-
-def on_device(dev: torch.device):
-    """Launches go to the tensors' device, whatever device is current."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
 
 
 def _dtype_id(what: str, t: torch.Tensor) -> int:
@@ -30,26 +23,10 @@ def _dtype_id(what: str, t: torch.Tensor) -> int:
         raise L.PhcError(f"{what}: float32, bfloat16 or float16 expected, got {t.dtype}") from None
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A 2-D tensor the kernels can read in place: unit column stride, rows that do not overlap; anything else is copied."""
-    if t.stride(1) == 1 and (t.stride(0) >= t.shape[1] or t.shape[0] == 1):
-        return t
-    return t.contiguous()
-
-
-def _row_stride(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1])
-
-
 def _int64(what: str, t: torch.Tensor) -> torch.Tensor:
     if t.dtype not in (torch.int64, torch.int32):
         raise L.PhcError(f"{what}: int64 or int32 expected, got {t.dtype}")
     return t.to(torch.int64).contiguous()
-
-
-def raw_stream(dev: torch.device) -> int:
-    """The current stream of ``dev`` as a hipStream_t (``lib.stream_ptr`` without the Python stream object)."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def _check_capture(who: str, *tensors: Optional[torch.Tensor]) -> None:
@@ -60,16 +37,19 @@ def _check_capture(who: str, *tensors: Optional[torch.Tensor]) -> None:
     if not leaves or not torch.is_grad_enabled() or not torch.cuda.is_current_stream_capturing():
         return
     for t in leaves:
-        if _torch_ops().gradient_on_another_stream(t):
+        if torch_ops().gradient_on_another_stream(t):
             raise L.PhcError(f"{who}: captured into a graph while an eager result of the same parameter, made on another stream, still holds its "
                              "autograd graph; detach or delete that result (or make it on the capture's stream) first")
 
 
+# the order of phc_torch_bind
+_BOUND = ("phc_embedding_fwd", "phc_embedding_bwd", "phc_embedding_bwd_ws_bytes", "phc_linear_xent_fwd", "phc_linear_xent_bwd",
+          "phc_linear_xent_state_bytes", "phc_linear_xent_ws_bytes", "phc_grad_norm_ws_bytes", "phc_grad_norm_clip", "phc_last_error")
 _ops = None
 
 
-def _torch_ops():
-    """The operators of torch in ``phc_gnn_amd`` (csrc/torch_embedding.cpp), bound to the loaded engine."""
+def torch_ops():
+    """The operators of torch in ``phc_gnn_amd`` (csrc/torch_vocab.cpp), bound to the loaded engine."""
     global _ops
     if _ops is None:
         path = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libphc_torch.so")
@@ -81,10 +61,21 @@ def _torch_ops():
             bind = C.CDLL(path).phc_torch_bind
         except (OSError, AttributeError) as exc:
             raise L.PhcError(f"cannot load {path}: {exc}; rebuild it") from exc
-        bind.restype, bind.argtypes = None, [C.c_void_p] * 4
-        bind(*(C.cast(f, C.c_void_p) for f in (lib.phc_embedding_fwd, lib.phc_embedding_bwd, lib.phc_embedding_bwd_ws_bytes, lib.phc_last_error)))
+        bind.restype, bind.argtypes = None, [C.c_void_p * len(_BOUND)]
+        bind((C.c_void_p * len(_BOUND))(*(C.cast(getattr(lib, f), C.c_void_p) for f in _BOUND)))
         _ops = torch.ops.phc_gnn_amd
     return _ops
+
+
+def _call(name: str, dev: torch.device, *args) -> torch.Tensor:
+    try:
+        out = getattr(_ops or torch_ops(), name).default(*args)
+    except RuntimeError as exc:
+        if str(exc).startswith("phc_"):                            # (the engine's refusal; out of memory and the like stay what they are)
+            raise L.PhcError(str(exc).splitlines()[0]) from None
+        raise
+    L.maybe_check_indices(dev)
+    return out
 
 
 # ---- embedding ------------------------------------------------------------------------------------------------------------------
@@ -105,94 +96,10 @@ def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, pa
         if not -V <= padding_idx < V:
             raise L.PhcError(f"embedding: padding_idx {padding_idx} outside the {V} rows")
         pad = int(padding_idx) % V
-    try:
-        out = (_ops or _torch_ops()).embedding.default(_int64("embedding: tokens", tokens), weight, float(scale), pad)
-    except RuntimeError as exc:
-        if str(exc).startswith("phc_embedding_fwd"):
-            raise L.PhcError(str(exc).splitlines()[0]) from None
-        raise
-    L.maybe_check_indices(dev)
-    return out
+    return _call("embedding", dev, _int64("embedding: tokens", tokens), weight, float(scale), pad)
 
 
 # ---- softmax cross entropy of a linear map ----------------------------------------------------------------------------------------
-def _xent_desc(x, w, bias, target, ignore_index, reduction, state, piece):
-    d = L.LinearXentDesc()
-    d.N, d.D = x.shape
-    d.V = w.shape[0]
-    d.ldx, d.ldw = _row_stride(x), _row_stride(w)
-    d.ignore_index, d.piece = ignore_index, piece
-    d.dtype, d.reduction = L.DTYPE_IDS[x.dtype], reduction
-    d.x, d.W, d.bias, d.target = L.ptr(x), L.ptr(w), L.ptr(bias), L.ptr(target)
-    d.state = L.ptr(state)
-    return d
-
-
-def _xent_workspace(lib, d, backward: int, dev) -> torch.Tensor:
-    n = lib.phc_linear_xent_ws_bytes(C.byref(d), backward)
-    if n == 0:
-        raise L.PhcError(f"linear_cross_entropy: {lib.phc_last_error().decode()}")
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
-    d.ws, d.ws_bytes = ws.data_ptr(), n
-    return ws
-
-
-class _LinearCrossEntropyFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, target, ignore_index: int, reduction: int, piece: int):
-        lib = L.load()
-        dev = x.device
-        N = x.shape[0]
-        ctx.meta = (ignore_index, reduction, piece)
-        if N == 0:
-            ctx.save_for_backward(x, weight, bias)
-            if reduction == 0:
-                return torch.zeros(0, dtype=torch.float32, device=dev)
-            return torch.full((), float("nan") if reduction == 2 else 0.0, dtype=torch.float32, device=dev)
-        x_, w_ = _rows(x), _rows(weight)
-        b_ = None if bias is None else bias.contiguous()
-        loss = torch.empty((N,) if reduction == 0 else (), dtype=torch.float32, device=dev)
-        state = torch.empty(lib.phc_linear_xent_state_bytes(N), dtype=torch.uint8, device=dev)
-        d = _xent_desc(x_, w_, b_, target, ignore_index, reduction, state, piece)
-        d.loss = L.ptr(loss)
-        ws = _xent_workspace(lib, d, 0, dev)
-        with on_device(dev):
-            L.check(lib.phc_linear_xent_fwd(C.byref(d), raw_stream(dev)), "phc_linear_xent_fwd")
-        del ws
-        L.maybe_check_indices(dev)
-        ctx.save_for_backward(x_, w_, b_, target, state)
-        return loss
-
-    @staticmethod
-    def backward(ctx, dloss):
-        return _xent_backward_once(ctx, dloss) if torch.is_grad_enabled() else _xent_backward(ctx, dloss)
-
-
-def _xent_backward(ctx, dloss):
-    lib = L.load()
-    ignore_index, reduction, piece = ctx.meta
-    need_x, need_w, need_b = ctx.needs_input_grad[:3]
-    if len(ctx.saved_tensors) == 3:                          # no rows
-        x, w, b = ctx.saved_tensors
-        return (torch.zeros_like(x) if need_x else None, torch.zeros_like(w) if need_w else None,
-                torch.zeros_like(b) if need_b else None, None, None, None, None)
-    x, w, b, target, state = ctx.saved_tensors
-    dev = x.device
-    g = dloss.to(torch.float32).contiguous()
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-    dw = torch.empty(w.shape, dtype=w.dtype, device=dev) if need_w else None
-    db = torch.empty(b.shape, dtype=b.dtype, device=dev) if need_b else None
-    d = _xent_desc(x, w, b, target, ignore_index, reduction, state, piece)
-    d.dloss, d.dx, d.dW, d.db = L.ptr(g), L.ptr(dx), L.ptr(dw), L.ptr(db)
-    ws = _xent_workspace(lib, d, 1, dev)
-    L.check(lib.phc_linear_xent_bwd(C.byref(d), raw_stream(dev)), "phc_linear_xent_bwd")       # (autograd has made dev the current device)
-    del ws
-    return dx, dw, db, None, None, None, None
-
-
-_xent_backward_once = once_differentiable(_xent_backward)
-
-
 def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Tensor, bias: Optional[torch.Tensor] = None,
                          ignore_index: int = -100, reduction: str = "mean", piece: int = 0) -> torch.Tensor:
     """Softmax cross entropy of the logits ``x @ weight.T + bias`` against ``target``, without the logits in memory.
@@ -220,6 +127,5 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     if piece < 0:
         raise L.PhcError(f"linear_cross_entropy: piece {piece}")
     _check_capture("linear_cross_entropy", x, weight, bias)
-    t = _int64("linear_cross_entropy: target", target).reshape(-1)
-    loss = _LinearCrossEntropyFn.apply(x.reshape(-1, x.shape[-1]), weight, bias, t, int(ignore_index), _REDUCTIONS[reduction], int(piece))
-    return loss.reshape(target.shape) if reduction == "none" else loss
+    return _call("linear_cross_entropy", dev, x, weight, bias, _int64("linear_cross_entropy: target", target), int(ignore_index),
+                 _REDUCTIONS[reduction], int(piece))

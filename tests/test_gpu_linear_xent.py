@@ -508,3 +508,34 @@ def test_few_rows_with_groups_of_columns_taken_out():
         # 16 products in fp32 (4 steps of 4): 16 * 2^-24 of sum |x w| <= 40 here; 8 roundings at the logits' size in what follows
         bound = (16 + 8) * 2.0 ** -24 * (2 * (x.abs() @ w[k].abs().T).max().double() + 20)
         assert float((got.double() - want).abs().max()) <= float(bound)
+
+
+def test_refusals_of_the_engine_are_phc_errors():
+    from phc_gnn_amd import ops
+    from phc_gnn_amd.lib import PhcError
+    w = torch.zeros(1, (1 << 20) + 1, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    t = torch.zeros(1, device=DEV, dtype=torch.int64)
+    with pytest.raises(PhcError, match="beyond"):
+        ops.embedding(t, w)
+    with pytest.raises(PhcError, match="beyond"):
+        ops.linear_cross_entropy(w.detach(), w, t)
+
+
+def test_leaves_of_any_shape_get_gradients_of_theirs():
+    from phc_gnn_amd import ops
+    x = torch.randn(2, 3, 16, device=DEV, requires_grad=True)
+    w = torch.randn(40, 16, device=DEV, requires_grad=True)
+    b = torch.zeros(40, device=DEV, requires_grad=True)
+    t = torch.randint(0, 40, (2, 3), device=DEV)
+    ops.linear_cross_entropy(x, w, t, b).backward()
+    assert x.grad.shape == x.shape and w.grad.shape == w.shape and b.grad.shape == b.shape
+    flat = x.detach().reshape(6, 16).requires_grad_()
+    got = torch.autograd.grad(ops.linear_cross_entropy(flat, w, t.reshape(-1), b), [flat, w, b])
+    assert torch.equal(got[0].reshape(2, 3, 16), x.grad) and torch.equal(got[1], w.grad) and torch.equal(got[2], b.grad)
+    v = torch.randn(16, device=DEV, requires_grad=True)                       # one row, no batch dimension; no bias
+    (dv,) = torch.autograd.grad(ops.linear_cross_entropy(v, w, t[0, 0]), [v])
+    assert dv.shape == v.shape
+    p = torch.softmax(v.detach().double() @ w.detach().double().T, 0)
+    p[t[0, 0]] -= 1
+    # 16 products and 40 terms in fp32: below 100 roundings of 2^-24 at the size of |p| |w| sums (at most 2 * 5)
+    assert float((dv.double() - p @ w.detach().double()).abs().max()) <= 100 * 2.0 ** -24 * 10
