@@ -158,6 +158,8 @@ __global__ __launch_bounds__(256) void xent_pack_kernel(const TIN *__restrict__ 
 
 // ---- the product ----------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void xt_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+template <int LOADS>
+__device__ __forceinline__ void xt_wait_but() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LOADS) : "memory"); }      // (loads return in order)
 __device__ __forceinline__ void xt_wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 // Eight (four) LDS-DMA instructions: every lane's 16 bytes at base + voff[q] land at LDS byte address lds + 1024 q + 16 lane.  In asm because hipcc
@@ -251,7 +253,7 @@ struct XGemm {
     int tilesM, tilesN, max_blocks;
     int split_k;                   // k that the number of splits goes by
     const int *count;              // packed rows
-    int pick;                      // launched with both tile sizes: the one that fits the rows that count does the work
+    int big, small;                // the logits' tile sizes to choose from (xt_tile); launched with each, one does the work
     // XE_STATS / XE_DLOGITS
     const void *bias;              // fp32 or the operand's type, of this piece; may be null
     const int *target;             // [packed rows]
@@ -278,6 +280,13 @@ struct XGemm {
 // 256 x 256 tiles need half the operand bytes of 128 x 128 ones per product, and fill the card only with enough of them.
 __host__ __device__ inline bool xt_big(int m, int n) {
     return m > 128 && n > 128 && ((m + 255) / 256) * ((n + 255) / 256) >= 192;
+}
+
+// The tile size of the logits, by the rows that count, which the device alone knows.  small = 0 (fp32 on its own matrix instructions, which bound
+// it): 64 where the last 128 rows would be at most half full (33 rows x 13565 x 1728: 116 -> 41 us), else 128.
+__host__ __device__ inline int xt_tile(int big, int small, int m, int count) {
+    if (big && xt_big(m, count)) return 256;
+    return small ? small : ((count + 63) / 64) % 2 ? 64 : 128;
 }
 
 // what the products of d are multiplied by: the largest |g_i| where the rows of d carry g_i / that, else the one g
@@ -349,7 +358,7 @@ struct XSide {
 // One workgroup a tile (or a split of its k).  Loads go straight to LDS two steps ahead; 16-byte LDS reads without bank conflicts; the matrix pipes
 // are busy 0.52 - 0.63 of the cycles.  256 x 256 by 8 wavefronts reads half the operand bytes of 128 x 128 by 4 (14.5 against 17.1 ms for
 // 8192 x 131072 x 2048).  Tried without gain: raised wave priority, all of a step's reads first, workgroups that stay for more tiles.
-template <typename T, int EPI, bool WIDE, int WM, int WN, int FM, int FN>
+template <typename T, int EPI, bool WIDE, int WM, int WN, int FM, int FN, int NB>
 __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     typedef typename Mfma16<T>::frag frag;
     constexpr int NW = WM * WN, TM = WM * FM * 16, TN = WN * FN * 16;
@@ -367,7 +376,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 
     // what there is to do goes by the rows that count
     const int count = *a.count;
-    if ((EPI == XE_STATS || EPI == XE_DLOGITS) && a.pick && xt_big(a.rowsA, count) != (TM == 256)) return;
+    if ((EPI == XE_STATS || EPI == XE_DLOGITS) && xt_tile(a.big, a.small, a.rowsA, count) != TM) return;
     const int rowsB = EPI == XE_DW ? a.rowsB : count;
     const int tilesN = (rowsB + TN - 1) / TN, tiles = a.tilesM * tilesN;
     const int ksteps = EPI == XE_DW ? (count + BK - 1) / BK : (int)((a.K + BK - 1) / BK);
@@ -434,7 +443,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
         float lse, rel;
     };
     static_assert(!LOGITS || NW * 64 >= TM + TN, "a thread for each row and column of the tile");
-    Row *const row_meta = reinterpret_cast<Row *>(smem + 2 * BUF + WM * TN * sizeof(float2));             // [TN]
+    Row *const row_meta = reinterpret_cast<Row *>(smem + NB * BUF + WM * TN * sizeof(float2));             // [TN]
     float *const bias_meta = reinterpret_cast<float *>(row_meta + TN);                                    // [TM]
     Row my_row{-1, 0.f, 0.f};
     float my_bias = 0.f;
@@ -447,8 +456,9 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
             my_bias = m >= a.rowsA ? -INFINITY : a.bias ? to_f32(static_cast<const TB *>(a.bias)[m]) : 0.f;     // (columns behind the vocabulary: exp 0)
         }
     }
-    if (n_steps > 0) issue(0);
-    if (n_steps > 1) issue(1);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+        if (n_steps > b) issue(b);
     if constexpr (LOGITS) {
         if ((int)threadIdx.x < TN) row_meta[threadIdx.x] = my_row;
         else if ((int)threadIdx.x < TN + TM) bias_meta[threadIdx.x - TN] = my_bias;
@@ -473,27 +483,33 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
         }
     };
 
-    // Two LDS buffers, two halves of a step.  While the products of one half run, the fragments of the next are read; the one barrier of a
-    // step stands between them: behind it the next step's buffer is complete, and this step's buffer, read to its end, is loaded anew.
+    // NB LDS buffers, two halves of a step.  While the products of one half run, the fragments of the next are read; the one barrier of a
+    // step stands between them: behind it the next step's buffer is complete, and this step's buffer, read to its end, is loaded anew with the
+    // step NB further on.
     lds_char *lds = (lds_char *)smem;
     if (n_steps > 0) {
         frag fa[2][FM], fb[2][FN];
-        xt_wait_all();
+        if (NB > 2 && n_steps >= NB) xt_wait_but<(NB - 1) * LOADS>();
+        else xt_wait_all();
         __builtin_amdgcn_s_barrier();
 #pragma unroll
         for (int j = 0; j < FN; ++j) fb[0][j] = SB::template read<frag>(lds + TM * XT_ROW, nb, j, 0, lane);
 #pragma unroll
         for (int i = 0; i < FM; ++i) fa[0][i] = SA::template read<frag>(lds, ma, i, 0, lane);
+        int slot = 0;
         for (int t = 0; t < n_steps; ++t) {
-            lds_char *cur = lds + (t & 1) * BUF, *nxt = lds + ((t & 1) ^ 1) * BUF;
+            const int next = NB == 2 ? slot ^ 1 : slot + 1 == NB ? 0 : slot + 1;
+            lds_char *cur = lds + slot * BUF, *nxt = lds + next * BUF;
             half(cur, 1, fa[0], fb[0], fa[1], fb[1], false);
             __builtin_amdgcn_sched_barrier(0);
-            xt_wait_all();
+            if (NB > 2 && t + NB <= n_steps) xt_wait_but<(NB - 2) * LOADS>();       // step t + 1; the NB - 2 behind it may still be under way
+            else xt_wait_all();
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
             // (behind the last step the fragments are read once more and not used)
-            half(nxt, 0, fa[1], fb[1], fa[0], fb[0], t + 2 < n_steps, t & 1);
+            half(nxt, 0, fa[1], fb[1], fa[0], fb[0], t + NB < n_steps, slot);
             __builtin_amdgcn_sched_barrier(0);
+            slot = next;
         }
     }
 
@@ -539,7 +555,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
                 sum[j] += __shfl_xor(sum[j], 32);
             }
             // the wavefronts along m, through LDS behind the buffers (a barrier that orders LDS alone)
-            float2 *meet = reinterpret_cast<float2 *>(smem + 2 * BUF);      // [WM][TN]
+            float2 *meet = reinterpret_cast<float2 *>(smem + NB * BUF);      // [WM][TN]
             if (fg == 0)
 #pragma unroll
                 for (int j = 0; j < FN; ++j) meet[wm * TN + nb + j * 16 + fr] = make_float2(mx[j], sum[j]);
@@ -888,7 +904,7 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int n = blockIdx.x * 16 + c, kept = *count;
     if (blockIdx.x * 16 >= kept) return;
-    const int parts = big && xt_big(V, kept) ? (V + 255) / 256 : (V + small - 1) / small;
+    const int tile = xt_tile(big, small, V, kept), parts = (V + tile - 1) / tile;
     float mx = -INFINITY, sum = 0.f;
     if (n < kept)
         for (int p = group; p < parts; p += 64) xt_join(mx, sum, part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
@@ -995,7 +1011,7 @@ __global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ 
                                                      const float *__restrict__ top, const float *__restrict__ dloss, int mean, T *__restrict__ db) {
     __shared__ float meet[16][16];
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4, v = blockIdx.x * 16 + c;
-    const int n = big && xt_big(nv, *count) ? (*count + 255) / 256 * 4 : (*count + small - 1) / small * 2;
+    const int tile = xt_tile(big, small, nv, *count), n = (*count + tile - 1) / tile * (tile == 256 ? 4 : 2);
     float s = 0.f;
     if (v < nv)
         for (int i = group; i < n; i += 16) s += part[(size_t)i * nv + v];
@@ -1017,15 +1033,17 @@ constexpr long long XT_PIECE_BYTES = 512ll << 20;
 
 // Tiles of 256 x 256 by 8 wavefronts (one workgroup on a CU) or 128 x 128 by 4 (two)
 struct Tile256 {
-    static constexpr int WM = 2, WN = 4, FM = 8, FN = 4, SIZE = 256, BLOCKS = 256;
+    static constexpr int WM = 2, WN = 4, FM = 8, FN = 4, SIZE = 256, BLOCKS = 256, NB = 2;
 };
 struct Tile128 {
-    static constexpr int WM = 2, WN = 2, FM = 4, FN = 4, SIZE = 128, BLOCKS = 512;
+    static constexpr int WM = 2, WN = 2, FM = 4, FN = 4, SIZE = 128, BLOCKS = 512, NB = 2;
 };
 
-// small problems: four times the workgroups of Tile128 for the logits, which do not split their k loop
+// Small problems: four times the workgroups of Tile128 for the logits, which do not split their k loop.  A step is short beside a load's way: three
+// buffers (213 x 3320 x 3989 fp16 forward 55 -> 44 us, 100 x 8000 x 2048 bf16 30 -> 25 us), of which three workgroups fit a CU (four buffers:
+// 200 x 10000 x 1024 bf16 25 -> 29 us).
 struct Tile64 {
-    static constexpr int WM = 2, WN = 2, FM = 2, FN = 2, SIZE = 64, BLOCKS = 512;
+    static constexpr int WM = 2, WN = 2, FM = 2, FN = 2, SIZE = 64, BLOCKS = 512, NB = 3;
 };
 
 struct XPlan {
@@ -1034,7 +1052,7 @@ struct XPlan {
     long long Kp, Np, piece, pieces;
     bool pack_w;
     bool big_fwd, big_d;       // 256 x 256 tiles, if enough rows count (known on the device alone)
-    int small_fwd, small_d;    // the other tile size
+    int small_fwd, small_d;    // the other tile size, 0: 64 or 128, as xt_tile says
     bool big_dx, big_dw;       // 256 x 256 tiles
     long long wcols;           // readable columns of W's operand rows
 };
@@ -1044,7 +1062,7 @@ static bool big_split(long long m, long long n) {
     return m > 128 && n > 128 && ceil_div(m, 256) * ceil_div(n, 256) >= 32;
 }
 
-static int small_tile(long long m, long long n) { return ceil_div(m, 128) * ceil_div(n, 128) < 192 ? 64 : 128; }
+static int small_tile(long long m, long long n, bool native) { return ceil_div(m, 128) * ceil_div(n, 128) < 192 ? 64 : native ? 0 : 128; }
 
 // Where the planes' cost (20 bytes of traffic for each element of W, over both directions) equals what they save (8 N products at 130 instead
 // of 200 TFLOP/s): N = 205.
@@ -1072,8 +1090,8 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     p.pieces = ceil_div(d->V, p.piece);
     p.big_fwd = p.bytes == 2 && xt_big((int)d->V, (int)d->N);
     p.big_d = p.bytes == 2 && xt_big((int)p.piece, (int)d->N);
-    p.small_fwd = small_tile(d->V, d->N);
-    p.small_d = small_tile(p.piece, d->N);
+    p.small_fwd = small_tile(d->V, d->N, p.bytes == 4);
+    p.small_d = small_tile(p.piece, d->N, p.bytes == 4);
     p.big_dx = p.bytes == 2 && big_split(d->D, d->N);
     p.big_dw = p.bytes == 2 && big_split(d->D, p.piece);
     return p;
@@ -1116,7 +1134,7 @@ struct XWs {
         planes(x, (size_t)p.Np * p.Kp);
         if (p.pack_w) planes(w, (size_t)(backward ? p.piece : d->V) * p.Kp);
         if (!backward) {
-            const size_t parts = ceil_div(d->V, p.small_fwd);
+            const size_t parts = ceil_div(d->V, p.small_fwd ? p.small_fwd : 64);
             part_max = c.take<float>(parts * d->N);
             part_sum = c.take<float>(parts * d->N);
             target_logit = c.take<float>(d->N);
@@ -1165,11 +1183,11 @@ constexpr long long XT_LINE = 1 << 21;         // workgroups in x: a dimension o
 
 template <typename T, int EPI, bool WIDE, typename TILE>
 static bool launch_gemm(int kid, XGemm &g, hipStream_t s) {
-    constexpr int LDS = 4 * TILE::SIZE * XT_ROW + TILE::SIZE * (TILE::WM * (int)sizeof(float2) + 12 + 4);      // buffers, the wavefronts' meeting place, rows and columns
+    constexpr int LDS = TILE::NB * 2 * TILE::SIZE * XT_ROW + TILE::SIZE * (TILE::WM * (int)sizeof(float2) + 12 + 4);      // buffers, the wavefronts' meeting place, rows and columns
     g.tilesM = (int)ceil_div(g.rowsA, TILE::SIZE);
     g.tilesN = (int)ceil_div(g.rowsB, TILE::SIZE);
     g.max_blocks = TILE::BLOCKS;
-    auto kernel = xent_gemm_kernel<T, EPI, WIDE, TILE::WM, TILE::WN, TILE::FM, TILE::FN>;
+    auto kernel = xent_gemm_kernel<T, EPI, WIDE, TILE::WM, TILE::WN, TILE::FM, TILE::FN, TILE::NB>;
     if (!ensure_dynamic_lds(kernel, LDS)) return false;
     // a workgroup for each tile; dx, dW: or for each split of them
     long long blocks = (long long)g.tilesM * g.tilesN;
@@ -1186,20 +1204,24 @@ static bool launch_tile(int kid, int tile, XGemm &g, hipStream_t s) {
         if (tile == 64) return launch_gemm<T, EPI, WIDE, Tile64>(kid, g, s);
     return launch_gemm<T, EPI, WIDE, Tile128>(kid, g, s);
 }
-// big: 256 x 256 tiles; for the logits only if the rows that count fill the card with them, otherwise tiles of `small`
 template <int EPI>
-static int gemm(const XPlan &p, int dtype, int kid, bool big, int small, XGemm &g, hipStream_t s) {
-    if ((EPI == XE_STATS || EPI == XE_DLOGITS) && big && !g.pick) {
-        // Enough rows for large tiles, if they count, which the device alone knows: both sizes are launched, one of them ends at once
-        // (4 us; 13 568 rows of which 15 % count against 5000 columns would fill 160 of the 256 CUs with large tiles).
-        g.pick = 1;
-        if (int rc = gemm<EPI>(p, dtype, kid, false, small, g, s)) return rc;
-    }
-    const int tile = big ? 256 : small;
+static int gemm(const XPlan &p, int dtype, int kid, int tile, XGemm &g, hipStream_t s) {
     const bool ok = p.wide ? launch_tile<bf16_t, EPI, true>(kid, tile, g, s) : dtype == PHC_DTYPE_F32 ? launch_tile<float, EPI, false>(kid, tile, g, s)
                     : dtype == PHC_DTYPE_BF16 ? launch_tile<bf16_t, EPI, false>(kid, tile, g, s) : launch_tile<f16_t, EPI, false>(kid, tile, g, s);
     PHC_REQUIRE(ok, PHC_ERR_LAUNCH, "phc_linear_xent: the runtime refused the kernel's LDS size");
     return PHC_OK;
+}
+// The logits, launched with every tile size that the rows that count may ask for: all but one launch end at once (4 us each; 13 568 rows of which
+// 15 % count against 5000 columns would fill 160 of the 256 CUs with large tiles).
+template <int EPI>
+static int gemm_logits(const XPlan &p, int dtype, int kid, bool big, int small, XGemm &g, hipStream_t s) {
+    g.big = big;
+    g.small = small;
+    if (small != 128)
+        if (int rc = gemm<EPI>(p, dtype, kid, 64, g, s)) return rc;
+    if (small != 64)
+        if (int rc = gemm<EPI>(p, dtype, kid, 128, g, s)) return rc;
+    return big ? gemm<EPI>(p, dtype, kid, 256, g, s) : PHC_OK;
 }
 
 template <typename T>
@@ -1314,7 +1336,7 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     g.part_max = w.part_max;
     g.part_sum = w.part_sum;
     g.target_logit = w.target_logit;
-    if (int rc = gemm<XE_STATS>(p, d->dtype, K_XENT_LOGITS, p.big_fwd, p.small_fwd, g, s)) return rc;
+    if (int rc = gemm_logits<XE_STATS>(p, d->dtype, K_XENT_LOGITS, p.big_fwd, p.small_fwd, g, s)) return rc;
     float *loss = d->reduction == PHC_REDUCE_NONE ? d->loss : nullptr;
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_kernel, dim3((unsigned)ceil_div(N, 16)), dim3(1024), 0, s, (const float *)w.part_max, (const float *)w.part_sum,
                   (int)d->V, p.big_fwd ? 1 : 0, p.small_fwd, N, g.count, (const float *)w.target_logit, (const int *)st.rows.from, st.lse, w.row_loss, loss);
@@ -1369,7 +1391,7 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         g.ldd = nvp;
         g.d_scale = d_scale;
         g.db_part = d->db ? w.db_part : nullptr;
-        if (int rc = gemm<XE_DLOGITS>(p, d->dtype, K_XENT_DLOGITS, p.big_d, p.small_d, g, s)) return rc;
+        if (int rc = gemm_logits<XE_DLOGITS>(p, d->dtype, K_XENT_DLOGITS, p.big_d, p.small_d, g, s)) return rc;
         if (d->db) {
             char *db = static_cast<char *>(d->db) + (size_t)v0 * es;
             if (d->dtype == PHC_DTYPE_F32) db_as<float>(w.db_part, st.rows, nv, p.big_d, p.small_d, top, d->dloss, mean, db, s);
@@ -1397,7 +1419,7 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             o.slabs = w.dx_slabs;
             o.accumulate = v0 > 0;
             o.pieces = (int)p.pieces;
-            if (int rc = gemm<XE_DX>(p, d->dtype, K_XENT_DX, p.big_dx, 128, o, s)) return rc;
+            if (int rc = gemm<XE_DX>(p, d->dtype, K_XENT_DX, p.big_dx ? 256 : 128, o, s)) return rc;
         }
         if (d->dW) {
             XGemm q{};
@@ -1416,7 +1438,7 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
             q.ldo = (int)d->D;
             q.slabs = w.dw_slabs;
             q.pieces = 1;
-            if (int rc = gemm<XE_DW>(p, d->dtype, K_XENT_DW, p.big_dw, 128, q, s)) return rc;
+            if (int rc = gemm<XE_DW>(p, d->dtype, K_XENT_DW, p.big_dw ? 256 : 128, q, s)) return rc;
             if ((long long)q.tilesM * q.tilesN * 2 <= q.max_blocks)
                 sum_slabs(d->dtype, K_XENT_DW, w.dw_slabs, q, p.big_dw ? 256 : 128, p.bk, 1, q.out, s);
         }

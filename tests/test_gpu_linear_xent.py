@@ -539,3 +539,18 @@ def test_leaves_of_any_shape_get_gradients_of_theirs():
     p[t[0, 0]] -= 1
     # 16 products and 40 terms in fp32: below 100 roundings of 2^-24 at the size of |p| |w| sums (at most 2 * 5)
     assert float((dv.double() - p @ w.detach().double()).abs().max()) <= 100 * 2.0 ** -24 * 10
+
+
+@pytest.mark.parametrize("kept", [0, 1, 63, 64, 65, 128, 129, 192, 193, 250])
+def test_fp32_rows_that_count_choose_the_tile(kept):
+    """fp32 on its own matrix instructions: the logits' tile size goes by the rows that count, known on the device alone."""
+    n, v, d = 250, 12500, 40
+    x, w, b, t = (q.to(DEV) for q in _case(n, v, d, torch.float32, ignored=0.0, seed=13))
+    gone = torch.randperm(n, generator=torch.Generator().manual_seed(kept))[kept:].to(DEV)
+    t = t.index_fill(0, gone, -100)
+    up = torch.tensor(1.0, device=DEV)
+    exact, bound = _formula(x, w, b, t, "sum", up)
+    for piece in (0, 6300):
+        for what, a, e, m in zip(("loss", "dx", "dW", "db"), _run(x, w, b, t, "sum", up, piece=piece), exact, bound):
+            err = (a.double() - e).abs()
+            assert bool((err <= m).all()), (what, float(err.max()))
