@@ -195,6 +195,15 @@ __device__ __forceinline__ void xt_dma(unsigned lds, const unsigned (&voff)[4], 
         : "memory", "scc");
 }
 
+// one of them, for the lanes that are active
+__device__ __forceinline__ void xt_dma(unsigned lds, unsigned voff, const void *base) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %2, %3\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "s"(lds), "v"(voff), "s"(base)
+                 : "memory");
+}
+
 // (the same in all lanes; hipcc must know it)
 __device__ __forceinline__ const char *uniform(const char *p) {
     const unsigned long long v = reinterpret_cast<unsigned long long>(p);
@@ -246,6 +255,7 @@ struct XGemm {
     const char *A[6], *B[6];       // operand planes of each segment of the k loop
     int segments;                  // 1, or 6 for fp32 inputs
     long long K;                   // valid k (XE_DW: the count of packed rows instead)
+    int kA;                        // the logits: k that A's rows hold, a whole number of 16-byte pieces (B has zeros up to K)
     unsigned lda, ldb;             // row strides in bytes
     int rowsA;                     // valid m
     int rowsB;                     // valid n (where n are the packed rows: at most)
@@ -425,6 +435,12 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 #pragma unroll
             for (int q = 0; q < LOADS; ++q) last[q] = offset(q, kst * BK, rows);
             xt_dma(lds_wave + buf * BUF, last, base);
+        } else if (!A_TR && loads_a && (kst + 1) * BK > a.kA) {              // A's rows end inside the step: zeros behind them
+            for (int q = 0; q < LOADS; ++q) {
+                const int piece = (lane & 7) ^ XSide<T, TM, false, PAIR>::f((dma0 + q) * 8 + (lane >> 3));
+                if (kst * BK + piece * PER < a.kA) xt_dma(lds_wave + buf * BUF + q * 1024, voff[q], base);
+                else *reinterpret_cast<uint4 *>(smem + wave * LOADS * 1024 + buf * BUF + q * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
+            }
         } else {
             xt_dma(lds_wave + buf * BUF, voff, base);
         }
@@ -1078,9 +1094,10 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     p.bk = XT_ROW / p.bytes;
     p.Kp = round_up(d->D, p.bk);
     p.Np = round_up(d->N, XT_BK);
-    // W is read where it lies when its rows are whole steps and 16-byte aligned
-    p.pack_w = p.wide || d->D % p.bk || d->ldw * p.bytes % 16 || !aligned_to(d->W, 16);
-    p.wcols = p.Kp;
+    // W is read where it lies when its rows are whole 16-byte pieces, 16-byte aligned (laid out anew, 192 x 31584 x 3448 bf16 took 163 us forward
+    // and 514 a step instead of 76 and 367)
+    p.pack_w = p.wide || d->D * p.bytes % 16 || d->ldw * p.bytes % 16 || !aligned_to(d->W, 16);
+    p.wcols = p.pack_w ? p.Kp : d->D;
     long long piece = XT_PIECE_BYTES / (p.bytes * p.planes * d->N) / 256 * 256;
     if (piece < 2048) piece = 2048;
     if (d->piece > 0) piece = round_up(d->piece, 64);
@@ -1326,6 +1343,7 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     XGemm g{};
     set_planes(p, W, w.x, &g);
     g.K = p.Kp;
+    g.kA = (int)p.wcols;
     g.lda = (unsigned)(p.pack_w ? p.Kp * p.bytes : d->ldw * es);
     g.ldb = (unsigned)(p.Kp * p.bytes);
     g.rowsA = (int)d->V;
@@ -1377,6 +1395,7 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
         XGemm g{};
         set_planes(p, W, w.x, &g);
         g.K = p.Kp;
+        g.kA = (int)p.wcols;
         g.lda = ldw;
         g.ldb = (unsigned)(p.Kp * p.bytes);
         g.rowsA = nv;

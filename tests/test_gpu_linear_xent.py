@@ -554,3 +554,22 @@ def test_fp32_rows_that_count_choose_the_tile(kept):
         for what, a, e, m in zip(("loss", "dx", "dW", "db"), _run(x, w, b, t, "sum", up, piece=piece), exact, bound):
             err = (a.double() - e).abs()
             assert bool((err <= m).all()), (what, float(err.max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(70, 300, 8), (150, 13000, 72), (300, 1000, 200), (129, 260, 344), (600, 26000, 136)])
+def test_rows_of_w_inside_wider_ones(n, v, d, dtype):
+    """W is read where it lies; what stands behind its rows' ends (NaN here) is not, nor is anything behind its last row."""
+    x, w, b, t = (q.to(DEV) for q in _case(n, v, d, dtype, seed=17))
+    up = torch.tensor(1.0, device=DEV)
+    want = _run(x, w.clone(), b, t, "mean", up)
+    for extra in (8, 64):
+        buf = torch.full((v * (d + extra) - extra,), float("nan"), device=DEV, dtype=dtype)
+        wide = torch.as_strided(buf, (v, d), (d + extra, 1))
+        wide.copy_(w)
+        from phc_gnn_amd import ops
+        xs, bs = x.clone().requires_grad_(), b.clone().requires_grad_()
+        ws = wide.requires_grad_()
+        loss = ops.linear_cross_entropy(xs, ws, t, bs)
+        got = (loss.detach(), *torch.autograd.grad(loss, [xs, ws, bs], up))
+        assert all(torch.equal(a, e) for a, e in zip(got, want)), extra
