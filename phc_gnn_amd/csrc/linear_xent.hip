@@ -670,7 +670,7 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
 
 // ---- a few rows -------------------------------------------------------------------------------------------------------------------------
 // Up to 64 rows (scoring a few tokens): W is read once and everything else is small, so the launch is W's bytes at the memory's rate and
-// latency.  A workgroup takes 64 columns at a time; its four wavefronts share the k and meet in LDS.  W and x go from memory straight into
+// latency.  A workgroup takes 16 FM columns at a time; its four wavefronts share the k and meet in LDS.  W and x go from memory straight into
 // matrix operands: lane (rho, g) loads 16 bytes of row rho at k = g * 16 bytes, the same for both operands, so any order of k inside a step
 // will do.  Two sets of registers: a step is loaded while the one before is multiplied.  fp32 on the fp32 matrix instructions (4 k each).
 // bf16, V = 131072, D = 2048 (537 MB): 1 / 16 / 32 / 64 rows 110 / 119 / 133 / 170 us = 4.9 .. 3.2 TB/s (x comes from L2 for every group, as
@@ -718,49 +718,49 @@ __device__ __forceinline__ frag few_load_part(const T *p, int left) {
     return __builtin_bit_cast(frag, q);
 }
 
-template <typename T, int NF, bool ODD>
+template <typename T, int FM, int NF, bool ODD>
 __global__ __launch_bounds__(256) void xent_few_kernel(XFew a) {
     typedef XFewStep<T> S;
     typedef typename S::frag frag;
-    constexpr int AHEAD = NF > 1 ? 1 : 2;                       // steps of a set of registers
-    __shared__ f32x4_t meet[4][4][64];
-    __shared__ float2 top[4][NF * 16];
+    constexpr int COLS = FM * 16, AHEAD = FM == 1 ? (NF > 2 ? 2 : 4) : NF > 1 ? 1 : 2;                       // steps of a set of registers
+    __shared__ f32x4_t meet[4][FM][64];
+    __shared__ float2 top[FM][NF * 16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
-    int v0 = blockIdx.x * 64;
-    const T *w[4], *x[NF];
+    int v0 = blockIdx.x * COLS;
+    const T *w[FM], *x[NF];
     auto columns = [&]() {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = static_cast<const T *>(a.W) + (long long)min(v0 + i * 16 + fr, a.V - 1) * a.ldw + fg * S::PER;
+        for (int i = 0; i < FM; ++i) w[i] = static_cast<const T *>(a.W) + (long long)min(v0 + i * 16 + fr, a.V - 1) * a.ldw + fg * S::PER;
     };
     columns();
 #pragma unroll
     for (int j = 0; j < NF; ++j) x[j] = static_cast<const T *>(a.x) + (long long)min(j * 16 + fr, a.N - 1) * a.ldx + fg * S::PER;
-    f32x4_t acc[4][NF];
+    f32x4_t acc[FM][NF];
     // a wavefront takes every fourth step; two sets of registers: one is loaded while the other is multiplied
     const int full = a.D / S::K;
-    auto load = [&](frag (&fw)[AHEAD][4], frag (&fx)[AHEAD][NF], int step) {
+    auto load = [&](frag (&fw)[AHEAD][FM], frag (&fx)[AHEAD][NF], int step) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (step + 4 * u >= full) break;
             const long long k = (long long)(step + 4 * u) * S::K;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fw[u][i] = few_load<T, ODD, frag>(w[i] + k);
+            for (int i = 0; i < FM; ++i) fw[u][i] = few_load<T, ODD, frag>(w[i] + k);
 #pragma unroll
             for (int j = 0; j < NF; ++j) fx[u][j] = few_load<T, ODD, frag>(x[j] + k);
         }
     };
-    auto multiply = [&](const frag (&fw)[4], const frag (&fx)[NF]) {
+    auto multiply = [&](const frag (&fw)[FM], const frag (&fx)[NF]) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int j = 0; j < NF; ++j) acc[i][j] = S::mul(fw[i], fx[j], acc[i][j]);
     };
-    auto multiply_all = [&](const frag (&fw)[AHEAD][4], const frag (&fx)[AHEAD][NF], int step) {
+    auto multiply_all = [&](const frag (&fw)[AHEAD][FM], const frag (&fx)[AHEAD][NF], int step) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
             if (step + 4 * u < full) multiply(fw[u], fx[u]);
     };
-    frag fw0[AHEAD][4], fx0[AHEAD][NF], fw1[AHEAD][4], fx1[AHEAD][NF];
+    frag fw0[AHEAD][FM], fx0[AHEAD][NF], fw1[AHEAD][FM], fx1[AHEAD][NF];
     int hit[NF];
 #pragma unroll
     for (int j = 0; j < NF; ++j) {
@@ -771,7 +771,7 @@ __global__ __launch_bounds__(256) void xent_few_kernel(XFew a) {
     load(fw0, fx0, wave);
     while (v0 < a.V) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
             for (int j = 0; j < NF; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
         for (int step = wave; step < full; step += 8 * AHEAD) {
@@ -785,25 +785,26 @@ __global__ __launch_bounds__(256) void xent_few_kernel(XFew a) {
         if (full * S::K < a.D && wave == full % 4) {            // the rest of the rows
             const int left = min(max(a.D - full * S::K - fg * S::PER, 0), S::PER);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fw0[0][i] = few_load_part<T, frag>(w[i] + full * S::K, left);
+            for (int i = 0; i < FM; ++i) fw0[0][i] = few_load_part<T, frag>(w[i] + full * S::K, left);
 #pragma unroll
             for (int j = 0; j < NF; ++j) fx0[0][j] = few_load_part<T, frag>(x[j] + full * S::K, left);
             multiply(fw0[0], fx0[0]);
         }
-        const int first = v0 + wave * 16 + fg * 4;              // this lane's columns of the 64
-        v0 += (int)gridDim.x * 64;
+        const int first = v0 + wave * 16 + fg * 4;              // this lane's columns
+        v0 += (int)gridDim.x * COLS;
         if (v0 < a.V) {                                         // the next ones are under way while these end
             columns();
             load(fw0, fx0, wave);
         }
-        // wavefront w: columns 16 w .. of the 64; a lane holds 4 columns of row fr.  16 rows at a time: LDS for all of them would halve the
+        // wavefront w < FM: columns 16 w ..; a lane holds 4 columns of row fr.  16 rows at a time: LDS for all of them would halve the
         // wavefronts on a CU
 #pragma unroll
         for (int j = 0; j < NF; ++j) {
             __syncthreads();
 #pragma unroll
-            for (int i = 0; i < 4; ++i) meet[wave][i][lane] = acc[i][j];
+            for (int i = 0; i < FM; ++i) meet[wave][i][lane] = acc[i][j];
             __syncthreads();
+            if (wave >= FM) continue;
             f32x4_t l = meet[0][wave][lane];
 #pragma unroll
             for (int q = 1; q < 4; ++q) l += meet[q][wave][lane];
@@ -832,7 +833,7 @@ __global__ __launch_bounds__(256) void xent_few_kernel(XFew a) {
         __syncthreads();
         if (threadIdx.x < NF * 16) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) xt_join(row_max, row_sum, top[q][threadIdx.x].x, top[q][threadIdx.x].y);
+            for (int q = 0; q < FM; ++q) xt_join(row_max, row_sum, top[q][threadIdx.x].x, top[q][threadIdx.x].y);
         }
     }
     if (threadIdx.x < NF * 16) {
@@ -1264,24 +1265,35 @@ static bool few_rows(const phc_linear_xent_desc *d) { return d->N <= XT_FEW; }
 // Workgroups: two on a CU, each with every 512th group of 64 columns (64 rows, V = 100000, D = 1024, bf16: 512, 768, 1024 and one workgroup for
 // each group took 68, 79, 75 and 81 us; fewer parts to join, and the next group's loads run beside a group's end).
 constexpr long long XT_FEW_BLOCKS = 512;
-static long long few_parts(long long V) { return ceil_div(V, 64) < XT_FEW_BLOCKS ? ceil_div(V, 64) : XT_FEW_BLOCKS; }
+// Columns of a group: 64, or 16 where groups of 64 are few (a CU's own rate bounds them), against more reads of x.  fp32 1193 x 2848: 1 row 29 -> 14 us,
+// 64 rows 57 -> 35 us; bf16 5000 x 4096: 1 row 23 -> 17 us, 64 rows 39 -> 48 us.
+static int few_columns(long long V, long long N) { return ceil_div(V, 64) < (N <= 16 ? 128 : 40) ? 16 : 64; }
+static long long few_parts(long long V, long long N) {
+    const long long groups = ceil_div(V, few_columns(V, N));
+    return groups < XT_FEW_BLOCKS ? groups : XT_FEW_BLOCKS;
+}
 
-template <typename T, bool ODD>
+template <typename T, int NF, bool ODD>
 static void launch_few_as(const XFew &f, hipStream_t s) {
-    const dim3 grid((unsigned)few_parts(f.V));
-    if (f.N <= 16) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 1, ODD>), grid, dim3(256), 0, s, f);
-    else if (f.N <= 32) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 2, ODD>), grid, dim3(256), 0, s, f);
-    else PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 4, ODD>), grid, dim3(256), 0, s, f);
+    const dim3 grid((unsigned)few_parts(f.V, f.N));
+    if (few_columns(f.V, f.N) == 16) PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 1, NF, ODD>), grid, dim3(256), 0, s, f);
+    else PHC_LAUNCH_AS(K_XENT_LOGITS, (xent_few_kernel<T, 4, NF, ODD>), grid, dim3(256), 0, s, f);
+}
+template <typename T, bool ODD>
+static void launch_few_rows(const XFew &f, hipStream_t s) {
+    if (f.N <= 16) launch_few_as<T, 1, ODD>(f, s);
+    else if (f.N <= 32) launch_few_as<T, 2, ODD>(f, s);
+    else launch_few_as<T, 4, ODD>(f, s);
 }
 template <typename T>
 static void launch_few(const XFew &f, hipStream_t s) {
     if constexpr (sizeof(T) == 2)
-        if ((f.ldw | f.ldx) & 1 || !aligned_to(f.W, 4) || !aligned_to(f.x, 4)) return launch_few_as<T, true>(f, s);
-    launch_few_as<T, false>(f, s);
+        if ((f.ldw | f.ldx) & 1 || !aligned_to(f.W, 4) || !aligned_to(f.x, 4)) return launch_few_rows<T, true>(f, s);
+    launch_few_rows<T, false>(f, s);
 }
 
 static int forward_few(const phc_linear_xent_desc *d, const XState &st, hipStream_t s) {
-    const int cols = d->N <= 16 ? 16 : d->N <= 32 ? 32 : 64, parts = (int)few_parts(d->V);
+    const int cols = d->N <= 16 ? 16 : d->N <= 32 ? 32 : 64, parts = (int)few_parts(d->V, d->N);
     Carve c(d->ws);
     XFew f{d->W, d->x, d->bias, d->ldw, d->ldx, (int)d->N, (int)d->V, (int)d->D, reinterpret_cast<const long long *>(d->target), d->ignore_index, err_word()};
     f.part_max = c.take<float>((size_t)parts * cols);
@@ -1317,7 +1329,7 @@ size_t phc_linear_xent_state_bytes(int64_t N) { return N < 0 || N > (1 << 22) ? 
 
 size_t phc_linear_xent_ws_bytes(const phc_linear_xent_desc *d, int backward) {
     if (xent_check("phc_linear_xent_ws_bytes", d)) return 0;
-    if (!backward && few_rows(d)) return (size_t)few_parts(d->V) * 64 * 2 * sizeof(float) + 2048;
+    if (!backward && few_rows(d)) return (size_t)few_parts(d->V, d->N) * 64 * 2 * sizeof(float) + 2048;
     return XWs(d, make_plan(d), backward != 0, nullptr).bytes + 256;
 }
 

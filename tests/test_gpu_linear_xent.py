@@ -573,3 +573,10 @@ def test_rows_of_w_inside_wider_ones(n, v, d, dtype):
         loss = ops.linear_cross_entropy(xs, ws, t, bs)
         got = (loss.detach(), *torch.autograd.grad(loss, [xs, ws, bs], up))
         assert all(torch.equal(a, e) for a, e in zip(got, want)), extra
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v,d", [(1, 17, 700), (16, 8128, 40), (16, 8129, 40), (17, 2496, 40), (33, 2497, 40), (64, 15, 600), (64, 1000, 264)])
+def test_few_rows_of_small_vocabularies(n, v, d, dtype):
+    """Groups of 16 columns and of 64, and the sizes where one gives way to the other."""
+    _check(n, v, d, dtype, bias=n % 2 == 1, reduction="none" if n > 16 else "sum", seed=19)
