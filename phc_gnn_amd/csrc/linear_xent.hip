@@ -277,7 +277,7 @@ struct XGemm {
     float *db_part;                // [tilesN * WN][rowsA] or null
     int N;
     // XE_DX / XE_DW
-    const float *top, *dloss;      // g of the products: *top, or (no top) *dloss over the rows that count
+    const float *top, *dloss;      // g of the products: *top (finite), or (no top) *dloss over the rows that count
     int mean;
     float out_scale;
     const int *row_of;             // XE_DX: packed row -> output row
@@ -299,7 +299,7 @@ __host__ __device__ inline int xt_tile(int big, int small, int m, int count) {
     return small ? small : ((count + 63) / 64) % 2 ? 64 : 128;
 }
 
-// what the products of d are multiplied by: the largest |g_i| where the rows of d carry g_i / that, else the one g
+// what the products of d are multiplied by: the largest finite |g_i| where the rows of d carry g_i / that, else the one g
 __device__ __forceinline__ float xt_scale(const float *top, const float *dloss, int mean, int count) {
     if (count <= 0) return 0.f;                                 // (a sum over nothing, whatever its factor)
     if (top) return *top;
@@ -968,23 +968,25 @@ __global__ __launch_bounds__(1024) void xent_reduce_kernel(const float *__restri
     }
 }
 
-// A g_i of its own for every packed row: top = max |g_i|, rel = g_i / top (what the rows of d carry; top goes to the products' outputs)
+// A g_i of its own for every packed row: top = max |g_i| of the finite ones, rel = g_i / top (what the rows of d carry; top goes to the products'
+// outputs).  An infinite or NaN g_i stays in its row of d: as the factor of every output it would reach all rows of dx.
 __global__ __launch_bounds__(1024) void xent_scales_kernel(const float *__restrict__ dloss, const int *__restrict__ count,
                                                           const int *__restrict__ from, float *__restrict__ rel, float *__restrict__ top) {
     __shared__ float red[16];
     const int kept = *count;
     float m = 0.f;
-    for (int i = threadIdx.x; i < kept; i += 1024) m = fmaxf(m, fabsf(dloss[from[i]]));
+    for (int i = threadIdx.x; i < kept; i += 1024) {
+        const float g = fabsf(dloss[from[i]]);
+        if (g < INFINITY) m = fmaxf(m, g);
+    }
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = m;
     __syncthreads();
     for (int w = 0; w < 16; ++w) m = fmaxf(m, red[w]);
+    if (m == 0.f) m = 1.f;
     if (threadIdx.x == 0) *top = m;
-    for (int i = threadIdx.x; i < kept; i += 1024) {
-        const float g = dloss[from[i]];
-        rel[i] = g == 0.f ? 0.f : g / m;
-    }
+    for (int i = threadIdx.x; i < kept; i += 1024) rel[i] = dloss[from[i]] / m;
 }
 
 // The splits' partial outputs in order.  dx: rows go back to their places; dW: nothing to do where one split wrote the result.

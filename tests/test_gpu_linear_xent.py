@@ -580,3 +580,37 @@ def test_rows_of_w_inside_wider_ones(n, v, d, dtype):
 def test_few_rows_of_small_vocabularies(n, v, d, dtype):
     """Groups of 16 columns and of 64, and the sizes where one gives way to the other."""
     _check(n, v, d, dtype, bias=n % 2 == 1, reduction="none" if n > 16 else "sum", seed=19)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [12, 150, 300])
+def test_an_infinite_upstream_gradient_stays_in_its_row(n, dtype):
+    """dx_i = g_i sum_v d_iv w_v: an infinite or NaN g_i leaves the other rows' dx as they are with g_i = 0, to the bit.  dW and db have a
+    term of it in every element."""
+    x, w, b, t = _case(n, 500, 72, dtype, ignored=0.0, seed=23)
+    t[4] = -100
+    g = torch.Generator().manual_seed(24)
+    up = torch.rand(n, generator=g) + 0.5
+    bad = {7: math.inf, 9: -math.inf, 11: math.nan}
+    up[list(bad)] = 0.0
+    want = _run(x, w, b, t, "none", up)
+    exact, bound = _formula(x, w, b, t, "none", up)
+    for a, e, m in zip(want, exact, bound):
+        assert bool(((a.cpu().double() - e).abs() <= m).all())
+    for rows in ([7], [9], [7, 9, 11]):
+        part = up.clone()
+        for i in rows:
+            part[i] = bad[i]
+        part[4] = math.inf                                           # (a row that does not count)
+        loss, dx, dw, db = _run(x, w, b, t, "none", part)
+        rest = torch.ones(n, dtype=torch.bool)
+        rest[rows] = False
+        assert torch.equal(loss, want[0])
+        assert torch.equal(dx.cpu()[rest], want[1].cpu()[rest])
+        assert not bool(dx.cpu()[~rest].isfinite().any())
+        assert not bool(dw.isfinite().any()) and not bool(db.isfinite().any())
+    part = torch.zeros(n)                                            # no other row has a gradient
+    part[7] = math.inf
+    _, dx, dw, _ = _run(x, w, b, t, "none", part)
+    rest = torch.arange(n) != 7
+    assert int(torch.count_nonzero(dx.cpu()[rest])) == 0 and not bool(dx[7].isfinite().any()) and not bool(dw.isfinite().any())
