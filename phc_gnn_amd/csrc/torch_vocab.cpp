@@ -48,7 +48,8 @@ void refuse_twice(const char *who, torch::autograd::variable_list &grads) {
     for (const at::Tensor &g : grads)
         if (g.defined()) known.push_back(g.set_requires_grad(true));
     const auto refusal = std::make_shared<torch::autograd::DelayedError>(
-        std::string(who) + ": its gradient is once_differentiable, second derivatives are not offered", (int64_t)known.size());
+        std::string(who) + ": its gradient is once_differentiable, second derivatives are not offered (detach it where what follows does not require gradients)",
+        (int64_t)known.size());
     known = (*refusal)(std::move(known));
     size_t k = 0;
     for (at::Tensor &g : grads)
@@ -73,7 +74,7 @@ struct Embedding : torch::autograd::Function<Embedding> {
     }
 
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        const bool again = at::GradMode::is_enabled() && grads[0].requires_grad();
+        const bool again = at::GradMode::is_enabled() && grads[0].requires_grad();       // (linear in grads[0], and does not depend on the table)
         at::Tensor dw;
         {
             const at::NoGradGuard no_grad;
@@ -142,7 +143,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     }
 
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx, torch::autograd::variable_list grads) {
-        const bool again = at::GradMode::is_enabled() && grads[0].requires_grad();
+        const bool again = at::GradMode::is_enabled();               // (they depend on x, W and b, one of which asks for gradients, whatever grads[0] does)
         const auto call = ctx->saved_data["call"].toIntVector(), shape = ctx->saved_data["shape"].toIntVector();
         at::Tensor dx, dw, db;
         {

@@ -614,3 +614,30 @@ def test_an_infinite_upstream_gradient_stays_in_its_row(n, dtype):
     _, dx, dw, _ = _run(x, w, b, t, "none", part)
     rest = torch.arange(n) != 7
     assert int(torch.count_nonzero(dx.cpu()[rest])) == 0 and not bool(dx[7].isfinite().any()) and not bool(dw.isfinite().any())
+
+
+def test_a_penalty_on_gradients_is_refused():
+    """The gradients depend on x, weight and bias whatever the upstream gradient is: a second derivative that would leave their terms out is refused,
+    also when the sum has other terms that autograd can go through."""
+    from phc_gnn_amd import ops
+    for n in (5, 90):
+        x, w, b, t = (q.to(DEV) for q in _case(n, 60, 16, torch.float32, ignored=0.0))
+        leaves = [q.requires_grad_() for q in (x, w, b)]
+        plain = torch.autograd.grad(ops.linear_cross_entropy(x, w, t, bias=b), leaves)
+        for k in range(3):
+            loss = ops.linear_cross_entropy(x, w, t, bias=b)
+            grads = torch.autograd.grad(loss, leaves, create_graph=True)
+            assert all(torch.equal(p, q.detach()) for p, q in zip(plain, grads))
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                (loss + grads[k].pow(2).sum()).backward()
+        # only one of them asks for a gradient
+        x1 = x.detach().requires_grad_()
+        loss = ops.linear_cross_entropy(x1, w.detach(), t)
+        (dx,) = torch.autograd.grad(loss, [x1], create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (loss + dx.pow(2).sum()).backward()
+        # a graph that is kept and not used again is no second derivative  (the refused call may have added its first term already)
+        x1.grad = None
+        ops.linear_cross_entropy(x1, w.detach(), t).backward(create_graph=True)
+        assert torch.equal(x1.grad.detach(), dx.detach())
+        x1.grad = None
