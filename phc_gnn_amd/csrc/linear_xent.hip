@@ -1103,7 +1103,7 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     p.wcols = p.pack_w ? p.Kp : d->D;
     long long piece = XT_PIECE_BYTES / (p.bytes * p.planes * d->N) / 256 * 256;
     if (piece < 2048) piece = 2048;
-    if (d->piece > 0) piece = round_up(d->piece, 64);
+    if (d->piece > 0) piece = round_up(d->piece < d->V ? d->piece : d->V, 64);
     if (piece >= d->V) piece = round_up(d->V, 64);
     p.pieces = ceil_div(d->V, piece);
     p.piece = d->piece > 0 ? piece : round_up(ceil_div(d->V, p.pieces), 64);

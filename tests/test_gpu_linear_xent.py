@@ -641,3 +641,13 @@ def test_a_penalty_on_gradients_is_refused():
         ops.linear_cross_entropy(x1, w.detach(), t).backward(create_graph=True)
         assert torch.equal(x1.grad.detach(), dx.detach())
         x1.grad = None
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [50, 150, 300])
+def test_all_columns_as_one_piece(n, dtype):
+    x, w, b, t = _case(n, 513, 96, dtype, seed=3)
+    up = torch.tensor(1.0)
+    want = _run(x, w, b, t, "mean", up, piece=513)
+    for piece in (514, 1 << 40, (1 << 63) - 64, (1 << 63) - 1):
+        assert all(torch.equal(p, q) for p, q in zip(want, _run(x, w, b, t, "mean", up, piece=piece))), piece

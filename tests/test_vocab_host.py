@@ -161,3 +161,18 @@ def test_sizes_beyond_one_launch_are_refused():
     n, d = 1 << 28, (1 << 20) - 1                       # an odd row length: a lane for each column
     need = h.phc_embedding_bwd_ws_bytes(n, 10, d)
     assert h.phc_embedding_bwd(ok, ok, n, 10, d, d, 1, 1.0, -1, ok, ok, need, None) == -2 and b"one launch" in h.phc_last_error()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+def test_pieces_of_more_columns_than_there_are(dtype):
+    """`piece` up to the largest int64 ("all at once") is all the columns: the same scratch, and no size that wrapped around."""
+    lib, h = _lib()
+    for n in (100, 8192):
+        d = _desc(lib, N=n, V=131071, D=96, ldx=96, ldw=96, dtype=dtype, dloss=1 << 20, dx=1 << 20, dW=1 << 20)
+        for backward in (0, 1):
+            d.piece = d.V
+            want = h.phc_linear_xent_ws_bytes(C.byref(d), backward)
+            assert backward == 0 or want >= n * d.V * 2
+            for piece in (d.V + 1, 1 << 22, 1 << 40, (1 << 63) - 65, (1 << 63) - 64, (1 << 63) - 63, (1 << 63) - 1):
+                d.piece = piece
+                assert h.phc_linear_xent_ws_bytes(C.byref(d), backward) == want, piece
