@@ -1240,7 +1240,9 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
  *   256-byte aligned: the rows that count and their logsumexp);
  *   bwd reads that state and dloss (fp32, [N] or one value), and writes whichever of dx [N, D], dW [V, D], db [V]
  *   (dense, of the inputs' type) is not NULL.  Rows that do not count have a zero gradient, whatever x holds there.
- * The backward walks the vocabulary in pieces of `piece` columns (0: as many as half a GiB of scratch holds).
+ * Both walk the vocabulary in pieces.  The forward's: as many columns as half a GiB of scratch holds, 2048 at least (N / 16 bytes a column, and
+ * the column's row of W where W has to be laid out anew: fp32 of more than 256 rows, rows that are not whole 16-byte pieces), `piece` at most where W is
+ * laid out.  The backward's: `piece` columns (0: as many as half a GiB of scratch holds).
  * N, V, ldx, ldw <= 2^22, D <= 2^20, all >= 1.  ws: phc_linear_xent_ws_bytes(desc, backward) bytes, 256-byte aligned, scratch. */
 #define PHC_REDUCE_NONE 0
 #define PHC_REDUCE_SUM 1

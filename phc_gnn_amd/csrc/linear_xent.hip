@@ -466,7 +466,8 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void xent_gemm_kernel(XGemm a) {
     if constexpr (LOGITS) {
         if ((int)threadIdx.x < TN) {
             const int n = tn * TN + threadIdx.x;
-            if (n < count) my_row = Row{a.target[n] - a.first_v, EPI == XE_DLOGITS ? a.lse[n] : 0.f, EPI == XE_DLOGITS && a.rel ? a.rel[n] : 1.f};
+            const int hit = n < count ? a.target[n] - a.first_v : -1;
+            if (n < count) my_row = Row{hit < a.rowsA ? hit : -1, EPI == XE_DLOGITS ? a.lse[n] : 0.f, EPI == XE_DLOGITS && a.rel ? a.rel[n] : 1.f};
         } else if ((int)threadIdx.x < TN + TM) {
             const int m = tm * TM + threadIdx.x - TN;
             my_bias = m >= a.rowsA ? -INFINITY : a.bias ? to_f32(static_cast<const TB *>(a.bias)[m]) : 0.f;     // (columns behind the vocabulary: exp 0)
@@ -912,16 +913,17 @@ __global__ __launch_bounds__(1024) void xent_few_finish_kernel(XFew a, int parts
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------------------------------------
-// A workgroup joins the parts of 16 rows: 64 lane groups share the parts, then one adds them up.
-__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int V, int big, int small, int N,
+// A workgroup joins the parts of 16 rows: 64 lane groups share the parts, then one adds them up.  nv: columns of the piece; `run` carries (maximum, sum)
+// from piece to piece, the last one ends the rows.
+__global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int nv, int big, int small, int N,
                                                         const int *__restrict__ count, const float *__restrict__ target_logit,
-                                                        const int *__restrict__ from, float *__restrict__ lse, float *__restrict__ row_loss,
-                                                        float *__restrict__ loss) {
+                                                        const int *__restrict__ from, float2 *__restrict__ run, int first, int last, float *__restrict__ lse,
+                                                        float *__restrict__ row_loss, float *__restrict__ loss) {
     __shared__ float sm[16][16], ss[16][16];
     const int c = threadIdx.x & 15, group = threadIdx.x >> 4;
     const int n = blockIdx.x * 16 + c, kept = *count;
     if (blockIdx.x * 16 >= kept) return;
-    const int tile = xt_tile(big, small, V, kept), parts = (V + tile - 1) / tile;
+    const int tile = xt_tile(big, small, nv, kept), parts = (nv + tile - 1) / tile;
     float mx = -INFINITY, sum = 0.f;
     if (n < kept)
         for (int p = group; p < parts; p += 64) xt_join(mx, sum, part_max[(size_t)p * N + n], part_sum[(size_t)p * N + n]);
@@ -939,6 +941,11 @@ __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict
 #pragma unroll
     for (int d = 16; d < 64; d <<= 1) xt_join(mx, sum, __shfl_xor(mx, d), __shfl_xor(sum, d));
     if (group == 0 && n < kept) {
+        if (!first) xt_join(mx, sum, run[n].x, run[n].y);
+        if (!last) {
+            run[n] = make_float2(mx, sum);
+            return;
+        }
         const float l = mx + logf(sum);
         lse[n] = l;
         row_loss[n] = l - target_logit[n];
@@ -1068,7 +1075,9 @@ struct Tile64 {
 struct XPlan {
     bool wide;                 // fp32 inputs in three planes
     int planes, segments, bytes, bk;       // bytes of an operand's element, k of a step
-    long long Kp, Np, piece, pieces;
+    long long Kp, Np;
+    long long cols;            // columns of a piece of the forward
+    long long piece, pieces;   // of the backward
     bool pack_w;
     bool big_fwd, big_d;       // 256 x 256 tiles, if enough rows count (known on the device alone)
     int small_fwd, small_d;    // the other tile size, 0: 64 or 128, as xt_tile says
@@ -1101,6 +1110,7 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     // and 514 a step instead of 76 and 367)
     p.pack_w = p.wide || d->D * p.bytes % 16 || d->ldw * p.bytes % 16 || !aligned_to(d->W, 16);
     p.wcols = p.pack_w ? p.Kp : d->D;
+    const long long w_column = p.pack_w ? p.Kp * p.bytes * p.planes : 0;     // bytes of W's layout
     long long piece = XT_PIECE_BYTES / (p.bytes * p.planes * d->N) / 256 * 256;
     if (piece < 2048) piece = 2048;
     if (d->piece > 0) piece = round_up(d->piece < d->V ? d->piece : d->V, 64);
@@ -1108,9 +1118,15 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     p.pieces = ceil_div(d->V, piece);
     p.piece = d->piece > 0 ? piece : round_up(ceil_div(d->V, p.pieces), 64);
     p.pieces = ceil_div(d->V, p.piece);
-    p.big_fwd = p.bytes == 2 && xt_big((int)d->V, (int)d->N);
+    // The forward's pieces are for memory alone too: the row statistics of all tiles (8 bytes for each row and 128 columns) and W's layout
+    p.cols = XT_PIECE_BYTES / (w_column + ceil_div(d->N, 16)) / 256 * 256;
+    if (p.cols < 2048) p.cols = 2048;
+    if (d->piece > 0 && p.pack_w && p.cols > piece) p.cols = piece;
+    if (p.cols >= d->V) p.cols = d->V;
+    else if (d->piece <= 0) p.cols = round_up(ceil_div(d->V, ceil_div(d->V, p.cols)), 256);
+    p.big_fwd = p.bytes == 2 && xt_big((int)p.cols, (int)d->N);
     p.big_d = p.bytes == 2 && xt_big((int)p.piece, (int)d->N);
-    p.small_fwd = small_tile(d->V, d->N, p.bytes == 4);
+    p.small_fwd = small_tile(p.cols, d->N, p.bytes == 4);
     p.small_d = small_tile(p.piece, d->N, p.bytes == 4);
     p.big_dx = p.bytes == 2 && big_split(d->D, d->N);
     p.big_dw = p.bytes == 2 && big_split(d->D, p.piece);
@@ -1144,6 +1160,7 @@ struct XState {
 struct XWs {
     XPlanes x{}, w{}, dl{};
     float *part_max = nullptr, *part_sum = nullptr, *target_logit = nullptr, *row_loss = nullptr;
+    float2 *run = nullptr;
     float *rel = nullptr, *top = nullptr, *dx_slabs = nullptr, *dw_slabs = nullptr, *db_part = nullptr;
     size_t bytes;
     XWs(const phc_linear_xent_desc *d, const XPlan &p, bool backward, void *ws) {
@@ -1152,9 +1169,10 @@ struct XWs {
             for (int i = 0; i < p.planes; ++i) o.p[i] = c.take<char>(count * p.bytes);
         };
         planes(x, (size_t)p.Np * p.Kp);
-        if (p.pack_w) planes(w, (size_t)(backward ? p.piece : d->V) * p.Kp);
+        if (p.pack_w) planes(w, (size_t)(backward ? p.piece : p.cols) * p.Kp);
         if (!backward) {
-            const size_t parts = ceil_div(d->V, p.small_fwd ? p.small_fwd : 64);
+            const size_t parts = ceil_div(p.cols, p.small_fwd ? p.small_fwd : 64);
+            if (p.cols < d->V) run = c.take<float2>(d->N);
             part_max = c.take<float>(parts * d->N);
             part_sum = c.take<float>(parts * d->N);
             target_logit = c.take<float>(d->N);
@@ -1349,30 +1367,36 @@ int phc_linear_xent_fwd(const phc_linear_xent_desc *d, void *stream) {
     PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_that_count_kernel, dim3(1), dim3(1024), 0, s, reinterpret_cast<const long long *>(d->target),
                   (long long)d->ignore_index, N, (long long)d->V, err_word(), st.rows);
     pack(p, d->dtype, d->x, d->ldx, d->N, d->D, &st.rows, nullptr, w.x, s);
-    XPlanes W{{const_cast<void *>(d->W)}};
-    if (p.pack_w) {
-        pack(p, d->dtype, d->W, d->ldw, d->V, d->D, nullptr, nullptr, w.w, s);
-        W = w.w;
-    }
-    XGemm g{};
-    set_planes(p, W, w.x, &g);
-    g.K = p.Kp;
-    g.kA = (int)p.wcols;
-    g.lda = (unsigned)(p.pack_w ? p.Kp * p.bytes : d->ldw * es);
-    g.ldb = (unsigned)(p.Kp * p.bytes);
-    g.rowsA = (int)d->V;
-    g.rowsB = g.N = N;
-    g.count = st.rows.count;
-    g.bias = d->bias;
-    g.target = st.rows.target;
-    g.part_max = w.part_max;
-    g.part_sum = w.part_sum;
-    g.target_logit = w.target_logit;
-    if (int rc = gemm_logits<XE_STATS>(p, d->dtype, K_XENT_LOGITS, p.big_fwd, p.small_fwd, g, s)) return rc;
     float *loss = d->reduction == PHC_REDUCE_NONE ? d->loss : nullptr;
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_kernel, dim3((unsigned)ceil_div(N, 16)), dim3(1024), 0, s, (const float *)w.part_max, (const float *)w.part_sum,
-                  (int)d->V, p.big_fwd ? 1 : 0, p.small_fwd, N, g.count, (const float *)w.target_logit, (const int *)st.rows.from, st.lse, w.row_loss, loss);
-    PHC_LAUNCH_AS(K_XENT_ROWS, xent_reduce_kernel, dim3(1), dim3(1024), 0, s, (const float *)w.row_loss, g.count, (const int *)st.rows.to, N,
+    for (long long v0 = 0; v0 < d->V; v0 += p.cols) {
+        const int nv = (int)(d->V - v0 < p.cols ? d->V - v0 : p.cols);
+        const char *Wv = static_cast<const char *>(d->W) + (size_t)v0 * d->ldw * es;
+        XPlanes W{{const_cast<char *>(Wv)}};
+        if (p.pack_w) {
+            pack(p, d->dtype, Wv, d->ldw, nv, d->D, nullptr, nullptr, w.w, s);
+            W = w.w;
+        }
+        XGemm g{};
+        set_planes(p, W, w.x, &g);
+        g.K = p.Kp;
+        g.kA = (int)p.wcols;
+        g.lda = (unsigned)(p.pack_w ? p.Kp * p.bytes : d->ldw * es);
+        g.ldb = (unsigned)(p.Kp * p.bytes);
+        g.rowsA = nv;
+        g.rowsB = g.N = N;
+        g.count = st.rows.count;
+        g.bias = d->bias ? static_cast<const char *>(d->bias) + (size_t)v0 * es : nullptr;
+        g.target = st.rows.target;
+        g.first_v = (int)v0;
+        g.part_max = w.part_max;
+        g.part_sum = w.part_sum;
+        g.target_logit = w.target_logit;
+        if (int rc = gemm_logits<XE_STATS>(p, d->dtype, K_XENT_LOGITS, p.big_fwd, p.small_fwd, g, s)) return rc;
+        PHC_LAUNCH_AS(K_XENT_ROWS, xent_rows_kernel, dim3((unsigned)ceil_div(N, 16)), dim3(1024), 0, s, (const float *)w.part_max, (const float *)w.part_sum, nv,
+                      p.big_fwd ? 1 : 0, p.small_fwd, N, g.count, (const float *)w.target_logit, (const int *)st.rows.from, w.run, v0 == 0 ? 1 : 0,
+                      v0 + p.cols >= d->V ? 1 : 0, st.lse, w.row_loss, loss);
+    }
+    PHC_LAUNCH_AS(K_XENT_ROWS, xent_reduce_kernel, dim3(1), dim3(1024), 0, s, (const float *)w.row_loss, (const int *)st.rows.count, (const int *)st.rows.to, N,
                   d->reduction == PHC_REDUCE_MEAN ? 1 : 0, loss ? (float *)nullptr : d->loss, loss);
     return launch_status("phc_linear_xent_fwd");
 }

@@ -110,7 +110,7 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     vocabulary.  A target outside [0, V) counts as 0 and is reported by ``phc_gnn_amd.check_indices()``.
 
     The backward computes the logits again, ``piece`` columns of the vocabulary at a time (0: as many as half a GiB of scratch holds; it
-    grows with ``piece``).  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
+    grows with ``piece``).  The forward takes as many as half a GiB holds, and ``piece`` at most where it has to lay W out anew.  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
     dev = L.require_device(x, weight, target, bias)
     _dtype_id("linear_cross_entropy: x", x)
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[0] < 1 or weight.shape[1] < 1 or x.shape[-1] != weight.shape[1]:

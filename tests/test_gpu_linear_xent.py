@@ -651,3 +651,49 @@ def test_all_columns_as_one_piece(n, dtype):
     want = _run(x, w, b, t, "mean", up, piece=513)
     for piece in (514, 1 << 40, (1 << 63) - 64, (1 << 63) - 1):
         assert all(torch.equal(p, q) for p, q in zip(want, _run(x, w, b, t, "mean", up, piece=piece))), piece
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n", [66, 150, 300])
+@pytest.mark.parametrize("piece", [64, 200, 256, 1024])
+def test_forward_in_pieces(piece, n, dtype):
+    """Rows of W that are laid out anew (97 columns; fp32 of 300 rows): the forward's statistics are carried from piece to piece.  Targets in the
+    first and last columns of pieces, whole pieces at -inf, one value that is far above all others in the first or the last piece."""
+    from phc_gnn_amd import ops
+    v = 1300
+    _check(n, v, 97, dtype, bias=n % 4 == 0, reduction=("mean", "sum", "none")[n % 3], piece=piece, seed=29)
+    x, w, b, t = _case(n, v, 97, dtype, ignored=0.1, seed=31)
+    edges = torch.tensor([0, piece - 1, piece, v - 1, v - 2]).clamp(max=v - 1)
+    t[:40] = edges[torch.arange(40) % 5]
+    for at in (None, 0, v - 1):
+        bias = b.clone()
+        bias[piece + 1:min(3 * piece, v - 2)] = -math.inf
+        if at is not None:
+            bias[at] = 60.0
+        keep = bias.isfinite().nonzero()[:, 0]
+        place = torch.full((v,), -1)
+        place[keep] = torch.arange(len(keep))
+        t1 = torch.where((t >= 0) & ~bias.isfinite()[t.clamp(min=0)], torch.zeros_like(t), t)
+        t2 = torch.where(t1 == -100, t1, place[t1.clamp(min=0)])
+        (e, *_), (m, *_) = _formula(x, w[keep], bias[keep], t2, "none", torch.ones(n))
+        got = ops.linear_cross_entropy(x.to(DEV), w.to(DEV), t1.to(DEV), bias=bias.to(DEV), reduction="none", piece=piece)
+        err = (got.cpu().double() - e).abs()
+        assert bool((err <= m).all()), float((err / m).max())
+
+
+def test_forward_scratch_is_what_is_taken():
+    """The memory a forward takes at its peak stays near half a GiB where the statistics or W's layout of the whole vocabulary would take several."""
+    from phc_gnn_amd import ops
+    for n, v, d, dtype, all_at_once in ((1 << 17, 1 << 19, 16, torch.bfloat16, 4 << 30), (300, 131072, 2049, torch.float32, 3 << 29)):
+        x, w = torch.zeros(n, d, device=DEV, dtype=dtype), torch.zeros(v, d, device=DEV, dtype=dtype)
+        t = torch.zeros(n, device=DEV, dtype=torch.int64)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        loss = ops.linear_cross_entropy(x, w, t, reduction="none")
+        torch.cuda.synchronize()
+        taken = torch.cuda.max_memory_allocated() - before
+        assert taken <= (640 << 20) < all_at_once
+        # v equal logits: log v, an exact sum of ones (v is a power of two), one logarithm
+        assert float((loss.double() - math.log(v)).abs().max()) <= 4 * U32 * math.log(v)
+        del x, w, loss

@@ -176,3 +176,25 @@ def test_pieces_of_more_columns_than_there_are(dtype):
             for piece in (d.V + 1, 1 << 22, 1 << 40, (1 << 63) - 65, (1 << 63) - 64, (1 << 63) - 63, (1 << 63) - 1):
                 d.piece = piece
                 assert h.phc_linear_xent_ws_bytes(C.byref(d), backward) == want, piece
+
+
+def _x_copy(n, d, dtype):
+    """x as the products read it: rows and columns rounded up to whole steps; fp32 of more than 256 rows in three 16-bit terms."""
+    wide = dtype == 0 and n > 256
+    size = 6 if wide else 4 if dtype == 0 else 2
+    line = 32 if dtype == 0 and not wide else 64
+    return (n + 63) // 64 * 64 * ((d + line - 1) // line * line) * size
+
+
+@pytest.mark.parametrize("n,v,d,dtype", [(257, 131072, 4096, 0), (1 << 20, 262144, 64, 1), (1 << 22, 1 << 22, 64, 2), (8192, 131072, 2048, 1),
+                                         (300, 131072, 4097, 1), (100, 1 << 22, 1023, 0), (65, 131072, 4097, 2), (1 << 18, 50000, 256, 0), (5, 1 << 22, 4097, 0)])
+def test_linear_xent_forward_scratch_is_bounded(n, v, d, dtype):
+    """Half a GiB for a piece of the vocabulary (its row statistics, its rows of W where they are laid out), and beside it x laid out and a few
+    words for each row.  An explicit piece bounds the layout of W."""
+    lib, h = _lib()
+    beside = _x_copy(n, d, dtype) + n * 16 + 8192
+    q = _desc(lib, N=n, V=v, D=d, ldx=d, ldw=d, dtype=dtype)
+    assert 0 < h.phc_linear_xent_ws_bytes(C.byref(q), 0) <= (512 << 20) + beside
+    q.piece = 2048
+    stats = (v + 63) // 64 * n * 8 if n <= 12288 else 512 << 20
+    assert 0 < h.phc_linear_xent_ws_bytes(C.byref(q), 0) <= min(stats, 512 << 20) + 2048 * ((d + 63) // 64 * 64) * 6 + beside
