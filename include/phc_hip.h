@@ -1240,9 +1240,11 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
  *   256-byte aligned: the rows that count and their logsumexp);
  *   bwd reads that state and dloss (fp32, [N] or one value), and writes whichever of dx [N, D], dW [V, D], db [V]
  *   (dense, of the inputs' type) is not NULL.  Rows that do not count have a zero gradient, whatever x holds there.
- * Both walk the vocabulary in pieces.  The forward's: as many columns as half a GiB of scratch holds, 2048 at least (N / 16 bytes a column, and
- * the column's row of W where W has to be laid out anew: fp32 of more than 256 rows, rows that are not whole 16-byte pieces), `piece` at most where W is
- * laid out.  The backward's: `piece` columns (0: as many as half a GiB of scratch holds).
+ * Both walk the vocabulary in pieces: as many columns as half a GiB of scratch holds, 2048 at least.  A column takes N / 16 bytes in the forward and
+ * N elements of d in the backward (fp32 of more than 256 rows: three times 16 bits), and in both its row of W where W has to be laid out anew:
+ * fp32 of more than 256 rows (three times 16 bits), rows that are not whole 16-byte pieces.  `piece` > 0: that many columns in the backward, and at most
+ * that many in the forward where W is laid out.  Beside a piece: x laid out, and in the backward N / 8 bytes a column for db, dx in fp32 if there are
+ * several pieces, and up to 128 MiB for split products.
  * N, V, ldx, ldw <= 2^22, D <= 2^20, all >= 1.  ws: phc_linear_xent_ws_bytes(desc, backward) bytes, 256-byte aligned, scratch. */
 #define PHC_REDUCE_NONE 0
 #define PHC_REDUCE_SUM 1

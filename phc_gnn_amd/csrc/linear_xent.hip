@@ -1053,8 +1053,8 @@ __global__ __launch_bounds__(256) void xent_db_kernel(const float *__restrict__ 
 static long long round_up(long long v, long long m) { return (v + m - 1) / m * m; }
 static long long ceil_div(long long v, long long m) { return (v + m - 1) / m; }
 
-// A piece's d.  Pieces are for memory alone: at N = 8192, V = 131072, D = 2048 (bf16) pieces of 8192, 16384, 32768 and all columns took 14.4,
-// 14.3, 14.3 and 14.3 ms, smaller ones cost (4096: 15.8 ms).
+// A piece's d, and its rows of W where they are laid out.  Pieces are for memory alone: at N = 8192, V = 131072, D = 2048 (bf16) pieces of 8192,
+// 16384, 32768 and all columns took 14.4, 14.3, 14.3 and 14.3 ms, smaller ones cost (4096: 15.8 ms), so that 2048 columns are the least.
 constexpr long long XT_PIECE_BYTES = 512ll << 20;
 
 // Tiles of 256 x 256 by 8 wavefronts (one workgroup on a CU) or 128 x 128 by 4 (two)
@@ -1111,7 +1111,7 @@ static XPlan make_plan(const phc_linear_xent_desc *d) {
     p.pack_w = p.wide || d->D * p.bytes % 16 || d->ldw * p.bytes % 16 || !aligned_to(d->W, 16);
     p.wcols = p.pack_w ? p.Kp : d->D;
     const long long w_column = p.pack_w ? p.Kp * p.bytes * p.planes : 0;     // bytes of W's layout
-    long long piece = XT_PIECE_BYTES / (p.bytes * p.planes * d->N) / 256 * 256;
+    long long piece = XT_PIECE_BYTES / (p.bytes * p.planes * d->N + w_column) / 256 * 256;
     if (piece < 2048) piece = 2048;
     if (d->piece > 0) piece = round_up(d->piece < d->V ? d->piece : d->V, 64);
     if (piece >= d->V) piece = round_up(d->V, 64);

@@ -109,8 +109,10 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     gradient and stay out of the mean; the mean of no rows is NaN, as for an empty selection.  A bias of -inf takes a column out of the
     vocabulary.  A target outside [0, V) counts as 0 and is reported by ``phc_gnn_amd.check_indices()``.
 
-    The backward computes the logits again, ``piece`` columns of the vocabulary at a time (0: as many as half a GiB of scratch holds; it
-    grows with ``piece``).  The forward takes as many as half a GiB holds, and ``piece`` at most where it has to lay W out anew.  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
+    The backward computes the logits again, ``piece`` columns of the vocabulary at a time (0: as many as half a GiB of scratch holds, 2048 at
+    least; it grows with ``piece``).  The forward takes as many as half a GiB holds, and ``piece`` at most where it has to lay W out anew (fp32 of
+    more than 256 rows, rows that are not whole 16-byte pieces).  Beside a piece lie a copy of ``x`` and, in the backward, ``dx`` in fp32 if there
+    are several pieces and up to 128 MiB for split products.  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
     dev = L.require_device(x, weight, target, bias)
     _dtype_id("linear_cross_entropy: x", x)
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[0] < 1 or weight.shape[1] < 1 or x.shape[-1] != weight.shape[1]:

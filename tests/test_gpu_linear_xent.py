@@ -697,3 +697,15 @@ def test_forward_scratch_is_what_is_taken():
         # v equal logits: log v, an exact sum of ones (v is a power of two), one logarithm
         assert float((loss.double() - math.log(v)).abs().max()) <= 4 * U32 * math.log(v)
         del x, w, loss
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_pieces_that_the_layout_of_w_asks_for(dtype):
+    """Rows of W that are laid out anew and fill the scratch before d does: several pieces in both directions without being asked for."""
+    n, v, d = 300, 131072, 2049
+    x, w, b, t = (q.to(DEV) for q in _case(n, v, d, dtype, seed=43))
+    up = torch.tensor(1.0, device=DEV)
+    exact, bound = _formula(x, w, b, t, "mean", up)
+    for what, a, e, m in zip(("loss", "dx", "dW", "db"), _run(x, w, b, t, "mean", up), exact, bound):
+        err = (a.double() - e).abs()
+        assert bool((err <= m).all()), (what, float(err.max()), float((err / m).max()))

@@ -198,3 +198,20 @@ def test_linear_xent_forward_scratch_is_bounded(n, v, d, dtype):
     q.piece = 2048
     stats = (v + 63) // 64 * n * 8 if n <= 12288 else 512 << 20
     assert 0 < h.phc_linear_xent_ws_bytes(C.byref(q), 0) <= min(stats, 512 << 20) + 2048 * ((d + 63) // 64 * 64) * 6 + beside
+
+
+@pytest.mark.parametrize("n,v,d,dtype", [(257, 131072, 4096, 0), (300, 131072, 4097, 1), (8192, 131072, 2048, 1), (100, 1 << 22, 1023, 0), (3000, 131072, 2050, 2),
+                                         (1, 1 << 22, 4097, 1), (1 << 18, 50000, 256, 0), (1 << 20, 32000, 64, 1)])
+def test_linear_xent_backward_scratch_is_what_is_documented(n, v, d, dtype):
+    """Half a GiB, or 2048 columns, for a piece's d and its rows of W where they are laid out; N / 8 bytes a column (rounded up) for db; x laid out; dx
+    in fp32 if there are several pieces; 128 MiB for split products."""
+    lib, h = _lib()
+    wide = dtype == 0 and n > 256
+    size = 4 if dtype == 0 else 2
+    column = (6 if wide else size) * ((n + 63) // 64 * 64) + ((d + 63) // 64 * 64 * (6 if wide else size) if wide or d * size % 16 else 0)
+    columns = min(v + 63, max(2048, (512 << 20) // column + 256))
+    beside = _x_copy(n, d, dtype) + n * d * 4 + (128 << 20) + ((n + 63) // 64 * 8 + 8) * columns + n * 16 + 16384
+    q = _desc(lib, N=n, V=v, D=d, ldx=d, ldw=d, dtype=dtype, dloss=1 << 20, dx=1 << 20, dW=1 << 20, bias=1 << 20, db=1 << 20)
+    assert 0 < h.phc_linear_xent_ws_bytes(C.byref(q), 1) <= columns * column + beside
+    q.piece = 2048
+    assert 0 < h.phc_linear_xent_ws_bytes(C.byref(q), 1) <= 2048 * column + beside
