@@ -1245,7 +1245,7 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
  * fp32 of more than 256 rows (three times 16 bits), rows that are not whole 16-byte pieces.  `piece` > 0: that many columns in the backward, and at most
  * that many in the forward where W is laid out.  Beside a piece: x laid out, and in the backward N / 8 bytes a column for db, dx in fp32 if there are
  * several pieces, and up to 128 MiB for split products.
- * N, V, ldx, ldw <= 2^22, D <= 2^20, all >= 1.  ws: phc_linear_xent_ws_bytes(desc, backward) bytes, 256-byte aligned, scratch. */
+ * N, V, ldw <= 2^22, D <= 2^20, ldx <= 2^38, all >= 1.  ws: phc_linear_xent_ws_bytes(desc, backward) bytes, 256-byte aligned, scratch. */
 #define PHC_REDUCE_NONE 0
 #define PHC_REDUCE_SUM 1
 #define PHC_REDUCE_MEAN 2

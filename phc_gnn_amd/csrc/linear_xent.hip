@@ -1331,8 +1331,10 @@ static int xent_check(const char *who, const phc_linear_xent_desc *d) {
     PHC_REQUIRE(dtype_bytes(d->dtype), PHC_ERR_INVALID_ARG, "%s: unknown dtype %d", who, d->dtype);
     PHC_REQUIRE(d->reduction >= 0 && d->reduction <= 2, PHC_ERR_INVALID_ARG, "%s: unknown reduction %d", who, d->reduction);
     PHC_REQUIRE(d->N >= 1 && d->V >= 1 && d->D >= 1, PHC_ERR_INVALID_ARG, "%s: N=%lld V=%lld D=%lld", who, (long long)d->N, (long long)d->V, (long long)d->D);
-    PHC_REQUIRE(d->N <= (1 << 22) && d->V <= (1 << 22) && d->D <= (1 << 20) && d->ldx <= (1 << 22) && d->ldw <= (1 << 22), PHC_ERR_UNSUPPORTED,
-                "%s: N=%lld, V=%lld, D=%lld or a row stride is beyond 2^22, 2^22, 2^20, 2^22", who, (long long)d->N, (long long)d->V, (long long)d->D);
+    // (x is read with 64-bit addresses, a tile's rows of W with 32-bit offsets)
+    PHC_REQUIRE(d->N <= (1 << 22) && d->V <= (1 << 22) && d->D <= (1 << 20) && d->ldx <= (1ll << 38) && d->ldw <= (1 << 22), PHC_ERR_UNSUPPORTED,
+                "%s: N=%lld, V=%lld, D=%lld or the row stride of x (%lld) or W (%lld) is beyond 2^22, 2^22, 2^20, 2^38, 2^22", who, (long long)d->N, (long long)d->V,
+                (long long)d->D, (long long)d->ldx, (long long)d->ldw);
     PHC_REQUIRE(d->ldx >= d->D && d->ldw >= d->D, PHC_ERR_INVALID_ARG, "%s: row stride below the row length", who);
     PHC_REQUIRE(d->piece >= 0, PHC_ERR_INVALID_ARG, "%s: piece %lld", who, (long long)d->piece);
     PHC_REQUIRE(d->x && d->W && d->target && d->state && aligned_to(d->state, 256), PHC_ERR_INVALID_ARG, "%s: null pointer, or a state that is not 256-byte aligned", who);

@@ -35,7 +35,7 @@ struct Engine {
 at::Tensor rows(const at::Tensor &t) {
     return t.stride(1) == 1 && (t.stride(0) >= t.size(1) || t.size(0) == 1) ? t : t.contiguous();
 }
-int64_t row_stride(const at::Tensor &t) { return std::max(t.stride(0), t.size(1)); }
+int64_t row_stride(const at::Tensor &t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 const int64_t *words(const at::Tensor &t) { return t.numel() ? t.const_data_ptr<int64_t>() : nullptr; }
 int dtype_id(at::ScalarType t) { return t == at::kFloat ? PHC_DTYPE_F32 : t == at::kBFloat16 ? PHC_DTYPE_BF16 : PHC_DTYPE_F16; }
 
@@ -123,7 +123,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const int64_t N = target.numel(), D = weight.size(1);
         const c10::DeviceGuard guard(x.device());
         const at::TensorOptions f32 = x.options().dtype(at::kFloat), bytes = x.options().dtype(at::kByte);
-        const at::Tensor x2 = rows(x.reshape({N, D})), w = rows(weight), b = bias && bias->defined() ? bias->contiguous() : at::Tensor();
+        at::Tensor w = rows(weight);
+        if (row_stride(w) > (1 << 22)) w = w.contiguous();           // (32-bit offsets inside a tile of rows)
+        const at::Tensor x2 = rows(x.reshape({N, D})), b = bias && bias->defined() ? bias->contiguous() : at::Tensor();
         ctx->saved_data["call"] = std::vector<int64_t>{ignore, reduction, piece, b.defined()};
         ctx->saved_data["shape"] = x.sizes().vec();
         if (N == 0) {

@@ -709,3 +709,29 @@ def test_pieces_that_the_layout_of_w_asks_for(dtype):
     for what, a, e, m in zip(("loss", "dx", "dW", "db"), _run(x, w, b, t, "mean", up), exact, bound):
         err = (a.double() - e).abs()
         assert bool((err <= m).all()), (what, float(err.max()), float((err / m).max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_that_lie_far_apart(dtype):
+    """The last position of long sequences, hidden[:, -1]; a table with rows far apart; a single row of any stride."""
+    from phc_gnn_amd import ops
+    far = (1 << 22) + 24
+    for n, v in ((3, 90), (70, 130)):
+        x, w, b, t = (q.to(DEV) for q in _case(n, v, 64, dtype, seed=37))
+        up = torch.tensor(1.0, device=DEV)
+        want = _run(x, w, b, t, "mean", up)
+        buf = torch.empty((max(n, v) - 1) * far + 64, device=DEV, dtype=dtype)
+        for which in ("x", "w"):
+            src = x if which == "x" else w
+            wide = torch.as_strided(buf, src.shape, (far, 1)).copy_(src).requires_grad_()
+            xs, ws = (wide, w.clone().requires_grad_()) if which == "x" else (x.clone().requires_grad_(), wide)
+            loss = ops.linear_cross_entropy(xs, ws, t, b)
+            got = (loss.detach(), *torch.autograd.grad(loss, [xs, ws]))
+            assert all(torch.equal(p, q) for p, q in zip(got, want)), (n, which)
+        del buf, wide
+    x, w, b, t = (q.to(DEV) for q in _case(5, 1, 64, dtype, ignored=0.0))
+    one = torch.as_strided(w, (1, 64), (1 << 40, 1))
+    assert torch.equal(ops.linear_cross_entropy(x, one, t), ops.linear_cross_entropy(x, w, t))
+    one = torch.as_strided(x, (1, 64), (1 << 40, 1))
+    assert torch.equal(ops.linear_cross_entropy(one, w, t[:1]), ops.linear_cross_entropy(x[:1], w, t[:1]))
+    assert torch.equal(ops.embedding(torch.zeros(2, dtype=torch.int64, device=DEV), torch.as_strided(w, (1, 64), (1 << 40, 1))), w.expand(2, 64))
