@@ -238,20 +238,23 @@ def clip_grads(grads: Sequence[torch.Tensor], max_norm: float, norm_type: float 
                error_if_nonfinite: bool = False) -> Tuple[torch.Tensor, List[torch.Tensor]]:
     """``(norm, results)``: the norm over ``grads`` together, and ``grads`` times ``min(1, max_norm / (norm + 1e-6))`` in new tensors or in
     ``out`` (same shapes, contiguous, fp32 / bf16 / fp16 — e.g. an optimizer's fp32 copies of 16-bit gradients).  ``out`` may be ``grads``
-    themselves; results must share memory neither with each other nor with another gradient."""
-    gs = list(grads)
+    themselves; results must share memory neither with each other nor with another gradient.  ``error_if_nonfinite`` raises before
+    ``out`` is written (one more read of the gradients, and a synchronisation)."""
+    gs, given = list(grads), out is not None
     out = [torch.empty_like(g, memory_format=torch.contiguous_format) for g in gs] if out is None else list(out)
     if len(out) != len(gs):
         raise L.PhcError(f"clip_grads: {len(gs)} gradients, {len(out)} results")
     if not gs:
         return torch.zeros(()), out
+    if error_if_nonfinite and given:
+        _finite_or_raise("clip_grads", grad_norm(gs, norm_type))
     res = _norm_clip("clip_grads", gs, _INTO, max_norm, norm_type, out)
     if res is None:
         for i, (g, o) in enumerate(zip(gs, out)):
             if o.shape != g.shape or not o.is_contiguous():
                 raise L.PhcError(f"clip_grads: result {i} has to be a contiguous tensor of shape {tuple(g.shape)}")
         res = _clip_or_raise("clip_grads", [g.contiguous() for g in gs], _INTO, max_norm, norm_type, out)
-    if error_if_nonfinite:
+    if error_if_nonfinite and not given:
         _finite_or_raise("clip_grads", res[0])
     return res[0], out
 

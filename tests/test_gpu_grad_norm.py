@@ -231,3 +231,23 @@ def test_inference_mode():
         norm, out = optim.clip_grads(g, 1.0)
         again, _ = optim.clip_grads(out, 10.0, out=out)
     assert float(norm) == pytest.approx(68 ** 0.5, rel=2.0 ** -23) and 0.99 < float(again) < 1.01
+
+
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_a_norm_that_is_not_finite_is_raised_before_anything_is_written(bad):
+    from phc_gnn_amd import optim
+    grads = [torch.ones(100, device=DEV), torch.ones(7, device=DEV, dtype=torch.bfloat16)]
+    grads[0][3] = bad
+    kept = [g.clone() for g in grads]
+    for out in (grads, [torch.full((100,), 7.0, device=DEV), torch.full((7,), 7.0, device=DEV)]):
+        before = [o.clone() for o in out]
+        with pytest.raises(RuntimeError, match="total norm"):
+            optim.clip_grads(grads, 1.0, out=out, error_if_nonfinite=True)
+        assert all(torch.equal(o.isnan(), q.isnan()) and torch.equal(o.nan_to_num(), q.nan_to_num()) for o, q in zip(out, before))
+    with pytest.raises(RuntimeError, match="total norm"):
+        optim.clip_grads(grads, 1.0, error_if_nonfinite=True)
+    assert all(torch.equal(g.nan_to_num(), k.nan_to_num()) for g, k in zip(grads, kept))
+    grads[0][3] = 2.0
+    norm, _ = optim.clip_grads(grads, 1.0, out=grads, error_if_nonfinite=True)
+    # 106 ones and one 2: sqrt(110), rounded once
+    assert abs(float(norm) - math.sqrt(110.0)) <= math.sqrt(110.0) * 2.0 ** -23 and float(grads[0][0]) < 1.0
