@@ -735,3 +735,19 @@ def test_rows_that_lie_far_apart(dtype):
     one = torch.as_strided(x, (1, 64), (1 << 40, 1))
     assert torch.equal(ops.linear_cross_entropy(one, w, t[:1]), ops.linear_cross_entropy(x[:1], w, t[:1]))
     assert torch.equal(ops.embedding(torch.zeros(2, dtype=torch.int64, device=DEV), torch.as_strided(w, (1, 64), (1 << 40, 1))), w.expand(2, 64))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ignored", [0.0, 0.85])
+@pytest.mark.parametrize("piece", [0, 1024])
+def test_large_tiles_of_dx_and_dw_with_splits(piece, ignored, dtype):
+    """256 x 256 tiles of both gradient products with their k loops split (7 and 5 ways; more where few rows count), and dx added up over pieces at the
+    same time.  The formula and its bounds on the GPU, in 64 bits."""
+    n, v, d = 2300, 3000, 1024
+    x, w, b, t = (q.to(DEV) for q in _case(n, v, d, dtype, ignored=ignored, seed=47))
+    for reduction in ("mean", "none"):
+        up = torch.tensor(1.0, device=DEV) if reduction == "mean" else torch.rand(n, generator=torch.Generator().manual_seed(3)).to(DEV) - 0.3
+        exact, bound = _formula(x, w, b, t, reduction, up)
+        for what, a, e, m in zip(("loss", "dx", "dW", "db"), _run(x, w, b, t, reduction, up, piece=piece), exact, bound):
+            err = (a.double() - e).abs()
+            assert bool((err <= m).all()), (what, reduction, float(err.max()), float((err / m).max()))
