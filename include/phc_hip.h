@@ -1214,7 +1214,8 @@ int phc_phm_weight_reg(const float *const *W, float *const *dW, const int32_t *n
 
 /* ------------------------------------------------------------------------- *
  * Large vocabularies: lookup, loss, gradient norm.  These take fp32 and 16-bit tensors (PHC_DTYPE_*, one type per call unless a
- * comment says otherwise); sums, statistics and norms are fp32 or fp64 in every case, results are rounded once.  Additions to ABI 8.
+ * comment says otherwise); sums, statistics and norms are fp32 or fp64 in every case.  Results are rounded once; the gradients of the cross
+ * entropy of 16-bit inputs carry one more rounding, of d (below).  Additions to ABI 8.
  * ------------------------------------------------------------------------- */
 #define PHC_DTYPE_F32 0
 #define PHC_DTYPE_BF16 1
@@ -1239,7 +1240,10 @@ int phc_embedding_bwd(const int64_t *tokens, const void *dy, int64_t N, int64_t 
  *   fwd writes loss ([N], or one value for sum and mean; the mean of no rows is NaN) and state (phc_linear_xent_state_bytes(N) bytes,
  *   256-byte aligned: the rows that count and their logsumexp);
  *   bwd reads that state and dloss (fp32, [N] or one value), and writes whichever of dx [N, D], dW [V, D], db [V]
- *   (dense, of the inputs' type) is not NULL.  Rows that do not count have a zero gradient, whatever x holds there.
+ *   (dense, of the inputs' type) is not NULL.  Rows that do not count have a zero gradient, whatever x holds there.  An infinite or NaN dloss of one
+ *   row stays in its row of dx (and reaches all of dW and db, which have a term of it).
+ * 16-bit inputs: d = (softmax - onehot) dloss_i / max |dloss| is rounded to their type before it is multiplied with W and x (sums in fp32, results
+ * rounded).  fp16: what of it is below 2^-28 is rounded to multiples of 2^-38, so that rows of a dloss far below the largest one lose bits.
  * Both walk the vocabulary in pieces: as many columns as half a GiB of scratch holds, 2048 at least.  A column takes N / 16 bytes in the forward and
  * N elements of d in the backward (fp32 of more than 256 rows: three times 16 bits), and in both its row of W where W has to be laid out anew:
  * fp32 of more than 256 rows (three times 16 bits), rows that are not whole 16-byte pieces.  `piece` > 0: that many columns in the backward, and at most

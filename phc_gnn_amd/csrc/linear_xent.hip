@@ -4,9 +4,15 @@
 //   d_iv = exp(l_iv - lse_i) - [v = t_i]       dx_i = g_i sum_v d_iv w_v       dw_v = sum_i g_i d_iv x_i       db_v = sum_i g_i d_iv
 //
 // Forward: ONE product whose tiles never leave the registers: every tile leaves the maximum and the sum of exponentials of its part
-// of a row and, where the target lies in it, the target's logit; a small kernel joins the parts.  Backward keeps only lse: the
-// vocabulary is walked in pieces, a piece's logits are computed again, become d in the tile's registers, and are written once,
-// [row][column], 16 bits (three times 16 for fp32), for the two gradient products.  Four products instead of three, and no N x V tensor.
+// of a row and, where the target lies in it, the target's logit; a small kernel joins the parts.  Backward keeps only lse: a piece's
+// logits are computed again, become d in the tile's registers, and are written once, [row][column], for the two gradient products.  Four
+// products instead of three, and no N x V tensor: both directions walk the vocabulary in pieces.
+//
+// Roundings.  Logits, statistics, losses, d and all sums are fp32.  For 16-bit inputs d g_i / max |g| is ROUNDED to their type, as an operand of
+// the gradient products; two such terms would double two of the four products.  Against 64 bits dx and dW of bf16 are then off by 0.0018 (relative,
+// over all elements) where products of unrounded d give 0.0017, those of fp16 by 0.00032 and 0.00032 (4096 x 32000 x 1024; 1021 x 30011 x 770): the
+// rounding of the results themselves is most of it.  fp32 keeps 24 bits of d in three terms.  The exponentials of 16-bit inputs are the fast ones: for
+// an argument x an error of |x| 2^-24 exp x, below the rounding of d.
 //
 // All products run through one kernel, C[m, n] = sum_k A[m, k] B[n, k], on 16-bit matrix instructions with fp32 accumulators.  An
 // operand lies in memory with k contiguous, or with m (n) contiguous (W in dx; x and d in dW) and is transposed by its LDS reads.  The
@@ -913,6 +919,10 @@ __global__ __launch_bounds__(1024) void xent_few_finish_kernel(XFew a, int parts
 }
 
 // ---- rows -------------------------------------------------------------------------------------------------------------------------------
+// The kernels over all rows that are one workgroup (the numbering above, the sum of the losses, the scales of g) are latency: 5 us each up to some
+// thousand rows.  They count where rows are very many and the vocabulary small: 2^20 rows, 1000 columns of 64 bf16: 0.43, 0.29 - 0.35 and 1.5 ms
+// of 5.0 ms for a step.
+//
 // A workgroup joins the parts of 16 rows: 64 lane groups share the parts, then one adds them up.  nv: columns of the piece; `run` carries (maximum, sum)
 // from piece to piece, the last one ends the rows.
 __global__ __launch_bounds__(1024) void xent_rows_kernel(const float *__restrict__ part_max, const float *__restrict__ part_sum, int nv, int big, int small, int N,
@@ -1092,8 +1102,9 @@ static bool big_split(long long m, long long n) {
 
 static int small_tile(long long m, long long n, bool native) { return ceil_div(m, 128) * ceil_div(n, 128) < 192 ? 64 : native ? 0 : 128; }
 
-// Where the planes' cost (20 bytes of traffic for each element of W, over both directions) equals what they save (8 N products at 130 instead
-// of 200 TFLOP/s): N = 205.
+// Rows up to which fp32 goes without planes.  A step in us without and with them, all rows counting: N = 256: 13565 x 1728 488 and 561, 32000 x 512
+// 337 and 367, 50000 x 1024 993 and 990; N = 128: 285 and 417, 223 and 273, 569 and 770.  With 15 % counting, N = 256: 220 and 446, 166 and 236, 406
+// and 662.  (Planes cost 20 bytes of traffic for each element of W and save 8 N products at 130 instead of 200 TFLOP/s, on tiles of 128 rows.)
 constexpr long long XT_NATIVE = 256;
 
 static XPlan make_plan(const phc_linear_xent_desc *d) {
@@ -1420,7 +1431,8 @@ int phc_linear_xent_bwd(const phc_linear_xent_desc *d, void *stream) {
     if (per_row)
         PHC_LAUNCH_AS(K_XENT_ROWS, xent_scales_kernel, dim3(1), dim3(1024), 0, s, d->dloss, (const int *)st.rows.count, (const int *)st.rows.from, w.rel, w.top);
     pack(p, d->dtype, d->x, d->ldx, d->N, d->D, &st.rows, d->dx, w.x, s);
-    // fp16 has no normal values below 6e-5, where most probabilities of a large vocabulary lie: its d are stored times 2^14
+    // fp16 has no normal values below 6e-5, where most probabilities of a large vocabulary lie: its d are stored times 2^14.  With a g_i for each row
+    // what is below 2^-28 of the largest |g| is then rounded to multiples of 2^-38 of it, in rows of small g_i too.
     const float d_scale = d->dtype == PHC_DTYPE_F16 ? 16384.f : 1.f;
     XGemm o{};                                                   // (the last piece's dx product: its splits are joined at the end)
     for (long long v0 = 0; v0 < d->V; v0 += p.piece) {

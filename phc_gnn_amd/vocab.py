@@ -2,7 +2,7 @@
 (csrc/embedding.hip, csrc/linear_xent.hip).  Exported by ``phc_gnn_amd.ops``.
 
 Unlike the message-passing operators they take fp32, bf16 and fp16 tensors.  Sums, softmax statistics and losses are fp32 in
-every case; gradients come in the type of their input, rounded once.  There is no CPU path."""
+every case; gradients come in the type of their input.  There is no CPU path."""
 from __future__ import annotations
 
 import ctypes as C
@@ -82,8 +82,8 @@ def _call(name: str, dev: torch.device, *args) -> torch.Tensor:
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0, padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * weight[tokens]``: ``weight`` [V, D], ``tokens`` int64 / int32 of any shape -> [*tokens.shape, D] in the weight's type.
 
-    The gradient of ``weight`` is dense, ``scale`` times the sum of the rows' gradients per token in a fixed order (bitwise
-    reproducible), zero in row ``padding_idx``.  A token outside [0, V) reads row 0, counts as 0 in the gradient and is reported by
+    The gradient of ``weight`` is dense, ``scale`` times the sum of the rows' gradients per token in a fixed order (fp32, rounded once;
+    bitwise reproducible), zero in row ``padding_idx``.  A token outside [0, V) reads row 0, counts as 0 in the gradient and is reported by
     ``phc_gnn_amd.check_indices()``, like the encoders' feature values."""
     dev = L.require_device(tokens, weight)
     _dtype_id("embedding: weight", weight)
@@ -112,7 +112,12 @@ def linear_cross_entropy(x: torch.Tensor, weight: torch.Tensor, target: torch.Te
     The backward computes the logits again, ``piece`` columns of the vocabulary at a time (0: as many as half a GiB of scratch holds, 2048 at
     least; it grows with ``piece``).  The forward takes as many as half a GiB holds, and ``piece`` at most where it has to lay W out anew (fp32 of
     more than 256 rows, rows that are not whole 16-byte pieces).  Beside a piece lie a copy of ``x`` and, in the backward, ``dx`` in fp32 if there
-    are several pieces and up to 128 MiB for split products.  fp32 inputs have to be finite; they are multiplied to the accuracy of fp32."""
+    are several pieces and up to 128 MiB for split products.
+
+    fp32 inputs have to be finite; they are multiplied to the accuracy of fp32.  With 16-bit inputs the logits' gradients, over the largest
+    upstream gradient, are rounded to that type before the products with ``weight`` and ``x`` (sums in fp32, results rounded); in fp16 rows whose
+    upstream gradient is far below the largest one lose bits (what is below 2^-28 of it is rounded to multiples of 2^-38).  An infinite or NaN
+    upstream gradient of one row stays in its row of ``dx``.  Second derivatives are refused."""
     dev = L.require_device(x, weight, target, bias)
     _dtype_id("linear_cross_entropy: x", x)
     if weight.dim() != 2 or x.dim() < 1 or weight.shape[0] < 1 or weight.shape[1] < 1 or x.shape[-1] != weight.shape[1]:
