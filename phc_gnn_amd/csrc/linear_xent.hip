@@ -732,7 +732,9 @@ __global__ __launch_bounds__(256) void xent_few_kernel(XFew a) {
     constexpr int COLS = FM * 16, AHEAD = FM == 1 ? (NF > 2 ? 2 : 4) : NF > 1 ? 1 : 2;                       // steps of a set of registers
     __shared__ f32x4_t meet[4][FM][64];
     __shared__ float2 top[FM][NF * 16];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fg = lane >> 4;
+    // (the wavefront's number is the same in all lanes, and hipcc must know it: under a condition that it takes for a lane's it may narrow EXEC and go on,
+    // and the matrix instructions do not look at EXEC)
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), fr = lane & 15, fg = lane >> 4;
     int v0 = blockIdx.x * COLS;
     const T *w[FM], *x[NF];
     auto columns = [&]() {

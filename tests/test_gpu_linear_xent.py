@@ -751,3 +751,16 @@ def test_large_tiles_of_dx_and_dw_with_splits(piece, ignored, dtype):
         for what, a, e, m in zip(("loss", "dx", "dW", "db"), _run(x, w, b, t, reduction, up, piece=piece), exact, bound):
             err = (a.double() - e).abs()
             assert bool((err <= m).all()), (what, reduction, float(err.max()), float((err / m).max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(4, 2180), (16, 900), (20, 1500), (32, 2400), (50, 1000), (5, 20000), (30, 9000), (60, 6000)])
+def test_few_rows_of_many_columns(n, v, dtype):
+    """Rows longer than one round of the k loop, ending at every step of the next: the wavefronts' last rounds are partly empty, each differently."""
+    from phc_gnn_amd import ops
+    x, w, b, t = (q.to(DEV) for q in _case(n, v, 2600, dtype, ignored=0.1, seed=53))
+    for d in (*range(500, 1600, 37), *range(1024, 1600, 32), 1343, 2048, 2065, 2577, 2600):
+        xs, ws = x[:, :d].contiguous(), w[:, :d].contiguous()
+        exact, bound = _formula(xs, ws, b, t, "none", torch.ones(n, device=DEV))
+        err = (ops.linear_cross_entropy(xs, ws, t, b, reduction="none").double() - exact[0]).abs()
+        assert bool((err <= bound[0]).all()), (d, float((err / bound[0]).max()))
