@@ -764,3 +764,34 @@ def test_few_rows_of_many_columns(n, v, dtype):
         exact, bound = _formula(xs, ws, b, t, "none", torch.ones(n, device=DEV))
         err = (ops.linear_cross_entropy(xs, ws, t, b, reduction="none").double() - exact[0]).abs()
         assert bool((err <= bound[0]).all()), (d, float((err / bound[0]).max()))
+
+
+def test_graph_replay_of_a_forward_in_pieces():
+    """Rows of W that are laid out anew, several pieces in both directions, a g for each row, the number of rows that count changing from replay to
+    replay."""
+    from phc_gnn_amd import ops
+    x, w, b, t = (q.to(DEV) for q in _case(200, 1100, 97, torch.bfloat16, seed=61))
+    up = torch.rand(200, device=DEV)
+    x.requires_grad_(), w.requires_grad_(), b.requires_grad_()
+
+    def step():
+        loss = ops.linear_cross_entropy(x, w, t, bias=b, piece=256, reduction="none")
+        return (loss.detach(), *torch.autograd.grad(loss, [x, w, b], up))
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            cap = step()
+    s.synchronize()
+    for k in range(4):
+        with torch.no_grad():
+            x.mul_(1.25)
+            t.copy_(torch.where(torch.arange(200, device=DEV) % 5 == k, torch.full_like(t, -100), torch.roll(t, 3)))
+            up.mul_(-0.5)
+        want = step()
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(cap, want)), k
